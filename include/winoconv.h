@@ -349,6 +349,53 @@ int wc_conv_backward_parameters(const wc_conv_desc* desc, const void* x, const v
 int wc_bias_gradient_workspace_bytes(long long rows, int K, int dtype, size_t* bytes);
 int wc_bias_gradient(const void* dy, void* db, long long rows, int K, int dtype, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/* ---- linear layers ---------------------------------------------------------------------------- */
+/* No counterpart in the reference, whose networks have their 1x1 convolutions and classifiers from torch.  A linear layer over rows of
+ * channels - the pixels of channel-last tensors of all images, or the samples of a batch:
+ *   z = x wT + bias (+ residual)          x (rows, C), w (K, C), bias (K) or null, residual (rows, K) or null
+ *   y = act(z)  (+ residual)              the residual on one side of the activation: before it, or with residual_after behind it
+ * y and, where it is not null, z (rows, K) - what the backward pass wants of a layer with an activation.  All contiguous and of one type,
+ * sums and activations in fp32, one rounding (the activation takes z before its rounding).  gelu: z Phi(z); gelu_tanh: z (1 + tanh(sqrt(2 / pi)
+ * (z + 0.044715 z^3))) / 2; silu: z / (1 + e^-z); gelu and silu of -infinity are 0.  rows = 0: nothing is done.
+ * y and z may not overlap any operand.  Workspace 256-byte aligned. */
+typedef enum { WC_ACT_NONE = 0, WC_ACT_RELU = 1, WC_ACT_GELU = 2, WC_ACT_GELU_TANH = 3, WC_ACT_SILU = 4 } wc_activation;
+typedef struct {
+  long long rows;
+  int C, K;
+  int dtype;
+  int activation;
+  int residual_after;
+} wc_linear_desc;
+int wc_linear_workspace_bytes(const wc_linear_desc* desc, size_t* bytes);
+int wc_linear_forward(const wc_linear_desc* desc, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradients of that layer: dz = dy act'(z), dx = dz w, dw = dzT x, db = the column sums of dz (before dz's rounding).  Those that are null
+ * are not computed; dz is also the gradient of a residual before the activation (of one behind it: dy).  dw and db in the operands' type
+ * or unrounded in fp32.  x and z of the operands' type, or, where their exponents are given, in 8 bits (wc_pack8); for relu anything with
+ * the sign of z does, y among it where no residual was added behind it.  relu's gradient is 0 at z = 0.  w and z may be null where nothing asks for them.  Sums in
+ * fp32 and a fixed order; dz is rounded to the operands' type, which the matrix cores take, before the products.  rows > 0. */
+typedef struct {
+  const void* dy;
+  const void* x; const signed char* x_exponents;
+  const void* w;
+  const void* z; const signed char* z_exponents;
+  void* dx;
+  void* dw; int dw_dtype;
+  void* db; int db_dtype;
+  void* dz;
+} wc_linear_gradients;
+int wc_linear_backward_workspace_bytes(const wc_linear_desc* desc, const wc_linear_gradients* gradients, size_t* bytes);   /* goes by which pointers are null */
+int wc_linear_backward(const wc_linear_desc* desc, const wc_linear_gradients* gradients, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Activations in 8 bits for the backward pass (no counterpart in the reference).  x (rows, C) -> codes (rows, C) and exponents
+ * (rows, ceil(C / 32)): the groups of 32 neighbouring channels of a row share a step 2^e, e = floor(log2(largest magnitude)) - 6 but at least -126;
+ * a value is the whole number nearest to its share of the step, ties to even, at most 127 either way.  It reads as code times 2^e, exact in x's
+ * type.  A group with an infinity or a NaN has the exponent 127 and reads as NaN.  keep_sign: values other than zero have a code other
+ * than zero (a step), for what is read by its sign alone. */
+int wc_pack8(const void* x, signed char* codes, signed char* exponents, long long rows, int C, int dtype, int keep_sign, void* stream);
+int wc_unpack8(const signed char* codes, const signed char* exponents, void* x, long long rows, int C, int dtype, void* stream);
 #ifdef __cplusplus
 }
 #endif

@@ -9,13 +9,15 @@ convolutions, which the Winograd algorithm here does not cover, go to
 torch.nn.functional.conv2d/conv3d on the same device like the reference does (conv.py:326-332).
 There is no CPU path: a CPU tensor, or a missing HIP library, raises.  The transformed filter
 is cached and recomputed only when the weight changes; a graph that is captured without gradients, or of a frozen
-weight, reads the filter as it was then.
+weight, reads the filter as it was then.  checkpoint="int8" keeps the input of a trained layer in 8 bits for its
+weight gradient (checkpoint8): half the memory of 16-bit types, a quarter of fp32.
 """
 import torch
 from torch import nn
 import torch.nn.functional as F
 
 from . import engine, matrix_conv, matrix_conv3d
+from .checkpoint8 import Packed8, pack8, unpack8
 
 
 class Wino:
@@ -49,18 +51,28 @@ class WinoConvFunction(torch.autograd.Function):
 
     # `cast`: (w, bias) in x's type, for parameters that are kept in another one: their gradients come back in theirs, without
     # an autograd node of its own for each cast
+    # `checkpoint`: "int8" keeps x in 8 bits until then (checkpoint8)
     @staticmethod
-    def forward(ctx, x, w, bias, stride, padding, m, U, cast=None):
+    def forward(ctx, x, w, bias, stride, padding, m, U, cast=None, checkpoint=None):
         ctx.types = (w.dtype, None if bias is None else bias.dtype)
         if cast is not None:
             w, bias = cast
-        ctx.save_for_backward(x, w)
+        ctx.packed = checkpoint is not None and ctx.needs_input_grad[1] and x.numel() > 0
+        if ctx.packed:
+            p = pack8(engine.channel_last(x))
+            ctx.save_for_backward(p.codes, w, p.exponents)
+        else:
+            ctx.save_for_backward(x, w)
         ctx.conf = (stride, padding, m, bias is not None)
         return engine.conv_forward(x, w, bias, stride, padding, m, U=U, row=True)
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
+        x, w = ctx.saved_tensors[:2]
+        if ctx.packed:
+            if torch.is_grad_enabled():
+                raise NotImplementedError("WinoConv: a gradient from 8 bits is not differentiable itself")
+            x = engine.channel_first_view(unpack8(Packed8(x, ctx.saved_tensors[2], dy.dtype)))
         stride, padding, m, has_bias = ctx.conf
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         need_db = has_bias and need_db
@@ -70,7 +82,7 @@ class WinoConvFunction(torch.autograd.Function):
             dx, dw, db = engine.conv_backward(x, w, dy, stride, padding, m, need_dx, need_dw, need_db, w_type, b_type or x.dtype)
         rest = gradients(x, w, dy, stride, padding, m, need_dx and dx is None, need_dw and dw is None, need_db and db is None, w_type, b_type)
         dx, dw, db = (a if b is None else b for a, b in zip((dx, dw, db), rest))
-        return dx, dw, db, None, None, None, None, None
+        return dx, dw, db, None, None, None, None, None, None
 
 
 def gradients(x, w, dy, stride, padding, m, need_dx, need_dw, need_db, w_type, b_type):
@@ -92,8 +104,11 @@ class _WinoConvNd(nn.Module):
     nd = 2
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1,
-                 groups=1, bias=True, output_block=None, device=None, dtype=None):
+                 groups=1, bias=True, output_block=None, device=None, dtype=None, checkpoint=None):
         super().__init__()
+        if checkpoint not in (None, "int8"):
+            raise ValueError("checkpoint %r: None or 'int8'" % (checkpoint,))
+        self.checkpoint = checkpoint
         tup = lambda v: (v,) * self.nd if isinstance(v, int) else tuple(v)
         self.in_channels, self.out_channels = in_channels, out_channels
         self.kernel_size, self.stride = tup(kernel_size), tup(stride)
@@ -108,6 +123,8 @@ class _WinoConvNd(nn.Module):
 
     # ((type, the engine's filter_form), its KeptFilter): the filter of the last pass
     _cache = None
+    # "int8": passes with gradients keep their input in 8 bits (files from before there was the choice have none)
+    checkpoint = None
     # (hyperparameters, the compiled host layer's plan for the last input's shape, what _cache has for it, the tile asked for).  Every
     # pass is one of a plan's where there is one, also the first: a plan costs what the call without it works out too.  Copies and files
     # go without.
@@ -181,7 +198,9 @@ class _WinoConvNd(nn.Module):
         return y
 
     def forward(self, x):
-        plan = self._plan if x.is_cuda and engine.USE_EXT else None
+        # (the plans' passes keep their input as it is)
+        plans = engine.USE_EXT and not (self.checkpoint is not None and torch.is_grad_enabled())
+        plan = self._plan if x.is_cuda and plans else None
         if plan is not None and plan[0] != self._conf():
             plan = None
         # weight and bias are read once in a pass: a parametrization runs, and may move on, each time
@@ -199,12 +218,14 @@ class _WinoConvNd(nn.Module):
         if plan is not None and plan[2][0] == x.dtype:
             m = plan[3]
         elif not self._winograd_ok(x):
+            if self.checkpoint is not None:
+                raise NotImplementedError("WinoConv: checkpoint=%r is for layers that the engine runs, and torch runs this one" % (self.checkpoint,))
             conv = F.conv2d if self.nd == 2 else F.conv3d
             return conv(x, weight, bias, self.stride, self.padding, self.dilation, self.groups)
         else:
             m = self._tile_for(x.dtype)
         cache = self._cache
-        if engine.USE_EXT:
+        if plans:
             made = engine.layer_plan(x, weight, self.stride[0], self.padding, m, cache and cache[1])
             if made is not None:
                 y = self._run((self._conf(), made, (x.dtype, made.form), m), x, weight, bias)
@@ -230,7 +251,7 @@ class _WinoConvNd(nn.Module):
         b = bias if bias is None or bias.dtype == x.dtype else bias.detach().to(x.dtype)
         if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
             return WinoConvFunction.apply(x, weight, bias, self.stride[0], self.padding, m, U,
-                                          None if w is weight and b is bias else (w, b))
+                                          None if w is weight and b is bias else (w, b), self.checkpoint)
         return engine.conv_forward(x, w, b, self.stride[0], self.padding, m, U=U, row=True)
 
 

@@ -15,6 +15,7 @@ except ImportError:
     from .backend import AddGPU, Foo, WinoSplit, WinoConcat, DWM, winograd_conv, split_and_concat  # noqa: F401
 from .Add import add_gpu  # noqa: F401
 from .Split_and_Concat import wino_split, wino_concat  # noqa: F401
-from . import dwm, matrix_conv, matrix_conv3d, WinoConv, network, engine  # noqa: F401
+from . import dwm, matrix_conv, matrix_conv3d, matrix_linear, checkpoint8, WinoConv, network, engine  # noqa: F401
 from .WinoConv import Wino, WinoConv2d, WinoConv3d  # noqa: F401
+from .matrix_linear import MatrixLinear  # noqa: F401
 from .network import Dwm  # noqa: F401

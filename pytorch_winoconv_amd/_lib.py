@@ -38,10 +38,22 @@ class ConvDesc(ctypes.Structure):
                 ("direct", ctypes.c_int), ("row", ctypes.c_int)]
 
 
+class LinearDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_longlong), ("C", ctypes.c_int), ("K", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("activation", ctypes.c_int), ("residual_after", ctypes.c_int)]
+
+
+class LinearGradients(ctypes.Structure):
+    _fields_ = [("dy", ctypes.c_void_p), ("x", ctypes.c_void_p), ("x_exponents", ctypes.c_void_p), ("w", ctypes.c_void_p),
+                ("z", ctypes.c_void_p), ("z_exponents", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dw", ctypes.c_void_p),
+                ("dw_dtype", ctypes.c_int), ("db", ctypes.c_void_p), ("db_dtype", ctypes.c_int), ("dz", ctypes.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/winoconv.h declares
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _desc_p, _plan_p = ctypes.POINTER(ConvDesc), ctypes.POINTER(Plan)
 _i64_5 = ctypes.POINTER(ctypes.c_int64)
+_linear_p, _linear_grads_p, _ll = ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearGradients), ctypes.c_longlong
 SIGNATURES = {
     "wc_version": (ctypes.c_char_p, []),
     "wc_last_error": (ctypes.c_char_p, []),
@@ -77,6 +89,12 @@ SIGNATURES = {
     "wc_conv_backward_parameters": (_i, [_desc_p, _vp, _vp, _vp, _i64_5, _i, _vp, _i, _vp, _sz, _vp]),
     "wc_bias_gradient_workspace_bytes": (_i, [ctypes.c_longlong, _i, _i, ctypes.POINTER(_sz)]),
     "wc_bias_gradient": (_i, [_vp, _vp, ctypes.c_longlong, _i, _i, _vp, _sz, _vp]),
+    "wc_linear_workspace_bytes": (_i, [_linear_p, ctypes.POINTER(_sz)]),
+    "wc_linear_forward": (_i, [_linear_p] + [_vp] * 7 + [_sz, _vp]),
+    "wc_linear_backward_workspace_bytes": (_i, [_linear_p, _linear_grads_p, ctypes.POINTER(_sz)]),
+    "wc_linear_backward": (_i, [_linear_p, _linear_grads_p, _vp, _sz, _vp]),
+    "wc_pack8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
+    "wc_unpack8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
 }
 
 _lib = None

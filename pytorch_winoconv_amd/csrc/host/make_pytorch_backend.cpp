@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <limits>
 #include <mutex>
 #include <optional>
 #include <sstream>
@@ -655,6 +656,112 @@ at::Tensor bias_gradient(at::Tensor dy) {
   return db;
 }
 
+// ---- linear layers and activations in 8 bits (matrix_linear.py, checkpoint8.py).  These return None for operands that do not fit together
+// or are not the engine's, which the Python layer then names, and for what it does without a launch.
+using MaybeTensor = std::optional<at::Tensor>;
+
+bool linear_type(const at::Tensor& t) {
+  return t.is_cuda() && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) && t.layout() == at::kStrided;
+}
+bool same_kind(const MaybeTensor& t, const at::Tensor& like) {
+  return !t || (t->scalar_type() == like.scalar_type() && t->device() == like.device() && t->layout() == at::kStrided);
+}
+bool fits(int64_t n) { return n <= std::numeric_limits<int>::max(); }
+MaybeTensor packed_rows(const MaybeTensor& t) { return t ? MaybeTensor(t->contiguous()) : t; }
+const void* data_or_null(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
+
+py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const MaybeTensor& bias_, const MaybeTensor& residual_, int activation, bool residual_after,
+                          bool keep_z) {
+  const int64_t nd = x_.dim();
+  if (!linear_type(x_) || nd < 1 || w_.dim() != 2 || w_.size(1) != x_.size(nd - 1) || x_.numel() == 0 || w_.numel() == 0 || !fits(w_.size(0)) || !fits(w_.size(1)) ||
+      !same_kind(w_, x_) || !same_kind(bias_, x_) || !same_kind(residual_, x_) || (bias_ && (bias_->dim() != 1 || bias_->size(0) != w_.size(0))))
+    return py::none();
+  at::DimVector shape(x_.sizes());
+  shape[nd - 1] = w_.size(0);
+  if (residual_ && residual_->sizes() != at::IntArrayRef(shape)) return py::none();
+  const c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = x_.contiguous(), w = w_.contiguous();
+  const MaybeTensor bias = packed_rows(bias_), residual = packed_rows(residual_);
+  const wc_linear_desc d = {x.numel() / x.size(nd - 1), (int)w.size(1), (int)w.size(0), dtype_of(x), activation, residual_after};
+  at::Tensor y = at::empty(shape, x.options()), z;
+  if (keep_z) z = at::empty(shape, x.options());
+  size_t bytes = 0;
+  check(wc_linear_workspace_bytes(&d, &bytes));
+  void* stream = stream_of(x);
+  at::Tensor ws;
+  if (bytes) ws = workspace_for(x, bytes, stream);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_linear_forward(&d, x.data_ptr(), w.data_ptr(), data_or_null(bias), data_or_null(residual), y.data_ptr(), keep_z ? z.data_ptr() : nullptr,
+                            bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  }
+  return keep_z ? py::object(py::make_tuple(y, z)) : py::cast(y);
+}
+
+// operands that the Python layer has checked; rows > 0
+py::tuple linear_backward(const at::Tensor& dy_, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w_, const MaybeTensor& z, const MaybeTensor& z_exp,
+                          int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, const py::object& w_type, const py::object& b_type) {
+  const c10::DeviceGuard guard(dy_.device());
+  const at::Tensor dy = dy_.contiguous();
+  const MaybeTensor w = packed_rows(w_);
+  const int64_t nd = dy.dim(), K = dy.size(nd - 1);
+  const at::ScalarType wt = torch::python::detail::py_object_to_dtype(w_type), bt = torch::python::detail::py_object_to_dtype(b_type);
+  at::DimVector shape(dy.sizes());
+  shape[nd - 1] = C;
+  at::Tensor dx, dw, db, dz;
+  if (need_dx) dx = at::empty(shape, dy.options());
+  if (need_dw) dw = at::empty({K, C}, dy.options().dtype(wt));
+  if (need_db) db = at::empty({K}, dy.options().dtype(bt));
+  if (need_dz) dz = at::empty(dy.sizes(), dy.options());
+  auto at_or_null = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  auto exps = [](const MaybeTensor& t) { return t ? static_cast<const signed char*>(t->data_ptr()) : nullptr; };
+  const int dtype = dtype_of(dy);
+  const wc_linear_desc d = {dy.numel() / K, C, (int)K, dtype, activation, 0};
+  const wc_linear_gradients g = {dy.data_ptr(), data_or_null(x), exps(x_exp), data_or_null(w), data_or_null(z), exps(z_exp), at_or_null(dx), at_or_null(dw),
+                                 wt == at::kFloat ? WC_F32 : dtype, at_or_null(db), bt == at::kFloat ? WC_F32 : dtype, at_or_null(dz)};
+  size_t bytes = 0;
+  check(wc_linear_backward_workspace_bytes(&d, &g, &bytes));
+  void* stream = stream_of(dy);
+  at::Tensor ws;
+  if (bytes) ws = workspace_for(dy, bytes, stream);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_linear_backward(&d, &g, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  }
+  return py::make_tuple(or_none(dx), or_none(dw), or_none(db), or_none(dz));
+}
+
+py::object pack8(const at::Tensor& x_, bool keep_sign) {
+  const int64_t nd = x_.dim();
+  if (!linear_type(x_) || nd < 1 || x_.numel() == 0 || !fits(x_.size(nd - 1))) return py::none();
+  const c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = x_.contiguous();
+  const int64_t C = x.size(nd - 1);
+  at::DimVector shape(x.sizes());
+  shape[nd - 1] = (C + 31) / 32;
+  at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)), exps = at::empty(shape, x.options().dtype(at::kChar));
+  void* stream = stream_of(x);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_pack8(x.data_ptr(), codes.data_ptr<int8_t>(), exps.data_ptr<int8_t>(), x.numel() / C, (int)C, dtype_of(x), keep_sign, stream));
+  }
+  return py::make_tuple(codes, exps);
+}
+
+// codes and exponents of a Packed8
+py::object unpack8(const at::Tensor& codes, const at::Tensor& exps, const py::object& type) {
+  if (codes.numel() == 0 || !fits(codes.size(-1))) return py::none();
+  const c10::DeviceGuard guard(codes.device());
+  const int64_t C = codes.size(-1);
+  at::Tensor x = at::empty(codes.sizes(), codes.options().dtype(torch::python::detail::py_object_to_dtype(type)));
+  void* stream = stream_of(codes);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_unpack8(codes.data_ptr<int8_t>(), exps.data_ptr<int8_t>(), x.data_ptr(), codes.numel() / C, (int)C, dtype_of(x), stream));
+  }
+  return py::cast(x);
+}
+
 bool channel_last_memory(const at::Tensor& t) {
   std::vector<int64_t> last{0};
   for (int64_t a = 2; a < t.dim(); ++a) last.push_back(a);
@@ -1182,5 +1289,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv_backward_input_strided", &conv_backward_input_strided, py::arg("dy"), py::arg("w"), py::arg("x_spatial"), py::arg("pads"));
   m.def("transform_filter", &transform_filter, py::arg("w"), py::arg("x_shape"), py::arg("stride") = 1, py::arg("padding") = 0, py::arg("m") = 2);
   m.def("bias_gradient", &bias_gradient, py::arg("dy"));
+  m.def("linear_forward", &linear_forward, py::arg("x"), py::arg("w"), py::arg("bias"), py::arg("residual"), py::arg("activation"),
+        py::arg("residual_after"), py::arg("keep_z"));
+  m.def("linear_backward", &linear_backward, py::arg("dy"), py::arg("x"), py::arg("x_exponents"), py::arg("w"), py::arg("z"), py::arg("z_exponents"), py::arg("C"),
+        py::arg("activation"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"), py::arg("need_dz"), py::arg("w_type"), py::arg("b_type"));
+  m.def("pack8", &pack8, py::arg("x"), py::arg("keep_sign"));
+  m.def("unpack8", &unpack8, py::arg("codes"), py::arg("exponents"), py::arg("type"));
   m.def("version", []() { return std::string(wc_version()); });
 }

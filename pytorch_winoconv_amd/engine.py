@@ -31,6 +31,22 @@ def _stream(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+class _on_device:
+    """The current device is t's within, so that launches on its streams find their kernels there."""
+
+    def __init__(self, t):
+        self._index = t.device.index
+
+    def __enter__(self):
+        self._last = torch.cuda.current_device()
+        if self._last != self._index:
+            torch.cuda.set_device(self._index)
+
+    def __exit__(self, *_):
+        if self._last != self._index:
+            torch.cuda.set_device(self._last)
+
+
 def _require_gpu(*tensors):
     for t in tensors:
         if t is None:
