@@ -86,6 +86,10 @@ struct LinearProduct {
 size_t linear_product_bytes(const LinearProduct& p, int dtype);
 int linear_product(const LinearProduct& p, int dtype, void* workspace, void* stream);
 
+// linear_dma.hip: 16-bit products whose rows are multiples of 16 bytes, on tiles of 64 w x 64 w, w = 1, 2 or 4, in s parts
+bool product_dma_fits(const LinearProduct& p, int dtype);
+int product_dma(const LinearProduct& p, int w, int s, long long R_part, float* parts, int dtype, void* stream);
+
 // linear_gradient.hip: dz (rows, K) = dy act'(z), rounded, and db[k] = the sum of column k before that rounding.  z of the storage type, or
 // codes with their exponents; dz null: none, db null: none.  part: scratch
 struct LinearSlope {

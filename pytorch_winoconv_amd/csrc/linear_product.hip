@@ -133,42 +133,57 @@ __global__ __launch_bounds__(256) void product_join_kernel(LinearEpilogue e, con
   finish<T>(e, i / N, i % N, N, v);
 }
 
-// Parts of the reduction: as many as bring four tiles to a compute unit, of 256 elements and more, within 256 MB of sums
-int parts_of(const LinearProduct& p, long long tiles) {
-  long long s = std::min(ceil_div_ll(4 * kCus, std::max(tiles, 1ll)), std::max(p.R / 256, 1ll));
-  s = std::min(s, std::max(1ll, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
-  return (int)std::max(s, 1ll);
+// Tiles of 64 w x 64 w (w = 1: product_general_kernel, too), s parts of the reduction
+struct ProductPlan { bool dma; int w, s; long long R_part; };
+
+ProductPlan plan_of(const LinearProduct& p, bool dma) {
+  ProductPlan l = {dma, 1, 1, 0};
+  auto tiles = [&](int w) { return ceil_div_ll(p.M, 64 * w) * ceil_div_ll(p.N, 64 * w); };
+  if (l.dma) l.w = tiles(4) >= kCus ? 4 : tiles(2) >= kCus / 4 ? 2 : 1;
+  // as many as bring two (w = 2) or four tiles to a compute unit, of 256 elements and more, within 256 MB of sums
+  long long s = l.w == 4 ? 1 : std::min((l.w == 2 ? 2 : 4) * kCus / std::max(tiles(l.w), 1ll), std::max(p.R / 256, 1ll));
+  s = std::max(1ll, std::min(s, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
+  l.R_part = std::max(64ll, ceil_div_ll(ceil_div_ll(p.R, s), 64) * 64);
+  l.s = (int)std::max(1ll, ceil_div_ll(p.R, l.R_part));
+  return l;
 }
 
 bool vectors(const void* p, long long ld, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0; }
 
 }  // namespace
 
+// (where the operands start is not known yet)
 size_t linear_product_bytes(const LinearProduct& p, int) {
-  const int s = parts_of(p, ceil_div_ll(p.M, 64) * ceil_div_ll(p.N, 64));
+  const int s = std::max(plan_of(p, true).s, plan_of(p, false).s);
   return s > 1 ? (size_t)s * p.M * p.N * 4 : 0;
 }
 
 int linear_product(const LinearProduct& p, int dtype, void* workspace, void* stream) {
   const int es = dtype == WC_F32 ? 4 : 2;
-  GeneralArgs g;
-  g.p = p;
-  const long long tiles_m = ceil_div_ll(p.M, 64), tiles_n = ceil_div_ll(p.N, 64);
-  const int s = parts_of(p, tiles_m * tiles_n);
-  if (tiles_m * tiles_n * s >= (1ll << 31) - 8) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
-  g.R_part = ceil_div_ll(ceil_div_ll(p.R, s), 64) * 64;
-  g.parts = s > 1 ? static_cast<float*>(workspace) : nullptr;
-  g.tiles_m = (int)tiles_m; g.tiles_n = (int)tiles_n;
-  g.n_blocks = (int)(tiles_m * tiles_n * s);
-  g.per_xcd = ceil_div(g.n_blocks, kXcds);
-  g.vec_a = vectors(p.a, p.lda, es);
-  g.vec_b = vectors(p.b, p.ldb, es);
+  const ProductPlan l = plan_of(p, product_dma_fits(p, dtype));
+  const long long tiles = ceil_div_ll(p.M, 64 * l.w) * ceil_div_ll(p.N, 64 * l.w);
+  if (tiles * l.s >= (1ll << 31) - 8 || ceil_div_ll(p.M * p.N, 256) >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
+  float* const parts = l.s > 1 ? static_cast<float*>(workspace) : nullptr;
+  if (l.dma) {
+    if (int rc = product_dma(p, l.w, l.s, l.R_part, parts, dtype, stream)) return rc;
+  }
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    hipLaunchKernelGGL(product_general_kernel<T>, dim3((unsigned)(g.per_xcd * kXcds)), dim3(256), 0, as_stream(stream), g);
-    WC_CHECK_LAUNCH("product_general_kernel");
-    if (s > 1) {
-      hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_ll(p.M * p.N, 256)), dim3(256), 0, as_stream(stream), p.e, g.parts, s, p.M, p.N);
+    if (!l.dma) {
+      GeneralArgs g;
+      g.p = p;
+      g.parts = parts;
+      g.R_part = l.R_part;
+      g.tiles_m = (int)ceil_div_ll(p.M, 64); g.tiles_n = (int)ceil_div_ll(p.N, 64);
+      g.n_blocks = (int)(tiles * l.s);
+      g.per_xcd = ceil_div(g.n_blocks, kXcds);
+      g.vec_a = vectors(p.a, p.lda, es);
+      g.vec_b = vectors(p.b, p.ldb, es);
+      hipLaunchKernelGGL(product_general_kernel<T>, dim3((unsigned)(g.per_xcd * kXcds)), dim3(256), 0, as_stream(stream), g);
+      WC_CHECK_LAUNCH("product_general_kernel");
+    }
+    if (parts) {
+      hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_ll(p.M * p.N, 256)), dim3(256), 0, as_stream(stream), p.e, parts, l.s, p.M, p.N);
       WC_CHECK_LAUNCH("product_join_kernel");
     }
     return WC_OK;

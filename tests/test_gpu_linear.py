@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 # rows, C, K: one of everything, odd, around tiles and stages, long reductions, few and many rows
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 31, 65), (8, 64, 64), (16, 512, 40), (33, 40, 72), (64, 64, 64), (65, 33, 17), (130, 257, 96), (200, 72, 264), (7, 1000, 3),
-          (513, 16, 300), (257, 136, 520), (1, 4096, 24), (5, 2056, 1000), (17, 3000, 128), (1025, 8, 8), (300, 300, 301)]
+          (513, 16, 300), (257, 136, 520), (1, 4096, 24), (5, 2056, 1000), (17, 3000, 128), (1025, 8, 8), (300, 300, 301), (1000, 520, 776),
+          (2000, 96, 640)]
 
 
 def _inputs(rows, C, K, t, seed, bias=True):
@@ -79,6 +80,26 @@ def test_gradients_from_8_bits(dev, shape, t):
         got = matrix_linear.linear_backward(dy.cuda(), P[0], w.cuda(), P[1], act, need_dz=True)
         for k, v in zip(("dx", "dw", "db", "dz"), got):
             lo.within(v, *want[k], "%s %s" % (k, act))
+
+
+@pytest.mark.parametrize("t", lo.TYPES[1:], ids=str)
+@pytest.mark.parametrize("deep", [8, 40, 64, 96, 136])
+def test_many_results(dev, t, deep):
+    """Products of so many results that they take the largest tiles, the last of them ragged, over few to some stages of the reduction."""
+    x, w, b, r, _ = _inputs(4090, deep, 4104, t, deep)
+    y, z, by, bz = lo.forward(x, w, b, r, "gelu", True)
+    got = matrix_linear.linear_forward(*_cuda(x, w, b, r), "gelu", True, True)
+    lo.within(got[0], y, by, "y")
+    lo.within(got[1], z, bz, "z")
+    x, w, _, _, dy = _inputs(4106, 4104, deep, t, deep)
+    dx = matrix_linear.linear_backward(dy.cuda(), None, w.cuda(), need_dw=False, need_db=False)[0]
+    DY, W = dy.double(), w.double()
+    lo.within(dx, DY @ W, lo.half_step(t) * (DY @ W).abs() + 2 * (deep + 8) * lo.SUM * (DY.abs() @ W.abs()) + lo.least(t), "dx")
+    x, _, _, _, dy = _inputs(deep + 3, 4096, 4112, t, deep)
+    X, DY = x.double(), dy.double()
+    for wide in (t, torch.float32):
+        dw = matrix_linear.linear_backward(dy.cuda(), x.cuda(), None, need_dx=False, need_db=False, w_type=wide)[1]
+        lo.within(dw, DY.t() @ X, lo.half_step(wide) * (DY.t() @ X).abs() + 2 * (deep + 11) * lo.SUM * (DY.abs().t() @ X.abs()) + lo.least(wide), "dw")
 
 
 @pytest.mark.parametrize("t", lo.TYPES, ids=str)
