@@ -667,7 +667,12 @@ bool same_kind(const MaybeTensor& t, const at::Tensor& like) {
   return !t || (t->scalar_type() == like.scalar_type() && t->device() == like.device() && t->layout() == at::kStrided);
 }
 bool fits(int64_t n) { return n <= std::numeric_limits<int>::max(); }
-MaybeTensor packed_rows(const MaybeTensor& t) { return t ? MaybeTensor(t->contiguous()) : t; }
+// contiguous, and starting where 16-byte loads may
+at::Tensor packed_rows(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+MaybeTensor packed_rows(const MaybeTensor& t) { return t ? MaybeTensor(packed_rows(*t)) : t; }
 const void* data_or_null(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 
 py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const MaybeTensor& bias_, const MaybeTensor& residual_, int activation, bool residual_after,
@@ -680,7 +685,7 @@ py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const Mayb
   shape[nd - 1] = w_.size(0);
   if (residual_ && residual_->sizes() != at::IntArrayRef(shape)) return py::none();
   const c10::DeviceGuard guard(x_.device());
-  const at::Tensor x = x_.contiguous(), w = w_.contiguous();
+  const at::Tensor x = packed_rows(x_), w = packed_rows(w_);
   const MaybeTensor bias = packed_rows(bias_), residual = packed_rows(residual_);
   const wc_linear_desc d = {x.numel() / x.size(nd - 1), (int)w.size(1), (int)w.size(0), dtype_of(x), activation, residual_after};
   at::Tensor y = at::empty(shape, x.options()), z;
@@ -702,7 +707,7 @@ py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const Mayb
 py::tuple linear_backward(const at::Tensor& dy_, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w_, const MaybeTensor& z, const MaybeTensor& z_exp,
                           int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, const py::object& w_type, const py::object& b_type) {
   const c10::DeviceGuard guard(dy_.device());
-  const at::Tensor dy = dy_.contiguous();
+  const at::Tensor dy = packed_rows(dy_);
   const MaybeTensor w = packed_rows(w_);
   const int64_t nd = dy.dim(), K = dy.size(nd - 1);
   const at::ScalarType wt = torch::python::detail::py_object_to_dtype(w_type), bt = torch::python::detail::py_object_to_dtype(b_type);

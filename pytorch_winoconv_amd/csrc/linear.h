@@ -82,24 +82,48 @@ struct LinearProduct {
   long long M, N, R;
   LinearEpilogue e;
 };
-// linear_product.hip: bytes of scratch (sums of the parts of the reduction), and the launches
-size_t linear_product_bytes(const LinearProduct& p, int dtype);
-int linear_product(const LinearProduct& p, int dtype, void* workspace, void* stream);
+// linear_product.hip: how a product is run - on which kernel and tiles, in how many parts of the reduction - and the launches.  Parts leave
+// their sums (s, M, N) in fp32, which linear_join adds.
+struct ProductTile { int m, n; };
+struct ProductPlan { bool dma; ProductTile tile; int s; long long R_part; };
+ProductPlan product_plan(const LinearProduct& p, int dtype);
+size_t product_parts_bytes(const LinearProduct& p, int dtype);      // whatever the operands' start
+int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream);
+// both, in one launch where their plans allow it
+int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream);
 
-// linear_dma.hip: 16-bit products whose rows are multiples of 16 bytes, on tiles of 64 w x 64 w, w = 1, 2 or 4, in s parts
+// linear_dma.hip: products whose rows are multiples of 16 bytes, on tiles of 256 x 256, 256 x 128 (16-bit types), 128 x 128 or 64 x 64
 bool product_dma_fits(const LinearProduct& p, int dtype);
-int product_dma(const LinearProduct& p, int w, int s, long long R_part, float* parts, int dtype, void* stream);
+int product_dma(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream);
+bool product_dma_pairs(const ProductPlan& plan, const ProductPlan& plan2);
+int product_dma_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream);
 
-// linear_gradient.hip: dz (rows, K) = dy act'(z), rounded, and db[k] = the sum of column k before that rounding.  z of the storage type, or
-// codes with their exponents; dz null: none, db null: none.  part: scratch
+// Matrices copied to rows that are multiples of 16 bytes, zeros behind their columns
+struct WideCopy { const void* from; void* to; long long rows, C, ld; };
+// dz (rows, K) = dy act'(z), rounded, and db[k] = the sum of column k before that rounding.  z of the storage type, or codes with their
+// exponents; dz null: none, db null: none
 struct LinearSlope {
   const void* dy; const void* z; const signed char* z_exp;
   void* dz; void* db;
+  void* dz_wide; long long ld_wide;      // dz in rows of ld_wide (a multiple of 16 bytes), zeros behind K; null: none
   int act, db_f32;
   long long rows; int K;
 };
-size_t linear_slope_bytes(const LinearSlope& s, int dtype);
-int linear_slope(const LinearSlope& s, int dtype, void* part, void* stream);
+// linear_gradient.hip: what stands before the products, in one launch: dz, copies, 8 bits read back (codes null: none) to rows of x_ld
+struct LinearPrepare {
+  bool run_slope;
+  LinearSlope slope;
+  WideCopy copies[2];
+  int n_copies;
+  const signed char* codes; const signed char* exps;
+  void* x;
+  long long x_rows, x_ld; int x_C;
+};
+size_t linear_sums_bytes(const LinearSlope& s);                     // of the columns' sums; 0: the first launch writes db itself
+int linear_prepare(const LinearPrepare& p, int dtype, float* sums, void* stream);
+// ... and behind them, in one launch: the parts of up to two products (s of 1: none) and the columns' sums (sums null: none)
+struct LinearJoin { LinearEpilogue e; const float* parts; int s; long long M, N; };
+int linear_join(const LinearJoin* joins, int n, const LinearSlope* slope, const float* sums, int dtype, void* stream);
 
 // pack8.hip
 constexpr int kPackGroup = 32;
@@ -111,5 +135,6 @@ __device__ __forceinline__ float pack_step(int e) {
 }
 int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, bool keep_sign, int dtype, void* stream);
 int unpack8(const signed char* codes, const signed char* exps, void* x, long long rows, int C, int dtype, void* stream);
+inline long long wide_row(long long C, int dtype) { const int epc = dtype == WC_F32 ? 4 : 8; return (C + epc - 1) / epc * epc; }
 
 }  // namespace wc

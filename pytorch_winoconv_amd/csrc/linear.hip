@@ -7,6 +7,8 @@ using namespace wc;
 
 namespace {
 
+constexpr double kWidenPays = 1e8;      // multiplications
+
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 bool known(int dtype) { return dtype == WC_F32 || dtype == WC_F16 || dtype == WC_BF16; }
 int size_of(int dtype) { return dtype == WC_F32 ? 4 : 2; }
@@ -33,49 +35,93 @@ int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
   return WC_OK;
 }
 
-LinearProduct forward_product(const wc_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z) {
-  return {x, w, d->C, d->C, false, false, d->rows, d->K, d->C, {bias, res, y, z, d->activation, d->residual_after != 0, 0}};
+// Rows that are no multiple of 16 bytes are copied to ones that are, for the kernel that brings them to LDS without registers, where the product is
+// worth it: the copy is a launch and a pass over the operands.
+bool widen_pays(long long M, long long N, long long R) { return (double)M * N * R >= kWidenPays; }
+
+struct Forward {
+  LinearProduct p;
+  WideCopy copies[2];
+  bool widen;
+  size_t scratch_at, bytes;
+};
+
+Forward forward_plan(const wc_linear_desc* d, const void* x, const void* w, const void* bias, const void* res, void* y, void* z, char* ws) {
+  Forward f;
+  const long long ld = wide_row(d->C, d->dtype);
+  const size_t es = size_of(d->dtype);
+  size_t at = 0;
+  f.widen = ld != d->C && widen_pays(d->rows, d->K, d->C);
+  if (f.widen) {
+    f.copies[0] = {x, ws, d->rows, d->C, ld};
+    at = rounded((size_t)d->rows * ld * es);
+    f.copies[1] = {w, ws + at, d->K, d->C, ld};
+    at += rounded((size_t)d->K * ld * es);
+    x = f.copies[0].to;
+    w = f.copies[1].to;
+  }
+  f.p = {x, w, f.widen ? ld : d->C, f.widen ? ld : d->C, false, false, d->rows, d->K, d->C, {bias, res, y, z, d->activation, d->residual_after != 0, 0}};
+  f.scratch_at = at;
+  f.bytes = at + rounded(product_parts_bytes(f.p, d->dtype));
+  return f;
 }
 
 // What a backward pass launches, and where its scratch lies
 struct Backward {
-  LinearSlope slope;
+  LinearPrepare before;
   LinearProduct dx, dw;
-  bool run_slope, unpack_x;
-  size_t dz_at, x_at, scratch_at, bytes;
+  size_t sums_at, dx_at, dw_at, bytes;
 };
 
 Backward backward_plan(const wc_linear_desc* d, const wc_linear_gradients* g, char* ws) {
-  Backward b;
+  Backward b = {};
   const size_t es = size_of(d->dtype);
-  const bool acts = d->activation != WC_ACT_NONE;
+  const bool acts = d->activation != WC_ACT_NONE, products = g->dx || g->dw;
+  // (either product reads what the other does, so they are widened together)
+  const long long ldc = wide_row(d->C, d->dtype), ldk = wide_row(d->K, d->dtype);
+  const bool widen = products && widen_pays(d->rows, d->K, d->C), wide_c = widen && ldc != d->C, wide_k = widen && ldk != d->K;
   size_t at = 0;
+  auto take = [&](size_t n) { void* const p = ws + at; at += rounded(n); return p; };
+  LinearPrepare& f = b.before;
   const void* dz = g->dy;
-  void* dz_out = nullptr;
-  b.dz_at = at;
-  if (acts && (g->dx || g->dw || g->dz)) {
-    dz_out = g->dz ? g->dz : ws + at;
+  void *dz_out = g->dz, *dz_wide = nullptr;       // without an activation: copies of dy
+  long long ld_dz = d->K;
+  if (products && wide_k) {
+    dz = dz_wide = take((size_t)d->rows * ldk * es);
+    ld_dz = ldk;
+  } else if (products && acts) {
+    if (!dz_out) dz_out = take((size_t)d->rows * d->K * es);
     dz = dz_out;
-    if (!g->dz) at += rounded((size_t)d->rows * d->K * es);
-  } else if (!acts) {
-    dz_out = g->dz;                              // a copy of dy
   }
-  b.unpack_x = g->dw && g->x_exponents;
-  b.x_at = at;
-  const void* x = g->x;
-  if (b.unpack_x) {
-    x = ws + at;
-    at += rounded((size_t)d->rows * d->C * es);
+  const long long ld = wide_c ? ldc : d->C;
+  const void *w = g->w, *x = g->x;
+  if (g->dx && wide_c) {
+    f.copies[f.n_copies++] = {w, take((size_t)d->K * ldc * es), d->K, d->C, ldc};
+    w = f.copies[0].to;
   }
-  b.scratch_at = at;
-  b.run_slope = dz_out || g->db;
-  b.slope = {g->dy, acts ? g->z : nullptr, acts ? g->z_exponents : nullptr, dz_out, g->db, d->activation, g->db_dtype == WC_F32, d->rows, d->K};
-  b.dx = {dz, g->w, d->K, d->C, false, true, d->rows, d->C, d->K, {nullptr, nullptr, g->dx, nullptr, WC_ACT_NONE, 0, 0}};
-  b.dw = {dz, x, d->K, d->C, true, true, d->K, d->C, d->rows, {nullptr, nullptr, g->dw, nullptr, WC_ACT_NONE, 0, g->dw_dtype == WC_F32}};
-  size_t scratch = b.run_slope ? linear_slope_bytes(b.slope, d->dtype) : 0;
-  if (g->dx) scratch = std::max(scratch, linear_product_bytes(b.dx, d->dtype));
-  if (g->dw) scratch = std::max(scratch, linear_product_bytes(b.dw, d->dtype));
-  b.bytes = at + rounded(scratch);
+  if (g->dw && (g->x_exponents || wide_c)) {
+    void* const to = take((size_t)d->rows * ld * es);
+    if (g->x_exponents) {
+      f.codes = static_cast<const signed char*>(g->x);
+      f.exps = g->x_exponents;
+      f.x = to;
+      f.x_rows = d->rows; f.x_ld = ld; f.x_C = d->C;
+    } else {
+      f.copies[f.n_copies++] = {x, to, d->rows, d->C, ldc};
+    }
+    x = to;
+  }
+  f.run_slope = dz_out || dz_wide || g->db;
+  f.slope = {g->dy, acts ? g->z : nullptr, acts ? g->z_exponents : nullptr, dz_out, g->db, dz_wide, ldk, d->activation, g->db_dtype == WC_F32, d->rows, d->K};
+  b.dx = {dz, w, ld_dz, ld, false, true, d->rows, d->C, d->K, {nullptr, nullptr, g->dx, nullptr, WC_ACT_NONE, 0, 0}};
+  b.dw = {dz, x, ld_dz, ld, true, true, d->K, d->C, d->rows, {nullptr, nullptr, g->dw, nullptr, WC_ACT_NONE, 0, g->dw_dtype == WC_F32}};
+  b.sums_at = at;
+  at += rounded(linear_sums_bytes(f.slope));
+  b.dx_at = at;
+  if (g->dx) at += rounded(product_parts_bytes(b.dx, d->dtype));
+  b.dw_at = at;
+  if (g->dw) at += rounded(product_parts_bytes(b.dw, d->dtype));
+  b.bytes = at;
   return b;
 }
 
@@ -86,7 +132,7 @@ extern "C" {
 int wc_linear_workspace_bytes(const wc_linear_desc* d, size_t* bytes) {
   WC_CHECK_ARG(bytes != nullptr, "wc_linear_workspace_bytes: null output");
   if (int rc = check_desc(d, "wc_linear_workspace_bytes")) return rc;
-  *bytes = d->rows == 0 ? 0 : linear_product_bytes(forward_product(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr), d->dtype);
+  *bytes = d->rows == 0 ? 0 : forward_plan(d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr).bytes;
   return WC_OK;
 }
 
@@ -97,7 +143,20 @@ int wc_linear_forward(const wc_linear_desc* d, const void* x, const void* w, con
   if (d->rows == 0) return WC_OK;
   WC_CHECK_ARG(x && w && y, "wc_linear_forward: null pointer");
   if (int rc = check_workspace(workspace, workspace_bytes, need, "wc_linear_forward")) return rc;
-  return linear_product(forward_product(d, x, w, bias, residual, y, z), d->dtype, workspace, stream);
+  char* const ws = static_cast<char*>(workspace);
+  const Forward f = forward_plan(d, x, w, bias, residual, y, z, ws);
+  if (f.widen) {
+    LinearPrepare before = {};
+    before.copies[0] = f.copies[0];
+    before.copies[1] = f.copies[1];
+    before.n_copies = 2;
+    if (int rc = linear_prepare(before, d->dtype, nullptr, stream)) return rc;
+  }
+  float* const parts = reinterpret_cast<float*>(ws + f.scratch_at);
+  const ProductPlan plan = product_plan(f.p, d->dtype);
+  if (int rc = product_run(f.p, plan, parts, d->dtype, stream)) return rc;
+  const LinearJoin join = {f.p.e, parts, plan.s, f.p.M, f.p.N};
+  return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
 }
 
 int wc_linear_backward_workspace_bytes(const wc_linear_desc* d, const wc_linear_gradients* g, size_t* bytes) {
@@ -120,15 +179,19 @@ int wc_linear_backward(const wc_linear_desc* d, const wc_linear_gradients* g, vo
   if (int rc = check_workspace(workspace, workspace_bytes, need, "wc_linear_backward")) return rc;
   char* const ws = static_cast<char*>(workspace);
   const Backward b = backward_plan(d, g, ws);
-  void* const scratch = ws + b.scratch_at;
-  if (b.run_slope)
-    if (int rc = linear_slope(b.slope, d->dtype, scratch, stream)) return rc;
-  if (g->dx)
-    if (int rc = linear_product(b.dx, d->dtype, scratch, stream)) return rc;
-  if (!g->dw) return WC_OK;
-  if (b.unpack_x)
-    if (int rc = unpack8(static_cast<const signed char*>(g->x), g->x_exponents, ws + b.x_at, d->rows, d->C, d->dtype, stream)) return rc;
-  return linear_product(b.dw, d->dtype, scratch, stream);
+  auto at = [&](size_t n) { return reinterpret_cast<float*>(ws + n); };
+  if (int rc = linear_prepare(b.before, d->dtype, at(b.sums_at), stream)) return rc;
+  LinearJoin joins[2];
+  int n = 0;
+  const ProductPlan dx = product_plan(b.dx, d->dtype), dw = product_plan(b.dw, d->dtype);
+  if (g->dx) joins[n++] = {b.dx.e, at(b.dx_at), dx.s, b.dx.M, b.dx.N};
+  if (g->dw) joins[n++] = {b.dw.e, at(b.dw_at), dw.s, b.dw.M, b.dw.N};
+  int rc = WC_OK;
+  if (n == 2) rc = product_run_pair(b.dx, dx, at(b.dx_at), b.dw, dw, at(b.dw_at), d->dtype, stream);
+  else if (g->dx) rc = product_run(b.dx, dx, at(b.dx_at), d->dtype, stream);
+  else if (g->dw) rc = product_run(b.dw, dw, at(b.dw_at), d->dtype, stream);
+  if (rc) return rc;
+  return linear_join(joins, n, g->db ? &b.before.slope : nullptr, at(b.sums_at), d->dtype, stream);
 }
 
 int wc_pack8(const void* x, signed char* codes, signed char* exponents, long long rows, int C, int dtype, int keep_sign, void* stream) {

@@ -1,9 +1,11 @@
-// What the activation's derivative makes of dy: dz = dy act'(z) in the storage type - the operand of both products of a layer's
-// gradient, and the gradient of its residual -, and the column sums of dz before that rounding (the bias gradient), in one read of dy and z.
+// What stands before and behind the products of a layer's gradient, one launch each: small kernels of their own cost a few us apiece.
 //
-// Bound by that read.  A workgroup takes a run of rows, a thread VEC neighbouring columns with fp32 sums in registers; the threads of a column
-// meet in LDS, the workgroups in a second kernel, all in a fixed order.
-#include "linear.h"
+// Before them, dz = dy act'(z) in the storage type - the operand of both products, and the gradient of the layer's residual - and the column sums
+// of dz before that rounding (the bias gradient), in one read of dy and z, which bounds it: a workgroup takes a run of rows and some
+// columns, a thread eight neighbouring ones (16 bytes of 16-bit types, wherever they start) with fp32 sums in registers; the threads of a column
+// meet in LDS.  Beside it the copies of operands whose rows are no multiple of 16 bytes, and activations that were kept in 8 bits.
+// Behind them, the sums of the parts of a product's reduction and of the workgroups' columns, all in a fixed order.
+#include "linear_rows.h"
 
 #include <algorithm>
 
@@ -11,128 +13,279 @@ namespace wc {
 
 namespace {
 
-constexpr int kSlopeThreads = 256;
+constexpr int kThreads = 256;
+
+constexpr int VEC = 8;
 
 struct SlopeArgs {
   LinearSlope s;
-  float* part;               // (blocks, K); null: no sums
+  float* part;               // (blocks, K); null: no sums, or one block, whose sums are db
   long long rows_per_block;
   int cols, groups;          // threads side by side, rows in flight
 };
 
-template <typename T, int VEC>
-__global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
-  __shared__ float sums[kSlopeThreads * (VEC + (VEC > 1))];
-  constexpr int PITCH = VEC + (VEC > 1);
+template <typename T>
+__device__ __forceinline__ void store_sum(const LinearSlope& l, int k, float v) {
+  if (l.db_f32) static_cast<float*>(l.db)[k] = v;
+  else static_cast<T*>(l.db)[k] = static_cast<T>(v);
+}
+
+template <typename T, int ACT, bool PACKED>
+__device__ __forceinline__ void slope_rows(const SlopeArgs& a, int k, long long begin, long long end, float (&s)[VEC]) {
+  const LinearSlope& l = a.s;
+  const long long n_groups = pack_groups(l.K);
+  const int have = max(min(l.K - k, VEC), 0);
+  constexpr int AHEAD = 4;                        // rows asked for before the first is used
+  auto rows = [&](auto full, long long r0, int n) {
+    const int h = full() ? VEC : have;
+    T dy[AHEAD][VEC], v[AHEAD][VEC];
+    signed char q[AHEAD][VEC];
+    int e8[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (j >= n) break;
+      const long long r = r0 + j * a.groups, i = r * l.K + k;
+      load_run<T, VEC>(l.dy, i, h, dy[j]);
+      if constexpr (ACT != WC_ACT_NONE && PACKED) {
+        load_run<signed char, VEC>(l.z, i, h, q[j]);
+        e8[j] = h > 0 ? l.z_exp[r * n_groups + k / kPackGroup] : 0;
+      } else if constexpr (ACT != WC_ACT_NONE) {
+        load_run<T, VEC>(l.z, i, h, v[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (j >= n) break;
+      const long long r = r0 + j * a.groups;
+      T dz[VEC];
+      float step = 0.f;
+      if constexpr (ACT != WC_ACT_NONE && PACKED) step = pack_step(e8[j]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float z = 0.f;
+        if constexpr (ACT != WC_ACT_NONE && PACKED) z = (float)q[j][e] * step;
+        else if constexpr (ACT != WC_ACT_NONE) z = static_cast<float>(v[j][e]);
+        const float g = full() || e < have ? through(static_cast<float>(dy[j][e]), z, ACT) : 0.f;
+        s[e] += g;
+        dz[e] = static_cast<T>(g);
+      }
+      if (l.dz) store_run<T, VEC>(l.dz, r * l.K + k, h, dz);
+      if (l.dz_wide) store_run<T, VEC>(l.dz_wide, r * l.ld_wide + k, full() ? VEC : (int)min(l.ld_wide - k, (long long)VEC), dz);
+    }
+  };
+  auto all = [&](auto full) {
+    long long r = begin;
+    for (; r + (AHEAD - 1) * a.groups < end; r += AHEAD * a.groups) rows(full, r, AHEAD);
+    for (; r < end; r += a.groups) rows(full, r, 1);
+  };
+  if (have == VEC) all(std::true_type{});
+  else all(std::false_type{});
+}
+
+template <typename T>
+__device__ __forceinline__ void slope_block(const SlopeArgs& a, int block, int tile, float* sums) {
+  constexpr int PITCH = VEC + 1;
   const LinearSlope& l = a.s;
   const int group = threadIdx.x / a.cols, col = threadIdx.x - group * a.cols;
-  const int k = (blockIdx.y * a.cols + col) * VEC;
-  const long long begin = blockIdx.x * a.rows_per_block, end = min(l.rows, begin + a.rows_per_block);
-  const long long n_groups = pack_groups(l.K);
+  const int k = (tile * a.cols + col) * VEC;
+  const long long begin = block * a.rows_per_block, end = min(l.rows, begin + a.rows_per_block);
   float s[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-  if (group < a.groups && k < l.K) {
-#pragma unroll 2
-    for (long long r = begin + group; r < end; r += a.groups) {
-      const long long i = r * l.K + k;
-      const Pack<T, VEC> dy = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(l.dy) + i);
-      Pack<T, VEC> dz;
-      float z[VEC];
-      if (l.act == WC_ACT_NONE) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = 0.f;
-      } else if (l.z_exp) {
-        const Pack<signed char, VEC> q = *reinterpret_cast<const Pack<signed char, VEC>*>(static_cast<const signed char*>(l.z) + i);
-        const float step = pack_step(l.z_exp[r * n_groups + k / kPackGroup]);      // (VEC divides the group)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = (float)q.v[e] * step;
-      } else {
-        const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(l.z) + i);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = static_cast<float>(v.v[e]);
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float v = through(static_cast<float>(dy.v[e]), z[e], l.act);
-        s[e] += v;
-        dz.v[e] = static_cast<T>(v);
-      }
-      if (l.dz) *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(l.dz) + i) = dz;
+  if (k < l.K) {
+    auto run = [&](auto act) {
+      if (act() != WC_ACT_NONE && l.z_exp) slope_rows<T, act(), true>(a, k, begin + group, end, s);
+      else slope_rows<T, act(), false>(a, k, begin + group, end, s);
+    };
+    switch (l.act) {
+      case WC_ACT_RELU: run(ic<WC_ACT_RELU>{}); break;
+      case WC_ACT_GELU: run(ic<WC_ACT_GELU>{}); break;
+      case WC_ACT_GELU_TANH: run(ic<WC_ACT_GELU_TANH>{}); break;
+      case WC_ACT_SILU: run(ic<WC_ACT_SILU>{}); break;
+      default: run(ic<WC_ACT_NONE>{});
     }
   }
-  if (!a.part) return;
+  if (!l.db) return;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) sums[threadIdx.x * PITCH + e] = s[e];
   __syncthreads();
-  for (int i = threadIdx.x; i < a.cols * VEC; i += kSlopeThreads) {
-    const int c = i / VEC, e = i - c * VEC;
-    const int kk = (blockIdx.y * a.cols + c) * VEC + e;
+  for (int i = threadIdx.x; i < a.cols * VEC; i += kThreads) {
+    const int c = i / VEC, e = i % VEC, kk = (tile * a.cols + c) * VEC + e;
     if (kk >= l.K) continue;
     float t = 0.f;
     for (int g = 0; g < a.groups; ++g) t += sums[(g * a.cols + c) * PITCH + e];
-    a.part[(long long)blockIdx.x * l.K + kk] = t;
+    if (a.part) a.part[(long long)block * l.K + kk] = t;
+    else store_sum<T>(l, kk, t);
   }
 }
 
-// db[k] = sum over the workgroups' rows; 16 channels a workgroup, 64 threads to a channel's sums
+struct PrepareArgs {
+  SlopeArgs slope;
+  int slope_blocks, slope_tiles;       // none: 0
+  WideCopy copies[2];
+  long long copy_blocks[2];
+  UnpackArgs unpack;
+  int line;
+};
+
 template <typename T>
-__global__ __launch_bounds__(1024) void slope_sums_kernel(const float* __restrict__ part, void* __restrict__ db, int blocks, int K, bool f32) {
-  __shared__ float sums[64][16];
-  const int c = threadIdx.x & 15, group = threadIdx.x >> 4, k = blockIdx.x * 16 + c;
-  float s = 0.f;
-  if (k < K) {
-#pragma unroll 4
-    for (int b = group; b < blocks; b += 64) s += part[(long long)b * K + k];
+__global__ __launch_bounds__(kThreads) void prepare_kernel(PrepareArgs a) {
+  __shared__ float sums[kThreads * (VEC + 1)];
+  long long b = blockIdx.x;
+  const long long n = (long long)a.slope_blocks * a.slope_tiles;
+  if (b < n) return slope_block<T>(a.slope, (int)(b / a.slope_tiles), (int)(b % a.slope_tiles), sums);
+  b -= n;
+  if (b < a.copy_blocks[0]) return widen_block<T>(a.copies[0], b);
+  b -= a.copy_blocks[0];
+  if (b < a.copy_blocks[1]) return widen_block<T>(a.copies[1], b);
+  b -= a.copy_blocks[1];
+  if (a.line) unpack_line_block<T>(a.unpack, b);
+  else unpack_block<T>(a.unpack, b);
+}
+
+struct JoinArgs {
+  LinearJoin join[2];
+  long long blocks[2];
+  LinearSlope slope;
+  const float* sums;
+  int sum_rows;
+};
+
+// four neighbouring results a thread: the parts' sums in their order, and the epilogue
+template <typename T>
+__device__ __forceinline__ void join_block(const LinearJoin& j, long long block) {
+  const long long total = j.M * j.N, i = (block * kThreads + threadIdx.x) * 4;
+  if (i >= total) return;
+  const int have = (int)min(total - i, 4ll);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (have == 4 && total % 4 == 0) {
+#pragma unroll 8
+    for (int s = 0; s < j.s; ++s) {
+      const float4 p = *reinterpret_cast<const float4*>(j.parts + s * total + i);
+      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+    }
+  } else {
+    for (int s = 0; s < j.s; ++s) {
+      float p[4];
+      load_run<float, 4>(j.parts, s * total + i, have, p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
   }
-  sums[group][c] = s;
+  const LinearEpilogue& e = j.e;
+  T r[4], z[4], y[4];
+  if (e.res) load_run<T, 4>(e.res, i, have, r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float res = e.res ? static_cast<float>(r[k]) : 0.f;
+    if (e.bias) v[k] += static_cast<float>(static_cast<const T*>(e.bias)[min(i + k, total - 1) % j.N]);
+    if (!e.res_after) v[k] += res;
+    z[k] = static_cast<T>(v[k]);
+    v[k] = activate(v[k], e.act);
+    if (e.res_after) v[k] += res;
+    y[k] = static_cast<T>(v[k]);
+  }
+  if (e.z) store_run<T, 4>(e.z, i, have, z);
+  if (e.y_f32) store_run<float, 4>(e.y, i, have, v);
+  else store_run<T, 4>(e.y, i, have, y);
+}
+
+// db[k] = the sum of the workgroups' sums; 16 channels a workgroup, 16 threads to a channel's
+template <typename T>
+__device__ __forceinline__ void sums_block(const LinearSlope& l, const float* part, int rows, int block, float* lds) {
+  const int c = threadIdx.x & 15, group = threadIdx.x >> 4, k = block * 16 + c;
+  float s = 0.f;
+  if (k < l.K) {
+#pragma unroll 8
+    for (int b = group; b < rows; b += 16) s += part[(long long)b * l.K + k];
+  }
+  lds[threadIdx.x] = s;
   __syncthreads();
-  for (int half = 32; half > 0; half >>= 1) {
-    if (group < half) sums[group][c] += sums[group + half][c];
+  for (int half = 8; half > 0; half >>= 1) {
+    if (group < half) lds[threadIdx.x] += lds[threadIdx.x + half * 16];
     __syncthreads();
   }
-  if (group || k >= K) return;
-  if (f32) static_cast<float*>(db)[k] = sums[0][c];
-  else static_cast<T*>(db)[k] = static_cast<T>(sums[0][c]);
+  if (group == 0 && k < l.K) store_sum<T>(l, k, lds[c]);
 }
 
-struct SlopePlan { int vec, cols, col_tiles, groups, blocks; long long rows_per_block; };
-SlopePlan slope_plan(long long rows, int K, int es, bool aligned) {
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(JoinArgs a) {
+  __shared__ float lds[kThreads];
+  long long b = blockIdx.x;
+  if (b < a.blocks[0]) return join_block<T>(a.join[0], b);
+  b -= a.blocks[0];
+  if (b < a.blocks[1]) return join_block<T>(a.join[1], b);
+  sums_block<T>(a.slope, a.sums, a.sum_rows, (int)(b - a.blocks[1]), lds);
+}
+
+struct SlopePlan { int cols, col_tiles, groups, blocks; long long rows_per_block; };
+// As many columns side by side as leave four workgroups to a compute unit
+SlopePlan slope_plan(long long rows, int K) {
   SlopePlan p;
-  p.vec = aligned && K * es % 16 == 0 ? 16 / es : 1;
-  const int n = K / p.vec;
-  p.cols = std::min(n, kSlopeThreads);
-  p.col_tiles = ceil_div(n, p.cols);
-  p.groups = kSlopeThreads / p.cols;
-  // 32 KB of dy a workgroup, at most two rounds of the eight that a CU holds
-  const long long blocks = std::max(1ll, std::min(std::max(1ll, 4096ll / p.col_tiles), rows * K * es / p.col_tiles / 32768));
-  p.rows_per_block = ceil_div_ll(rows, blocks);
-  p.blocks = (int)ceil_div_ll(rows, p.rows_per_block);
-  return p;
+  for (p.cols = kThreads;; p.cols /= 2) {
+    p.groups = kThreads / p.cols;
+    p.col_tiles = ceil_div(ceil_div(K, VEC), p.cols);
+    const long long most = std::max(1ll, rows / p.groups), blocks = std::min<long long>(most, ceil_div(4 * kCus, p.col_tiles));
+    p.rows_per_block = ceil_div_ll(rows, blocks);
+    p.blocks = (int)ceil_div_ll(rows, p.rows_per_block);
+    if (p.cols == 16 || (ceil_div(K, VEC) > p.cols / 2 && (long long)p.col_tiles * blocks >= 4 * kCus)) return p;
+  }
 }
 
 }  // namespace
 
-size_t linear_slope_bytes(const LinearSlope& s, int dtype) {
-  if (!s.db) return 0;
-  const int es = dtype == WC_F32 ? 4 : 2;
-  return (size_t)std::max(slope_plan(s.rows, s.K, es, true).blocks, slope_plan(s.rows, s.K, es, false).blocks) * s.K * 4;
+size_t linear_sums_bytes(const LinearSlope& s) {
+  const int blocks = slope_plan(s.rows, s.K).blocks;
+  return s.db && blocks > 1 ? (size_t)blocks * s.K * 4 : 0;
 }
 
-int linear_slope(const LinearSlope& s, int dtype, void* part, void* stream) {
-  const int es = dtype == WC_F32 ? 4 : 2;
-  const bool aligned = (reinterpret_cast<uintptr_t>(s.dy) | reinterpret_cast<uintptr_t>(s.z) | reinterpret_cast<uintptr_t>(s.dz)) % 16 == 0;
-  const SlopePlan p = slope_plan(s.rows, s.K, es, aligned);
-  const SlopeArgs a = {s, s.db ? static_cast<float*>(part) : nullptr, p.rows_per_block, p.cols, p.groups};
+int linear_prepare(const LinearPrepare& p, int dtype, float* sums, void* stream) {
+  PrepareArgs a = {};
+  if (p.run_slope) {
+    const SlopePlan l = slope_plan(p.slope.rows, p.slope.K);
+    a.slope = {p.slope, p.slope.db && l.blocks > 1 ? sums : nullptr, l.rows_per_block, l.cols, l.groups};
+    a.slope_blocks = l.blocks;
+    a.slope_tiles = l.col_tiles;
+  }
+  for (int i = 0; i < p.n_copies; ++i) {
+    a.copies[i] = p.copies[i];
+    a.copy_blocks[i] = widen_blocks(p.copies[i]);
+  }
+  long long n = (long long)a.slope_blocks * a.slope_tiles + a.copy_blocks[0] + a.copy_blocks[1];
+  if (p.codes) {
+    const int rg = (int)pack_groups(p.x_C);
+    a.unpack = {p.codes, p.exps, p.x, p.x_rows * rg, p.x_ld, p.x_C, rg};
+    a.line = p.x_ld == p.x_C && on_a_line(p.x_C, p.x, p.codes);
+    n += unpack_blocks(a.unpack, a.line != 0);
+  }
+  if (n == 0) return WC_OK;
+  if (n >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "%lld rows of %d and %d elements are too many", p.slope.rows, p.slope.K, p.x_C);
   return dispatch_dtype(dtype, [&](auto t) -> int {
-    using T = decltype(t);
-    constexpr int FULL = 16 / sizeof(T);
-    hipLaunchKernelGGL((p.vec == FULL ? &slope_kernel<T, FULL> : &slope_kernel<T, 1>), dim3((unsigned)p.blocks, (unsigned)p.col_tiles), dim3(kSlopeThreads), 0, as_stream(stream), a);
-    WC_CHECK_LAUNCH("slope_kernel");
-    if (s.db) {
-      hipLaunchKernelGGL(slope_sums_kernel<T>, dim3((unsigned)ceil_div(s.K, 16)), dim3(1024), 0, as_stream(stream), a.part, s.db, p.blocks, s.K, s.db_f32 != 0);
-      WC_CHECK_LAUNCH("slope_sums_kernel");
-    }
+    hipLaunchKernelGGL(prepare_kernel<decltype(t)>, dim3((unsigned)n), dim3(kThreads), 0, as_stream(stream), a);
+    WC_CHECK_LAUNCH("prepare_kernel");
+    return WC_OK;
+  });
+}
+
+int linear_join(const LinearJoin* joins, int n, const LinearSlope* slope, const float* sums, int dtype, void* stream) {
+  JoinArgs a = {};
+  long long blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    a.join[i] = joins[i];
+    a.blocks[i] = joins[i].s > 1 ? ceil_div_ll(joins[i].M * joins[i].N, 4 * kThreads) : 0;
+    blocks += a.blocks[i];
+  }
+  if (slope && linear_sums_bytes(*slope)) {
+    a.slope = *slope;
+    a.sums = sums;
+    a.sum_rows = slope_plan(slope->rows, slope->K).blocks;
+    blocks += ceil_div(slope->K, 16);
+  }
+  if (blocks == 0) return WC_OK;
+  if (blocks >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "%lld x %lld results are too many", joins[0].M, joins[0].N);
+  return dispatch_dtype(dtype, [&](auto t) -> int {
+    hipLaunchKernelGGL(join_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), a);
+    WC_CHECK_LAUNCH("join_kernel");
     return WC_OK;
   });
 }

@@ -1,11 +1,9 @@
-// The products of a linear layer and of its gradients, D (M, N) = sum over R of A (x) B with an epilogue, operands with the reduction
-// axis innermost (x and w of the forward pass, dz of the input gradient) or outermost (w of the input gradient, dz and x of the weight
-// gradient), in any size and at any alignment.
+// Which kernel a product of linear.h takes, and the one for every size, alignment and layout: small products of rows that are no multiple
+// of 16 bytes, which are not worth a copy to ones that are.
 //
-// 64 x 64 results per workgroup, a 32 x 32 block of the matrix cores per wavefront; a stage of the reduction is brought to LDS with the
-// reduction innermost, whichever way it lies.  Where there are few tiles the reduction is cut into parts, whose fp32 sums a second kernel
-// adds in a fixed order before the epilogue.
-#include "linear.h"
+// 64 x 64 results per workgroup, a 32 x 32 block of the matrix cores per wavefront.  A stage of 64 bytes of the reduction goes through registers, three
+// stages ahead, to one of two LDS buffers with the reduction innermost, whichever way it lies; one barrier a stage.
+#include "linear_rows.h"
 
 #include <algorithm>
 
@@ -22,7 +20,6 @@ struct GeneralArgs {
   float* parts;               // (S, M, N); null: one part, the epilogue here
   long long R_part;
   int tiles_m, tiles_n, n_blocks, per_xcd;
-  bool vec_a, vec_b;          // 16-byte loads
 };
 
 template <typename T>
@@ -38,34 +35,27 @@ __device__ __forceinline__ void finish(const LinearEpilogue& e, long long m, lon
   else static_cast<T*>(e.y)[i] = static_cast<T>(v);
 }
 
-template <typename T>
+template <typename T, bool AO, bool BO>
 __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
-  constexpr int EPC = 16 / sizeof(T), BK = 4 * EPC, PITCH = BK + EPC;       // 64 bytes of a row and stage
-  __shared__ __attribute__((aligned(16))) T tile[2][64 * PITCH];
+  constexpr int EPC = 16 / sizeof(T), BK = 4 * EPC, PITCH = BK + EPC, AHEAD = 4;
+  __shared__ __attribute__((aligned(16))) T tile[2][2][64 * PITCH];
   const int blk = xcd_remap(blockIdx.x, g.per_xcd);
   if (blk >= g.n_blocks) return;
   const int tn = blk % g.tiles_n, tm = blk / g.tiles_n % g.tiles_m, s = blk / (g.tiles_n * g.tiles_m);
   const LinearProduct& p = g.p;
   const long long m0 = (long long)tm * 64, n0 = (long long)tn * 64;
   const long long begin = s * g.R_part, end = min(p.R, begin + g.R_part);
+  const int nk = end > begin ? (int)((end - begin + BK - 1) / BK) : 0;
   const int tid = threadIdx.x;
 
   // EPC elements a thread: of one row along the reduction, or of one reduction element along the rows
-  auto load = [&](const void* src, long long ld, bool outer, bool vec, long long row0, long long rows, long long k0, T (&v)[EPC]) {
-    const long long r = row0 + (outer ? tid % (64 / EPC) * EPC : tid / 4), k = k0 + (outer ? tid / (64 / EPC) : tid % 4 * EPC);
-    const T* q = static_cast<const T*>(src) + (outer ? k * ld + r : r * ld + k);
-    const long long have = outer ? (k < end ? rows - r : 0) : (r < rows ? end - k : 0);
-    if (vec && have >= EPC) {
-      const Pack<T, EPC> w = *reinterpret_cast<const Pack<T, EPC>*>(q);
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) v[e] = w.v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) v[e] = e < have ? q[e] : static_cast<T>(0.f);
-    }
+  auto load = [&](auto outer, const void* src, long long ld, long long row0, long long rows, int ks, T (&v)[EPC]) {
+    const long long r = row0 + (outer() ? tid % (64 / EPC) * EPC : tid / 4), k = begin + (long long)ks * BK + (outer() ? tid / (64 / EPC) : tid % 4 * EPC);
+    const long long have = outer() ? (k < end ? rows - r : 0) : (r < rows ? end - k : 0);
+    load_run<T, EPC>(src, outer() ? k * ld + r : r * ld + k, (int)min(max(have, 0ll), (long long)EPC), v);
   };
-  auto store = [&](T* to, bool outer, const T (&v)[EPC]) {
-    if (outer) {
+  auto store = [&](auto outer, T* to, const T (&v)[EPC]) {
+    if constexpr (outer()) {
 #pragma unroll
       for (int e = 0; e < EPC; ++e) to[(tid % (64 / EPC) * EPC + e) * PITCH + tid / (64 / EPC)] = v[e];
     } else {
@@ -75,36 +65,46 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
       *reinterpret_cast<Pack<T, EPC>*>(to + tid / 4 * PITCH + tid % 4 * EPC) = w;
     }
   };
+  using OA = std::integral_constant<bool, AO>;
+  using OB = std::integral_constant<bool, BO>;
 
   const int lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lhi = lane >> 5;
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
   f32x16 acc = {};
-  T va[EPC], vb[EPC];
-  if (begin < end) {
-    load(p.a, p.lda, p.a_outer, g.vec_a, m0, p.M, begin, va);
-    load(p.b, p.ldb, p.b_outer, g.vec_b, n0, p.N, begin, vb);
+  T va[AHEAD][EPC], vb[AHEAD][EPC];
+#pragma unroll
+  for (int u = 0; u < AHEAD - 1; ++u) {
+    if (u >= nk) break;
+    load(OA{}, p.a, p.lda, m0, p.M, u, va[u]);
+    load(OB{}, p.b, p.ldb, n0, p.N, u, vb[u]);
   }
-  for (long long k0 = begin; k0 < end; k0 += BK) {
-    __syncthreads();
-    store(tile[0], p.a_outer, va);
-    store(tile[1], p.b_outer, vb);
-    __syncthreads();
-    if (k0 + BK < end) {
-      load(p.a, p.lda, p.a_outer, g.vec_a, m0, p.M, k0 + BK, va);
-      load(p.b, p.ldb, p.b_outer, g.vec_b, n0, p.N, k0 + BK, vb);
-    }
-    const T* const ra = tile[0] + (wm + l32) * PITCH;
-    const T* const rb = tile[1] + (wn + l32) * PITCH;
-    if constexpr (sizeof(T) == 4) {
+#pragma unroll 1
+  for (int k0 = 0; k0 < nk; k0 += AHEAD) {
 #pragma unroll
-      for (int k = 0; k < BK; k += 2) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(rb[k + lhi], ra[k + lhi], acc, 0, 0, 0);
-    } else {
+    for (int u = 0; u < AHEAD; ++u) {
+      const int ks = k0 + u;
+      if (ks >= nk) break;
+      if (ks + AHEAD - 1 < nk) {
+        load(OA{}, p.a, p.lda, m0, p.M, ks + AHEAD - 1, va[(u + AHEAD - 1) % AHEAD]);
+        load(OB{}, p.b, p.ldb, n0, p.N, ks + AHEAD - 1, vb[(u + AHEAD - 1) % AHEAD]);
+      }
+      T(&lds)[2][64 * PITCH] = tile[u & 1];
+      store(OA{}, lds[0], va[u]);
+      store(OB{}, lds[1], vb[u]);
+      __syncthreads();                             // and nobody multiplies from the other buffer any more
+      const T* const ra = lds[0] + (wm + l32) * PITCH;
+      const T* const rb = lds[1] + (wn + l32) * PITCH;
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int k = 0; k < BK; k += 16) {
-        if constexpr (std::is_same<T, half_t>::value)
-          acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(rb + k + lhi * 8), *reinterpret_cast<const f16x8*>(ra + k + lhi * 8), acc, 0, 0, 0);
-        else
-          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(rb + k + lhi * 8), *reinterpret_cast<const bf16x8*>(ra + k + lhi * 8), acc, 0, 0, 0);
+        for (int k = 0; k < BK; k += 2) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(rb[k + lhi], ra[k + lhi], acc, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < BK; k += 16) {
+          if constexpr (std::is_same<T, half_t>::value)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(rb + k + lhi * 8), *reinterpret_cast<const f16x8*>(ra + k + lhi * 8), acc, 0, 0, 0);
+          else
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(rb + k + lhi * 8), *reinterpret_cast<const bf16x8*>(ra + k + lhi * 8), acc, 0, 0, 0);
+        }
       }
     }
   }
@@ -122,72 +122,64 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
     }
 }
 
-// the parts' sums added in their order, and the epilogue
-template <typename T>
-__global__ __launch_bounds__(256) void product_join_kernel(LinearEpilogue e, const float* __restrict__ parts, int S, long long M, long long N) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * N) return;
-  float v = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < S; ++s) v += parts[s * M * N + i];
-  finish<T>(e, i / N, i % N, N, v);
-}
+long long tiles_of(const LinearProduct& p, ProductTile t) { return ceil_div_ll(p.M, t.m) * ceil_div_ll(p.N, t.n); }
 
-// Tiles of 64 w x 64 w (w = 1: product_general_kernel, too), s parts of the reduction
-struct ProductPlan { bool dma; int w, s; long long R_part; };
-
-ProductPlan plan_of(const LinearProduct& p, bool dma) {
-  ProductPlan l = {dma, 1, 1, 0};
-  auto tiles = [&](int w) { return ceil_div_ll(p.M, 64 * w) * ceil_div_ll(p.N, 64 * w); };
-  if (l.dma) l.w = tiles(4) >= kCus ? 4 : tiles(2) >= kCus / 4 ? 2 : 1;
-  // as many as bring two (w = 2) or four tiles to a compute unit, of 256 elements and more, within 256 MB of sums
-  long long s = l.w == 4 ? 1 : std::min((l.w == 2 ? 2 : 4) * kCus / std::max(tiles(l.w), 1ll), std::max(p.R / 256, 1ll));
+ProductPlan plan_of(const LinearProduct& p, bool dma, int dtype) {
+  ProductPlan l = {dma, {64, 64}, 1, 0};
+  const int forced = test_gemm_config();
+  if (forced >= 32 && forced <= 35 && dma) {
+    const ProductTile tiles[] = {{64, 64}, {128, 128}, {256, 128}, {256, 256}};
+    l.tile = tiles[dtype == WC_F32 ? std::min(forced - 32, 1) : forced - 32];
+  } else if (dma) {
+    const bool heavy = p.e.act != WC_ACT_NONE || p.e.z || p.e.res;
+    if (dtype != WC_F32 && tiles_of(p, {256, 256}) >= kCus && p.R >= (heavy ? 8192 : 2048)) l.tile = {256, 256};
+    else if (dtype != WC_F32 && p.R >= 128 && tiles_of(p, {256, 128}) >= 2 * kCus) l.tile = {256, 128};
+    else if (tiles_of(p, {128, 128}) >= 3 * kCus / 2) l.tile = {128, 128};
+  }
+  // as many as bring two tiles of 128 x 128 or four of 64 x 64 to a compute unit, of 256 elements and more (of small products 64), within 256 MB
+  // of sums
+  const long long tiles = tiles_of(p, l.tile), least = tiles * p.R < 64 * kCus ? 64 : 256;
+  long long s = l.tile.m == 256 ? 1 : std::min((l.tile.m == 128 ? 2 : 4) * kCus / std::max(tiles, 1ll), std::max(p.R / least, 1ll));
   s = std::max(1ll, std::min(s, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
   l.R_part = std::max(64ll, ceil_div_ll(ceil_div_ll(p.R, s), 64) * 64);
   l.s = (int)std::max(1ll, ceil_div_ll(p.R, l.R_part));
   return l;
 }
 
-bool vectors(const void* p, long long ld, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0; }
-
 }  // namespace
 
-// (where the operands start is not known yet)
-size_t linear_product_bytes(const LinearProduct& p, int) {
-  const int s = std::max(plan_of(p, true).s, plan_of(p, false).s);
+ProductPlan product_plan(const LinearProduct& p, int dtype) { return plan_of(p, test_gemm_config() != 31 && product_dma_fits(p, dtype), dtype); }
+
+size_t product_parts_bytes(const LinearProduct& p, int dtype) {
+  const int s = std::max(plan_of(p, true, dtype).s, plan_of(p, false, dtype).s);
   return s > 1 ? (size_t)s * p.M * p.N * 4 : 0;
 }
 
-int linear_product(const LinearProduct& p, int dtype, void* workspace, void* stream) {
-  const int es = dtype == WC_F32 ? 4 : 2;
-  const ProductPlan l = plan_of(p, product_dma_fits(p, dtype));
-  const long long tiles = ceil_div_ll(p.M, 64 * l.w) * ceil_div_ll(p.N, 64 * l.w);
-  if (tiles * l.s >= (1ll << 31) - 8 || ceil_div_ll(p.M * p.N, 256) >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
-  float* const parts = l.s > 1 ? static_cast<float*>(workspace) : nullptr;
-  if (l.dma) {
-    if (int rc = product_dma(p, l.w, l.s, l.R_part, parts, dtype, stream)) return rc;
-  }
+int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream) {
+  const long long tiles = tiles_of(p, plan.tile);
+  if (tiles * plan.s >= (1ll << 31) - 8) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
+  if (plan.dma) return product_dma(p, plan, parts, dtype, stream);
+  GeneralArgs g;
+  g.p = p;
+  g.parts = plan.s > 1 ? parts : nullptr;
+  g.R_part = plan.R_part;
+  g.tiles_m = (int)ceil_div_ll(p.M, 64); g.tiles_n = (int)ceil_div_ll(p.N, 64);
+  g.n_blocks = (int)(tiles * plan.s);
+  g.per_xcd = ceil_div(g.n_blocks, kXcds);
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (!l.dma) {
-      GeneralArgs g;
-      g.p = p;
-      g.parts = parts;
-      g.R_part = l.R_part;
-      g.tiles_m = (int)ceil_div_ll(p.M, 64); g.tiles_n = (int)ceil_div_ll(p.N, 64);
-      g.n_blocks = (int)(tiles * l.s);
-      g.per_xcd = ceil_div(g.n_blocks, kXcds);
-      g.vec_a = vectors(p.a, p.lda, es);
-      g.vec_b = vectors(p.b, p.ldb, es);
-      hipLaunchKernelGGL(product_general_kernel<T>, dim3((unsigned)(g.per_xcd * kXcds)), dim3(256), 0, as_stream(stream), g);
-      WC_CHECK_LAUNCH("product_general_kernel");
-    }
-    if (parts) {
-      hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_ll(p.M * p.N, 256)), dim3(256), 0, as_stream(stream), p.e, parts, l.s, p.M, p.N);
-      WC_CHECK_LAUNCH("product_join_kernel");
-    }
+    auto fn = p.a_outer ? &product_general_kernel<T, true, true> : p.b_outer ? &product_general_kernel<T, false, true> : &product_general_kernel<T, false, false>;
+    hipLaunchKernelGGL(fn, dim3((unsigned)(g.per_xcd * kXcds)), dim3(256), 0, as_stream(stream), g);
+    WC_CHECK_LAUNCH("product_general_kernel");
     return WC_OK;
   });
+}
+
+int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream) {
+  const bool few = tiles_of(p, plan.tile) * plan.s + tiles_of(p2, plan2.tile) * plan2.s < (1ll << 31) - 16;
+  if (few && product_dma_pairs(plan, plan2)) return product_dma_pair(p, plan, parts, p2, plan2, parts2, dtype, stream);
+  if (int rc = product_run(p, plan, parts, dtype, stream)) return rc;
+  return product_run(p2, plan2, parts2, dtype, stream);
 }
 
 }  // namespace wc

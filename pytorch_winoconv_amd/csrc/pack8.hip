@@ -9,8 +9,9 @@
 // A group with an infinity or a NaN has the exponent 127 and reads as NaN throughout, so that such values still show in the gradients.
 // keep_sign: values other than zero keep a code other than zero, one step - for what is read by its sign alone (the gate of a ReLU).
 //
-// Bound by memory.  A thread takes four neighbouring elements, eight threads a group.
-#include "linear.h"
+// Bound by memory.  Rows of whole groups are one line of groups: a thread takes eight neighbouring elements four times, 16 bytes a load, and
+// four threads a group.  Other rows take eight threads a group, four elements each, wherever they start.
+#include "linear_rows.h"
 
 #include <algorithm>
 
@@ -19,7 +20,7 @@ namespace wc {
 namespace {
 
 struct PackArgs {
-  const void* x; void* out;
+  const void* x;
   signed char* codes; signed char* exps;
   long long groups;          // of all rows
   int C, row_groups;
@@ -37,6 +38,36 @@ __device__ __forceinline__ int pack_code(float v, int e, bool keep_sign) {
   return keep_sign && q == 0.f && v != 0.f ? (v > 0.f ? 1 : -1) : (int)q;
 }
 
+// the exponent of a group from N of its elements in each of 32 / N neighbouring lanes
+template <typename T, int N>
+__device__ __forceinline__ int group_exponent(const T (&x)[N]) {
+  unsigned top = 0;                                        // bits: a maximum of floats would drop a NaN
+#pragma unroll
+  for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(static_cast<float>(x[e])) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < kPackGroup / N; d <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+  return pack_exponent(__uint_as_float(top));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void pack8_line_kernel(PackArgs a) {
+  const long long total = a.groups * kPackGroup, first = (long long)blockIdx.x * kLine + threadIdx.x * 8;
+  T x[4][8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) load_run<T, 8>(a.x, first + j * 2048, first + j * 2048 < total ? 8 : 0, x[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const long long i = first + j * 2048;
+    const int e = group_exponent<T, 8>(x[j]);
+    Pack<signed char, 8> q;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q.v[k] = (signed char)pack_code(static_cast<float>(x[j][k]), e, a.keep_sign);
+    if (i >= total) continue;
+    *reinterpret_cast<Pack<signed char, 8>*>(a.codes + i) = q;
+    if ((threadIdx.x & 3) == 0) a.exps[i / kPackGroup] = (signed char)e;
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void pack8_kernel(PackArgs a) {
   const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
@@ -44,44 +75,32 @@ __global__ __launch_bounds__(256) void pack8_kernel(PackArgs a) {
   const long long row = g / a.row_groups;
   const int c0 = (int)(g - row * a.row_groups) * kPackGroup + part * 4;
   const int n = g < a.groups ? min(a.C - c0, 4) : 0;
-  const T* x = static_cast<const T*>(a.x) + row * a.C + c0;
-  float v[4], top = 0.f;
+  T x[4];
+  load_run<T, 4>(a.x, row * a.C + c0, n, x);
+  const int e = group_exponent<T, 4>(x);
+  signed char q[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = e < n ? static_cast<float>(x[e]) : 0.f;
-    // (bits: a maximum of floats would drop a NaN)
-    top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(v[e]) & 0x7fffffffu));
-  }
-#pragma unroll
-  for (int d = 1; d < 8; d <<= 1) top = __uint_as_float(max(__float_as_uint(top), (unsigned)__shfl_xor((int)__float_as_uint(top), d)));
-  const int e = pack_exponent(top);
-  if (n <= 0) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) a.codes[row * a.C + c0 + i] = (signed char)pack_code(v[i], e, a.keep_sign);
-  if (part == 0) a.exps[g] = (signed char)e;
+  for (int k = 0; k < 4; ++k) q[k] = (signed char)pack_code(static_cast<float>(x[k]), e, a.keep_sign);
+  store_run<signed char, 4>(a.codes, row * a.C + c0, n, q);
+  if (part == 0 && n > 0) a.exps[g] = (signed char)e;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void unpack8_kernel(PackArgs a) {
-  const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
-  if (g >= a.groups) return;
-  const long long row = g / a.row_groups;
-  const int c0 = (int)(g - row * a.row_groups) * kPackGroup + (threadIdx.x & 7) * 4;
-  const float step = pack_step(a.exps[g]);
-  const long long i = row * a.C + c0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (c0 + e < a.C) static_cast<T*>(a.out)[i + e] = static_cast<T>((float)a.codes[i + e] * step);
+template <typename T, bool LINE>
+__global__ __launch_bounds__(256) void unpack8_kernel(UnpackArgs a) {
+  if constexpr (LINE) unpack_line_block<T>(a, blockIdx.x);
+  else unpack_block<T>(a, blockIdx.x);
 }
 
 }  // namespace
 
 int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, bool keep_sign, int dtype, void* stream) {
   const int rg = (int)pack_groups(C);
-  const PackArgs a = {x, nullptr, codes, exps, rows * rg, C, rg, keep_sign};
+  const PackArgs a = {x, codes, exps, rows * rg, C, rg, keep_sign};
+  const bool line = on_a_line(C, x, codes);
   return dispatch_dtype(dtype, [&](auto t) -> int {
-    hipLaunchKernelGGL(pack8_kernel<decltype(t)>, dim3((unsigned)ceil_div_ll(a.groups, 32)), dim3(256), 0, as_stream(stream), a);
+    using T = decltype(t);
+    hipLaunchKernelGGL((line ? &pack8_line_kernel<T> : &pack8_kernel<T>), dim3((unsigned)(line ? ceil_div_ll(a.groups * kPackGroup, kLine) : ceil_div_ll(a.groups, 32))), dim3(256), 0,
+                       as_stream(stream), a);
     WC_CHECK_LAUNCH("pack8_kernel");
     return WC_OK;
   });
@@ -89,9 +108,11 @@ int pack8(const void* x, signed char* codes, signed char* exps, long long rows, 
 
 int unpack8(const signed char* codes, const signed char* exps, void* x, long long rows, int C, int dtype, void* stream) {
   const int rg = (int)pack_groups(C);
-  const PackArgs a = {nullptr, x, const_cast<signed char*>(codes), const_cast<signed char*>(exps), rows * rg, C, rg, 0};
+  const UnpackArgs a = {codes, exps, x, rows * rg, C, C, rg};
+  const bool line = on_a_line(C, x, codes);
   return dispatch_dtype(dtype, [&](auto t) -> int {
-    hipLaunchKernelGGL(unpack8_kernel<decltype(t)>, dim3((unsigned)ceil_div_ll(a.groups, 32)), dim3(256), 0, as_stream(stream), a);
+    using T = decltype(t);
+    hipLaunchKernelGGL((line ? &unpack8_kernel<T, true> : &unpack8_kernel<T, false>), dim3((unsigned)unpack_blocks(a, line)), dim3(256), 0, as_stream(stream), a);
     WC_CHECK_LAUNCH("unpack8_kernel");
     return WC_OK;
   });

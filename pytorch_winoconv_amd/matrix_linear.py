@@ -51,7 +51,11 @@ def _rows(shape):
 
 
 def _contiguous(t):
-    return None if t is None else t.detach().contiguous()
+    """Contiguous and, for 16-byte loads, starting at a multiple of 16 bytes."""
+    if t is None:
+        return None
+    t = t.detach().contiguous()
+    return t.clone() if engine.misaligned(t) else t
 
 
 def _desc(rows, C, K, dtype, activation, residual_after=False):

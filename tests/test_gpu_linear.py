@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 # rows, C, K: one of everything, odd, around tiles and stages, long reductions, few and many rows
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 31, 65), (8, 64, 64), (16, 512, 40), (33, 40, 72), (64, 64, 64), (65, 33, 17), (130, 257, 96), (200, 72, 264), (7, 1000, 3),
           (513, 16, 300), (257, 136, 520), (1, 4096, 24), (5, 2056, 1000), (17, 3000, 128), (1025, 8, 8), (300, 300, 301), (1000, 520, 776),
-          (2000, 96, 640)]
+          (2000, 96, 640), (600, 501, 403), (600, 504, 403), (600, 501, 408)]
 
 
 def _inputs(rows, C, K, t, seed, bias=True):
@@ -66,7 +66,7 @@ def test_gradients(dev, shape, t):
 
 
 @pytest.mark.parametrize("t", lo.TYPES, ids=str)
-@pytest.mark.parametrize("shape", [(3, 5, 7), (8, 64, 64), (33, 40, 72), (65, 33, 17), (200, 72, 264), (1000, 136, 96), (300, 300, 301), (1, 4096, 24)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 5, 7), (8, 64, 64), (33, 40, 72), (65, 33, 17), (200, 72, 264), (1000, 136, 96), (300, 300, 301), (1, 4096, 24), (600, 501, 403), (600, 504, 408)], ids=str)
 def test_gradients_from_8_bits(dev, shape, t):
     for i, act in enumerate(lo.ACTS):
         x, w, b, r, dy = _inputs(*shape, t, 7 * i + shape[2])
@@ -80,6 +80,25 @@ def test_gradients_from_8_bits(dev, shape, t):
         got = matrix_linear.linear_backward(dy.cuda(), P[0], w.cuda(), P[1], act, need_dz=True)
         for k, v in zip(("dx", "dw", "db", "dz"), got):
             lo.within(v, *want[k], "%s %s" % (k, act))
+
+
+@pytest.mark.parametrize("t", lo.TYPES, ids=str)
+@pytest.mark.parametrize("config", [31, 32, 33, 34, 35])
+def test_every_tile(dev, gemm_override, config, t):
+    """Each kernel and tile on small ragged problems: one part of the reduction and several, one row of tiles and some."""
+    gemm_override(config)
+    for shape in [(1, 8, 8), (70, 40, 72), (300, 264, 328), (130, 1160, 264), (520, 72, 517), (65, 2000, 24)]:
+        for act, keep in (("none", False), ("gelu", True), ("relu", False)):
+            x, w, b, r, dy = _inputs(*shape, t, config)
+            y, z, by, bz = lo.forward(x, w, b, r, act, keep)
+            got = matrix_linear.linear_forward(*_cuda(x, w, b, r), act, keep, keep)
+            if keep:
+                lo.within(got[1], z, bz, "z %r" % (shape,))
+            lo.within(got[0] if keep else got, y, by, "y %r" % (shape,))
+            z = z.to(t)
+            want = lo.backward(dy, x, w, z, act)
+            for k, v in zip(("dx", "dw", "db", "dz"), matrix_linear.linear_backward(*_cuda(dy, x, w, z), act, need_dz=True)):
+                lo.within(v, *want[k], "%s %r" % (k, shape))
 
 
 @pytest.mark.parametrize("t", lo.TYPES[1:], ids=str)
