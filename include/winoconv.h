@@ -165,8 +165,8 @@ const char* wc_last_error(void);
  * config 22 to 26: the direct form of 16-bit types on tiles of 256 x 128, 128 x 128, 256 x 64, 128 x 64 or 64 x 64 whatever the
  * problem (direct_dma.hip); 22 also: fp32 products and weight gradients on the fp32 instructions.  config 27 to 29: its forward
  * products on tiles of 320, 384 or 448 x 128.
- * config 31: linear layers take the product kernel of every alignment; config 32 to 35: the one fed by LDS-DMA, where it runs, on tiles of 64 x 64,
- * 128 x 128, 256 x 128 or 256 x 256 (the last two in 16-bit types).
+ * config 31: linear layers take the product kernel of every alignment; config 32 to 34: the one fed by LDS-DMA, where it runs, on tiles of 64 x 64,
+ * 128 x 128 or, in 16-bit types, 256 x 256.
  * config 0 to 4 in fp32: the tiles of the product in three bf16 parts.  config 0: the direct form of 16-bit
  * types through registers (gemm.hip).
  * Works only in a process started with WINOCONV_TEST_HOOKS=1 in its environment (WC_ERR_UNSUPPORTED

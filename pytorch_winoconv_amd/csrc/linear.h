@@ -86,13 +86,13 @@ struct LinearProduct {
 // their sums (s, M, N) in fp32, which linear_join adds.
 struct ProductTile { int m, n; };
 struct ProductPlan { bool dma; ProductTile tile; int s; long long R_part; };
-ProductPlan product_plan(const LinearProduct& p, int dtype);
+ProductPlan product_plan(const LinearProduct& p, int dtype, const LinearProduct* beside);      // beside: runs in the same launch; null: none
 size_t product_parts_bytes(const LinearProduct& p, int dtype);      // whatever the operands' start
 int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream);
 // both, in one launch where their plans allow it
 int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream);
 
-// linear_dma.hip: products whose rows are multiples of 16 bytes, on tiles of 256 x 256, 256 x 128 (16-bit types), 128 x 128 or 64 x 64
+// linear_dma.hip: products whose rows are multiples of 16 bytes, on tiles of 256 x 256 (16-bit types), 128 x 128 or 64 x 64
 bool product_dma_fits(const LinearProduct& p, int dtype);
 int product_dma(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream);
 bool product_dma_pairs(const ProductPlan& plan, const ProductPlan& plan2);

@@ -153,7 +153,7 @@ int wc_linear_forward(const wc_linear_desc* d, const void* x, const void* w, con
     if (int rc = linear_prepare(before, d->dtype, nullptr, stream)) return rc;
   }
   float* const parts = reinterpret_cast<float*>(ws + f.scratch_at);
-  const ProductPlan plan = product_plan(f.p, d->dtype);
+  const ProductPlan plan = product_plan(f.p, d->dtype, nullptr);
   if (int rc = product_run(f.p, plan, parts, d->dtype, stream)) return rc;
   const LinearJoin join = {f.p.e, parts, plan.s, f.p.M, f.p.N};
   return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
@@ -183,7 +183,7 @@ int wc_linear_backward(const wc_linear_desc* d, const wc_linear_gradients* g, vo
   if (int rc = linear_prepare(b.before, d->dtype, at(b.sums_at), stream)) return rc;
   LinearJoin joins[2];
   int n = 0;
-  const ProductPlan dx = product_plan(b.dx, d->dtype), dw = product_plan(b.dw, d->dtype);
+  const ProductPlan dx = product_plan(b.dx, d->dtype, nullptr), dw = product_plan(b.dw, d->dtype, &b.dx);      // dw's bits do not hang on whether dx is asked for
   if (g->dx) joins[n++] = {b.dx.e, at(b.dx_at), dx.s, b.dx.M, b.dx.N};
   if (g->dw) joins[n++] = {b.dw.e, at(b.dw_at), dw.s, b.dw.M, b.dw.N};
   int rc = WC_OK;

@@ -9,7 +9,7 @@
 //
 // Results go through LDS in fp32, 32 rows of a wavefront at a time, so that bias, residual, y and z are read and written 16 bytes a lane in
 // whole row segments; few tiles: parts of the reduction, whose sums join_kernel (linear_gradient.hip) adds.
-#include "linear.h"
+#include "linear_rows.h"
 #include "lds_dma.h"
 #include "wc_transform.h"
 
@@ -79,13 +79,25 @@ template <typename T, int W, bool OUTER> struct DmaOperand {
       }
     }
   }
-  // queues the next stage; `have` reduction elements are left of the part
-  __device__ __forceinline__ void queue(unsigned lds, int wave, int i, long long have) const {
-    const DmaDesc d = dma_descriptor(base, left);
-    const unsigned to = lds + (OUTER ? wave * LOADS + i : wave + 4 * i) * 1024;
-    dma16(d, OUTER || chunk * EPC < have ? voff[i] : kOutside, to);
+  // of the next stage, or of the next two: descriptors, and what puts a lane's chunk outside them where the part ends before it
+  DmaDesc d, d2;
+  unsigned out, out2;
+  template <bool PAIR> __device__ __forceinline__ void aim(long long have) {                   // `have` reduction elements are left of the part
+    d = dma_descriptor(base, left);
+    out = OUTER || chunk * EPC < have ? 0u : kOutside;
+    if constexpr (PAIR) {
+      d2 = dma_descriptor(base + advance, left - advance);
+      out2 = OUTER || chunk * EPC + kDeep<T> < have ? 0u : kOutside;
+    }
+    base += (PAIR ? 2 : 1) * advance;
+    left -= (PAIR ? 2 : 1) * advance;
   }
-  __device__ __forceinline__ void next() { base += advance; left -= advance; }
+  // queues load i of them, into LDS at `lds` and `lds2`
+  template <bool PAIR> __device__ __forceinline__ void queue(unsigned lds, unsigned lds2, int wave, int i) const {
+    const unsigned to = (OUTER ? wave * LOADS + i : wave + 4 * i) * 1024;
+    dma16(d, voff[i] | out, lds + to);
+    if constexpr (PAIR) dma16(d2, voff[i] | out2, lds2 + to);
+  }
 
   // byte offset of a lane's part of the fragment of half `kk` of a stage, rows 32 b .. of the tile
   static __device__ __forceinline__ int offset(int b, int kk, int lane) {
@@ -117,100 +129,102 @@ template <typename T, int W, bool OUTER> struct DmaOperand {
   }
 };
 
+constexpr int kBand = 8;       // tiles along M that are neighbours
+
 struct DmaArgs {
   LinearProduct p;
   float* parts;               // (S, M, N); null: one part, the epilogue here
   long long R_part;
   int tiles_m, tiles_n, n_blocks, per_xcd;
-  int vec;                    // rows of the results are multiples of 16 bytes
+  int vec;                    // rows of the parts' sums are multiples of 16 bytes
 };
 
-// Eight elements at a multiple of 16 bytes, 16 bytes an access
-template <typename T> using Sixteen = Pack<T, kChunk<T>>;
-template <typename T> __device__ __forceinline__ void store8(T* to, const Pack<T, 8>& v) {
-#pragma unroll
-  for (int i = 0; i < 8 / kChunk<T>; ++i) reinterpret_cast<Sixteen<T>*>(to)[i] = reinterpret_cast<const Sixteen<T>*>(&v)[i];
-}
-template <typename T> __device__ __forceinline__ void load8(const T* from, Pack<T, 8>& v) {
-#pragma unroll
-  for (int i = 0; i < 8 / kChunk<T>; ++i) reinterpret_cast<Sixteen<T>*>(&v)[i] = reinterpret_cast<const Sixteen<T>*>(from)[i];
-}
-
-// Eight neighbouring results of a row, of which `have` are there: sums to z and y.  VEC: elements of an access.
-template <typename T, int ACT, int VEC>
-__device__ __forceinline__ void finish_run(const LinearEpilogue& e, long long i, int have, const float (&sum)[8], const float (&bias)[8], const Pack<T, 8>& res) {
-  Pack<T, 8> z, y;
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] = sum[j] + bias[j];
-    const float r = static_cast<float>(res.v[j]);
-    if (!e.res_after) v[j] += r;
-    z.v[j] = static_cast<T>(v[j]);
-    v[j] = activate(v[j], ACT);
-    if (e.res_after) v[j] += r;
-    y.v[j] = static_cast<T>(v[j]);
-  }
-  if constexpr (VEC == 8) {
-    if (e.z) store8(static_cast<T*>(e.z) + i, z);
-    if (e.y_f32 && sizeof(T) == 2) {
-      float* const to = static_cast<float*>(e.y) + i;
-      *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
-    } else {
-      store8(static_cast<T*>(e.y) + i, y);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j >= have) break;
-      if (e.z) static_cast<T*>(e.z)[i + j] = z.v[j];
-      if (e.y_f32) static_cast<float*>(e.y)[i + j] = v[j];
-      else static_cast<T*>(e.y)[i + j] = y.v[j];
-    }
-  }
-}
-
-// A wavefront's WM x WN blocks through 32 rows of LDS of its own
-template <typename T, int ACT, int VEC, int WM, int WN>
+// A wavefront's WM x WN blocks through 32 rows of LDS of its own, a lane finishing eight neighbouring results of some rows, which start anywhere.
+// ALL: the tile is whole, no lane asks whether its results are there - a branch at every access leaves none to overlap.  MORE: there may be a
+// residual or z.
+template <typename T, int ACT, bool ALL, bool MORE, int WM, int WN>
 __device__ __forceinline__ void finish_blocks(const LinearEpilogue& e, const f32x16 (&acc)[WM][WN], float* stage, long long m0, long long M, int n0, long long N, int lane) {
-  constexpr int PITCH = WN * 32 + 4, LPR = WN * 4, RPI = 64 / LPR;          // floats of a row, lanes to a row, rows of an access
+  constexpr int PITCH = WN * 32 + 4, LPR = WN * 4, RPI = 64 / LPR;      // floats of a row, lanes to a row, rows of an access
+  constexpr int RUNS = 32 / RPI, AT_ONCE = RUNS < 4 || !MORE ? RUNS : 4;
   const int l32 = lane & 31, lhi = lane >> 5, row0 = lane / LPR, n = n0 + lane % LPR * 8;
-  const int have = (int)min(8ll, N - n);
+  const int have = ALL ? 8 : (int)max(min(8ll, N - n), 0ll);
   float bias[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) bias[j] = e.bias && j < have ? static_cast<float>(static_cast<const T*>(e.bias)[n + j]) : 0.f;
+  for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+  if (e.bias) {
+    T b[8];
+    load_run<T, 8>(e.bias, n, have, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[j] = static_cast<float>(b[j]);
+  }
 #pragma unroll
   for (int i = 0; i < WM; ++i) {
     const long long first = (m0 + i * 32 + row0) * N + n;
     const int rows = (int)min(32ll, M - m0 - i * 32);
-    Pack<T, 8> res[32 / RPI];
-#pragma unroll
-    for (int r = 0; r < 32 / RPI; ++r) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) res[r].v[j] = static_cast<T>(0.f);
-      if (e.res && have > 0 && row0 + r * RPI < rows) {
-        const T* const from = static_cast<const T*>(e.res) + first + (long long)(r * RPI) * N;
-        if constexpr (VEC == 8) load8(from, res[r]);
-        else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < have) res[r].v[j] = from[j];
-        }
-      }
-    }
+    auto there = [&](int r) { return ALL ? 8 : row0 + r * RPI < rows ? have : 0; };
+    auto at = [&](int r) { return first + (long long)(r * RPI) * N; };
 #pragma unroll
     for (int j = 0; j < WN; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(stage + l32 * PITCH + j * 32 + 8 * q + 4 * lhi) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
 #pragma unroll
-    for (int r = 0; r < 32 / RPI; ++r) {
-      float v[8];
-      const float* const from = stage + (row0 + r * RPI) * PITCH + lane % LPR * 8;
-      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(from);
-      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(from + 4);
-      if (have > 0 && row0 + r * RPI < rows) finish_run<T, ACT, VEC>(e, first + (long long)(r * RPI) * N, have, v, bias, res[r]);
+    for (int r0 = 0; r0 < RUNS; r0 += AT_ONCE) {
+      T res[AT_ONCE][8];
+      float v[AT_ONCE][8];
+      if (MORE && e.res) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) load_run<T, 8>(e.res, at(r0 + r), there(r0 + r), res[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) res[r][j] = static_cast<T>(0.f);
+      }
+#pragma unroll
+      for (int r = 0; r < AT_ONCE; ++r) {
+        const float* const from = stage + (row0 + (r0 + r) * RPI) * PITCH + lane % LPR * 8;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[r][j] = lo[j] + bias[j];
+          v[r][j + 4] = hi[j] + bias[j + 4];
+        }
+      }
+      if (MORE && !e.res_after) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[r][j] += static_cast<float>(res[r][j]);
+      }
+      auto store = [&](void* to) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) {
+          T o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = static_cast<T>(v[r][j]);
+          store_run<T, 8>(to, at(r0 + r), there(r0 + r), o);
+        }
+      };
+      if (MORE && e.z) store(e.z);
+      if constexpr (ACT != WC_ACT_NONE) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[r][j] = activate(v[r][j], ACT);
+      }
+      if (MORE && e.res_after) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[r][j] += static_cast<float>(res[r][j]);
+      }
+      if (e.y_f32 && sizeof(T) == 2) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) store_run<float, 8>(e.y, at(r0 + r), there(r0 + r), v[r]);
+      } else {
+        store(e.y);
+      }
     }
   }
 }
@@ -233,10 +247,10 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   const int blk = xcd_remap(hw_block, g.per_xcd);
   if (blk >= g.n_blocks) return;
-  // eight tiles along M, then along N: the workgroups of an XCD that run together share the rows of few tiles of either operand
+  // a band of tiles along M, then along N: the workgroups of an XCD that run together share the rows of few tiles of either operand
   const int tiles = g.tiles_m * g.tiles_n, s = blk / tiles, t = blk % tiles;
-  const int band = t / (8 * g.tiles_n), in_band = t % (8 * g.tiles_n), high = min(8, g.tiles_m - band * 8);
-  const long long m0 = (long long)(band * 8 + in_band % high) * (64 * WM), n0 = (long long)(in_band / high) * (64 * WN);
+  const int band = t / (kBand * g.tiles_n), in_band = t % (kBand * g.tiles_n), high = min(kBand, g.tiles_m - band * kBand);
+  const long long m0 = (long long)(band * kBand + in_band % high) * (64 * WM), n0 = (long long)(in_band / high) * (64 * WN);
   const LinearProduct& p = g.p;
   const long long begin = s * g.R_part, end = min(p.R, begin + g.R_part);
   const int nk = end > begin ? (int)((end - begin + kDeep<T> - 1) / kDeep<T>) : 0;
@@ -247,15 +261,24 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   B b;
   a.start(p.a, p.lda, m0, p.M, begin, end, wave, lane);
   b.start(p.b, p.ldb, n0, p.N, begin, end, wave, lane);
-  int queued = 0;
-  auto queue = [&](int q) {                         // load q of the L of stage `queued`
-    const unsigned to = lds0 + (queued % kRing) * STAGE;
-    const long long have = end - begin - (long long)queued * kDeep<T>;
-    if (q < WM) a.queue(to, wave, q, have);
-    else b.queue(to + A::BYTES, wave, q - WM, have);
+  constexpr bool PAIR = !AHEAD;
+  long long left = end - begin;
+  int to = 0;                                       // slot of the ring of the next stage to be queued ...
+  auto after = [](int slot) { return slot + 1 == kRing ? 0 : slot + 1; };
+  auto queue = [&](int q) {                         // load q of the L of a stage, or of two
+    const unsigned at = lds0 + to * STAGE, at2 = lds0 + after(to) * STAGE;
+    if (q < WM) a.template queue<PAIR>(at, at2, wave, q);
+    else b.template queue<PAIR>(at + A::BYTES, at2 + A::BYTES, wave, q - WM);
   };
-  auto queue_next = [&] { a.next(); b.next(); ++queued; };
+  auto aim = [&] {
+    a.template aim<PAIR>(left);
+    b.template aim<PAIR>(left);
+    left -= (PAIR ? 2 : 1) * kDeep<T>;
+  };
+  auto queue_next = [&] { to = PAIR ? after(after(to)) : after(to); aim(); };
+  aim();
 
+  const long long wm0 = m0 + wm * WM * 32, wn0 = n0 + wn * WN * 32;
   f32x16 acc[WM][WN];
 #pragma unroll
   for (int i = 0; i < WM; ++i)
@@ -273,16 +296,18 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   }
   s16x8 va[2][WM], vb[2][WN];
 
-  if (nk > 0) {
+  int now = 0;                                      // ... and of the stage that is multiplied
+  if constexpr (AHEAD) {
+    // One wavefront to a SIMD.  Three stages in flight; the first half of a stage is read while the last one of the stage before is multiplied
+    static_assert(kRing == 4, "three stages in flight beside the one that is multiplied");
+    if (nk > 0) {
 #pragma unroll
-    for (int k = 0; k < kRing - 1; ++k) {
-      if (k >= nk) break;
+      for (int k = 0; k < kRing - 1; ++k) {
+        if (k >= nk) break;
 #pragma unroll
-      for (int q = 0; q < L; ++q) queue(q);
-      queue_next();
-    }
-    if constexpr (AHEAD) {
-      static_assert(kRing == 4, "three stages in flight");
+        for (int q = 0; q < L; ++q) queue(q);
+        queue_next();
+      }
       if (nk >= 3) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * L) : "memory");
       else if (nk == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(L) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
@@ -291,17 +316,16 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
 #pragma unroll
       for (int j = 0; j < WN; ++j) vb[0][j] = B::read(lds + fb[0][j]);
     }
-  }
 #pragma unroll 1
-  for (int ks = 0; ks < nk; ++ks) {
-    const bool more = ks + kRing - 1 < nk;
-    if constexpr (AHEAD) {
+    for (int ks = 0; ks < nk; ++ks) {
       // stage ks + 1 has landed, in flight may be that of ks + 2; nobody reads stage ks - 1 any more, which that of ks + 3 overwrites
       if (ks + 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(L) : "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const bool more = ks + kRing - 1 < nk;
+      const int then = ks + 1 < nk ? after(now) : now;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        const unsigned char* const st = lds + (kk ? min(ks + 1, nk - 1) % kRing : ks % kRing) * STAGE;      // of the half after this one
+        const unsigned char* const st = lds + (kk ? then : now) * STAGE;      // of the half after this one
 #pragma unroll
         for (int i = 0; i < WM; ++i) {
           va[kk ^ 1][i] = A::read(st + fa[kk ^ 1][i]);
@@ -322,13 +346,28 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      now = after(now);
       if (more) queue_next();
-    } else {
-      // stage ks has landed, in flight may be the RING - 2 after it; nobody reads stage ks - 1 any more
-      if (ks + kRing - 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((kRing - 2) * L) : "memory");
-      else if (kRing > 3 && ks + 1 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(L) : "memory");
+    }
+  } else {
+    // Several wavefronts to a SIMD.  Stages are queued in pairs, load by load: the 64 bytes of a row and stage are half a line of the L2, whose other half
+    // the load of the next stage finds in the L1 where it follows at once: an operand with the reduction innermost then comes at 120
+    // bytes a ns and compute unit from the L2, at 64 otherwise (measured on loads alone).
+    static_assert(kRing == 5, "a pair in flight and one that lands beside the stage that is multiplied");
+    const int pairs = (nk + 1) / 2;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k >= pairs) break;
+#pragma unroll
+      for (int q = 0; q < L; ++q) queue(q);
+      queue_next();
+    }
+    auto wait = [&](bool one_in_flight) {           // for all but the last pair, and for all wavefronts
+      if (one_in_flight) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * L) : "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      const unsigned char* const st = lds + ks % kRing * STAGE;
+    };
+    auto step = [&](bool more) {
+      const unsigned char* const st = lds + now * STAGE;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
@@ -347,12 +386,25 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
         for (int i = 0; i < WM; ++i)
 #pragma unroll
           for (int j = 0; j < WN; ++j) acc[i][j] = product(vb[kk][j], va[kk][i], acc[i][j], T{});
+      now = after(now);
+    };
+#pragma unroll 1
+    for (int j = 0; j < nk / 2; ++j) {
+      // stages 2 j and 2 j + 1 have landed, in flight may be the pair after them
+      wait(j + 1 < pairs);
+      step(false);
+      // nobody reads stages 2 j - 1 and 2 j any more: there goes the pair after the next
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      step(j + 2 < pairs);
+    }
+    if (nk & 1) {
+      wait(false);
+      step(false);
     }
   }
 
   // register 4 q + e of a lane: row l32, column 8 q + 4 lhi + e of the block
   const int l32 = lane & 31, lhi = lane >> 5;
-  const long long wm0 = m0 + wm * WM * 32, wn0 = n0 + wn * WN * 32;
   if (g.parts) {
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
@@ -378,18 +430,19 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   }
   __syncthreads();                                          // the ring is done with
   float* const stage = reinterpret_cast<float*>(lds) + wave * 32 * (WN * 32 + 4);
-  auto finish = [&](auto act) {
-    if (g.vec) finish_blocks<T, act(), 8, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
-    else finish_blocks<T, act(), 1, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
+  auto finish = [&](auto act, auto more) {
+    if (m0 + 64 * WM <= p.M && n0 + 64 * WN <= p.N) finish_blocks<T, act(), true, more(), WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
+    else finish_blocks<T, act(), false, more(), WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
   };
-  if constexpr (BO) finish(ic<WC_ACT_NONE>{});              // a gradient has no epilogue
+  // (a gradient has no epilogue, and the largest tiles, whose epilogue nothing runs beside, are left to products without a heavy one)
+  if constexpr (BO || AHEAD) finish(ic<WC_ACT_NONE>{}, std::false_type{});
   else {
     switch (p.e.act) {
-      case WC_ACT_RELU: finish(ic<WC_ACT_RELU>{}); break;
-      case WC_ACT_GELU: finish(ic<WC_ACT_GELU>{}); break;
-      case WC_ACT_GELU_TANH: finish(ic<WC_ACT_GELU_TANH>{}); break;
-      case WC_ACT_SILU: finish(ic<WC_ACT_SILU>{}); break;
-      default: finish(ic<WC_ACT_NONE>{});
+      case WC_ACT_RELU: finish(ic<WC_ACT_RELU>{}, std::true_type{}); break;
+      case WC_ACT_GELU: finish(ic<WC_ACT_GELU>{}, std::true_type{}); break;
+      case WC_ACT_GELU_TANH: finish(ic<WC_ACT_GELU_TANH>{}, std::true_type{}); break;
+      case WC_ACT_SILU: finish(ic<WC_ACT_SILU>{}, std::true_type{}); break;
+      default: finish(ic<WC_ACT_NONE>{}, std::true_type{});
     }
   }
 }
@@ -420,15 +473,14 @@ DmaArgs dma_args(const LinearProduct& p, const ProductPlan& plan, float* parts) 
   g.tiles_n = (int)ceil_div_ll(p.N, plan.tile.n);
   g.n_blocks = g.tiles_m * g.tiles_n * plan.s;
   g.per_xcd = ceil_div(g.n_blocks, kXcds);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p.e.y) | reinterpret_cast<uintptr_t>(p.e.z) | reinterpret_cast<uintptr_t>(p.e.res);
-  g.vec = p.N % 8 == 0 && at % 16 == 0;
+  g.vec = p.N % 4 == 0;
   return g;
 }
 
 // LDS of a product: the stages that its reduction has, and no less than the epilogue takes
 template <typename T, typename SH>
 size_t lds_of(const DmaArgs& g) {
-  const long long stages = std::min<long long>(SH::RING, std::max(1ll, ceil_div_ll(std::min(g.R_part, g.p.R), kDeep<T>)));
+  const long long pairs = std::max(1ll, ceil_div_ll(std::min(g.R_part, g.p.R), 2 * kDeep<T>)), stages = std::min<long long>(SH::RING, 2 * pairs);
   return std::max<size_t>((size_t)stages * SH::STAGE, SH::EPILOGUE);
 }
 template <typename SH> constexpr size_t kMostLds = SH::RING * SH::STAGE > SH::EPILOGUE ? SH::RING * SH::STAGE : SH::EPILOGUE;
@@ -453,9 +505,8 @@ int launch_pair(const DmaArgs& g, const DmaArgs& g2, void* stream) {
 }
 
 using Tile256 = Shape<4, 4, 4, true>;
-using Tile256x128 = Shape<4, 2, 3, false>;
-using Tile128 = Shape<2, 2, 4, false>;
-using Tile64 = Shape<1, 1, 4, false>;
+using Tile128 = Shape<2, 2, 5, false>;
+using Tile64 = Shape<1, 1, 5, false>;
 
 }  // namespace
 
@@ -473,8 +524,7 @@ int product_dma(const LinearProduct& p, const ProductPlan& plan, float* parts, i
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     if constexpr (sizeof(T) == 2) {
-      if (plan.tile.n == 256) return launch<T, Tile256>(g, stream);
-      if (plan.tile.m == 256) return launch<T, Tile256x128>(g, stream);
+      if (plan.tile.m == 256) return launch<T, Tile256>(g, stream);
     }
     return plan.tile.m == 128 ? launch<T, Tile128>(g, stream) : launch<T, Tile64>(g, stream);
   });

@@ -124,34 +124,49 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
 
 long long tiles_of(const LinearProduct& p, ProductTile t) { return ceil_div_ll(p.M, t.m) * ceil_div_ll(p.N, t.n); }
 
-ProductPlan plan_of(const LinearProduct& p, bool dma, int dtype) {
+// beside: steps of 64 elements of another product's tiles that run beside this one's
+ProductPlan plan_of(const LinearProduct& p, bool dma, int dtype, long long beside) {
   ProductPlan l = {dma, {64, 64}, 1, 0};
   const int forced = test_gemm_config();
-  if (forced >= 32 && forced <= 35 && dma) {
-    const ProductTile tiles[] = {{64, 64}, {128, 128}, {256, 128}, {256, 256}};
-    l.tile = tiles[dtype == WC_F32 ? std::min(forced - 32, 1) : forced - 32];
+  const bool heavy = p.e.act != WC_ACT_NONE || p.e.z || p.e.res;
+  if (forced >= 32 && forced <= 34 && dma) {
+    const ProductTile tiles[] = {{64, 64}, {128, 128}, {256, 256}};
+    l.tile = tiles[std::min(forced - 32, dtype == WC_F32 || heavy ? 1 : 2)];
   } else if (dma) {
-    const bool heavy = p.e.act != WC_ACT_NONE || p.e.z || p.e.res;
-    if (dtype != WC_F32 && tiles_of(p, {256, 256}) >= kCus && p.R >= (heavy ? 8192 : 2048)) l.tile = {256, 256};
-    else if (dtype != WC_F32 && p.R >= 128 && tiles_of(p, {256, 128}) >= 2 * kCus) l.tile = {256, 128};
-    else if (tiles_of(p, {128, 128}) >= 3 * kCus / 2) l.tile = {128, 128};
+    if (dtype != WC_F32 && !heavy && tiles_of(p, {256, 256}) >= kCus && p.R >= 2048) l.tile = {256, 256};
+    else if (tiles_of(p, {128, 128}) * std::max(1ll, p.R / 512) >= 3 * kCus / 2) l.tile = {128, 128};
   }
-  // as many as bring two tiles of 128 x 128 or four of 64 x 64 to a compute unit, of 256 elements and more (of small products 64), within 256 MB
-  // of sums
-  const long long tiles = tiles_of(p, l.tile), least = tiles * p.R < 64 * kCus ? 64 : 256;
-  long long s = l.tile.m == 256 ? 1 : std::min((l.tile.m == 128 ? 2 : 4) * kCus / std::max(tiles, 1ll), std::max(p.R / least, 1ll));
-  s = std::max(1ll, std::min(s, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
-  l.R_part = std::max(64ll, ceil_div_ll(ceil_div_ll(p.R, s), 64) * 64);
+  // Parts: the number with the least estimate.  Two tiles of 128 x 128 or four of 64 x 64 are on a compute unit at a time, whose workgroups take some 0.5
+  // or 0.35 us for 64 elements then (product_general_kernel's 2); a part's sums cost their way to memory and back, and the launch that adds them
+  const long long tiles = tiles_of(p, l.tile), steps = std::max(1ll, ceil_div_ll(p.R, 64)), slots = (l.tile.m == 128 ? 2 : 4) * kCus;
+  const double step_us = (l.tile.m == 128 ? 0.5 : dma ? 0.35 : 2) * (dtype == WC_F32 ? 4 : 1);
+  double least = 0;
+  long long best = 1;
+  const long long most = l.tile.m == 256 ? 1 : std::min(steps, std::max(1ll, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
+  for (long long s = 1; s <= most && s <= 4 * kCus; s += 1 + s / 8) {
+    const long long each = ceil_div_ll(steps, s), rounds = ceil_div_ll(tiles * ceil_div_ll(steps, each), slots);
+    const double us = std::max((double)(rounds * each), (double)(tiles * steps + beside) / slots) * step_us + (s > 1 ? 4 + 8e-6 * s * p.M * p.N / 4 : 0);
+    if (s == 1 || us < least) { least = us; best = s; }
+  }
+  l.R_part = ceil_div_ll(steps, best) * 64;
   l.s = (int)std::max(1ll, ceil_div_ll(p.R, l.R_part));
   return l;
 }
 
 }  // namespace
 
-ProductPlan product_plan(const LinearProduct& p, int dtype) { return plan_of(p, test_gemm_config() != 31 && product_dma_fits(p, dtype), dtype); }
+ProductPlan product_plan(const LinearProduct& p, int dtype, const LinearProduct* beside) {
+  const bool dma = test_gemm_config() != 31 && product_dma_fits(p, dtype);
+  if (!beside) return plan_of(p, dma, dtype, 0);
+  const ProductPlan other = plan_of(*beside, dma, dtype, 0);
+  const long long per = other.tile.m == 128 ? 1 : 4;           // (a step of a 64 x 64 tile is a quarter of one of 128 x 128)
+  const ProductPlan own = plan_of(p, dma, dtype, 0);
+  return plan_of(p, dma, dtype, tiles_of(*beside, other.tile) * ceil_div_ll(beside->R, 64) * (own.tile.m == 128 ? 1 : 4) / per);
+}
 
 size_t product_parts_bytes(const LinearProduct& p, int dtype) {
-  const int s = std::max(plan_of(p, true, dtype).s, plan_of(p, false, dtype).s);
+  // (what runs beside makes parts fewer)
+  const int s = std::max(plan_of(p, true, dtype, 0).s, plan_of(p, false, dtype, 0).s);
   return s > 1 ? (size_t)s * p.M * p.N * 4 : 0;
 }
 
