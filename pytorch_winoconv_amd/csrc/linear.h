@@ -82,12 +82,13 @@ struct LinearProduct {
   long long M, N, R;
   LinearEpilogue e;
 };
+inline bool linear_heavy(const LinearEpilogue& e) { return e.act != WC_ACT_NONE || e.z || e.res; }
 // linear_product.hip: how a product is run - on which kernel and tiles, in how many parts of the reduction - and the launches.  Parts leave
 // their sums (s, M, N) in fp32, which linear_join adds.
 struct ProductTile { int m, n; };
-struct ProductPlan { bool dma; ProductTile tile; int s; long long R_part; };
+struct ProductPlan { bool dma, few; ProductTile tile; int s; long long R_part; };
 ProductPlan product_plan(const LinearProduct& p, int dtype, const LinearProduct* beside);      // beside: runs in the same launch; null: none
-size_t product_parts_bytes(const LinearProduct& p, int dtype);      // whatever the operands' start
+size_t product_parts_bytes(const LinearProduct& p, int dtype, const LinearProduct* beside);      // enough for every start of the operands and every epilogue
 int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream);
 // both, in one launch where their plans allow it
 int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream);

@@ -35,6 +35,11 @@ int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
   return WC_OK;
 }
 
+// (a plan never has more parts than the workspace was sized for; checked all the same, since they would be written behind it)
+bool parts_fit(const LinearProduct& p, const ProductPlan& plan, size_t at, size_t end) {
+  return plan.s == 1 || at + (size_t)plan.s * p.M * p.N * 4 <= end;
+}
+
 // Rows that are no multiple of 16 bytes are copied to ones that are, for the kernel that brings them to LDS without registers, where the product is
 // worth it: the copy is a launch and a pass over the operands.
 bool widen_pays(long long M, long long N, long long R) { return (double)M * N * R >= kWidenPays; }
@@ -62,7 +67,7 @@ Forward forward_plan(const wc_linear_desc* d, const void* x, const void* w, cons
   }
   f.p = {x, w, f.widen ? ld : d->C, f.widen ? ld : d->C, false, false, d->rows, d->K, d->C, {bias, res, y, z, d->activation, d->residual_after != 0, 0}};
   f.scratch_at = at;
-  f.bytes = at + rounded(product_parts_bytes(f.p, d->dtype));
+  f.bytes = at + rounded(product_parts_bytes(f.p, d->dtype, nullptr));
   return f;
 }
 
@@ -118,9 +123,9 @@ Backward backward_plan(const wc_linear_desc* d, const wc_linear_gradients* g, ch
   b.sums_at = at;
   at += rounded(linear_sums_bytes(f.slope));
   b.dx_at = at;
-  if (g->dx) at += rounded(product_parts_bytes(b.dx, d->dtype));
+  if (g->dx) at += rounded(product_parts_bytes(b.dx, d->dtype, nullptr));
   b.dw_at = at;
-  if (g->dw) at += rounded(product_parts_bytes(b.dw, d->dtype));
+  if (g->dw) at += rounded(product_parts_bytes(b.dw, d->dtype, &b.dx));
   b.bytes = at;
   return b;
 }
@@ -145,6 +150,9 @@ int wc_linear_forward(const wc_linear_desc* d, const void* x, const void* w, con
   if (int rc = check_workspace(workspace, workspace_bytes, need, "wc_linear_forward")) return rc;
   char* const ws = static_cast<char*>(workspace);
   const Forward f = forward_plan(d, x, w, bias, residual, y, z, ws);
+  float* const parts = reinterpret_cast<float*>(ws + f.scratch_at);
+  const ProductPlan plan = product_plan(f.p, d->dtype, nullptr);
+  if (!parts_fit(f.p, plan, f.scratch_at, need)) return fail(WC_ERR_WORKSPACE, "wc_linear_forward: %d parts do not fit the workspace", plan.s);
   if (f.widen) {
     LinearPrepare before = {};
     before.copies[0] = f.copies[0];
@@ -152,8 +160,6 @@ int wc_linear_forward(const wc_linear_desc* d, const void* x, const void* w, con
     before.n_copies = 2;
     if (int rc = linear_prepare(before, d->dtype, nullptr, stream)) return rc;
   }
-  float* const parts = reinterpret_cast<float*>(ws + f.scratch_at);
-  const ProductPlan plan = product_plan(f.p, d->dtype, nullptr);
   if (int rc = product_run(f.p, plan, parts, d->dtype, stream)) return rc;
   const LinearJoin join = {f.p.e, parts, plan.s, f.p.M, f.p.N};
   return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
@@ -180,10 +186,12 @@ int wc_linear_backward(const wc_linear_desc* d, const wc_linear_gradients* g, vo
   char* const ws = static_cast<char*>(workspace);
   const Backward b = backward_plan(d, g, ws);
   auto at = [&](size_t n) { return reinterpret_cast<float*>(ws + n); };
-  if (int rc = linear_prepare(b.before, d->dtype, at(b.sums_at), stream)) return rc;
   LinearJoin joins[2];
   int n = 0;
   const ProductPlan dx = product_plan(b.dx, d->dtype, nullptr), dw = product_plan(b.dw, d->dtype, &b.dx);      // dw's bits do not hang on whether dx is asked for
+  if ((g->dx && !parts_fit(b.dx, dx, b.dx_at, b.dw_at)) || (g->dw && !parts_fit(b.dw, dw, b.dw_at, need)))
+    return fail(WC_ERR_WORKSPACE, "wc_linear_backward: %d and %d parts do not fit the workspace", dx.s, dw.s);
+  if (int rc = linear_prepare(b.before, d->dtype, at(b.sums_at), stream)) return rc;
   if (g->dx) joins[n++] = {b.dx.e, at(b.dx_at), dx.s, b.dx.M, b.dx.N};
   if (g->dw) joins[n++] = {b.dw.e, at(b.dw_at), dw.s, b.dw.M, b.dw.N};
   int rc = WC_OK;

@@ -45,9 +45,9 @@ __device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c, float) {
 template <typename T> constexpr int kDeep = 64 / sizeof(T);
 template <typename T> constexpr int kChunk = 16 / sizeof(T);
 
-// One operand of a tile of 64 W rows of the result
-template <typename T, int W, bool OUTER> struct DmaOperand {
-  static constexpr int BT = 64 * W, BYTES = BT * 64, LOADS = W;           // a stage, 1 KB loads per wavefront
+// One operand of a tile of BT rows of the result, brought by NW wavefronts
+template <typename T, int BT, int NW, bool OUTER> struct DmaOperand {
+  static constexpr int BYTES = BT * 64, LOADS = BT / (16 * NW);           // a stage, 1 KB loads per wavefront
   static constexpr int ES = sizeof(T), EPC = kChunk<T>, CHUNKS = BT / EPC, RPI = 64 / CHUNKS;      // outer: chunks of a row, rows of a load
   static_assert(RPI >= 1, "a load holds whole rows");
   const unsigned char* base;       // of the next stage to be queued
@@ -57,7 +57,7 @@ template <typename T, int W, bool OUTER> struct DmaOperand {
   int chunk;                       // inner: the lane's chunk of a stage's row
 
   // outer: the exchange of a row's chunks
-  static __device__ __forceinline__ int exchange(int row) { return ES == 4 ? (row >> 2 & 1) * 8 : W == 1 ? (row >> 1 & 1) * 4 : (row & 3) * 4; }
+  static __device__ __forceinline__ int exchange(int row) { return ES == 4 ? (row >> 2 & 1) * 8 : BT == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4; }
   static __device__ __forceinline__ int swizzle(int r) { return (((r >> 1) ^ (r >> 3)) & 1) | ((r >> 2) & 1) << 1; }
 
   __device__ __forceinline__ void start(const void* p, long long ld, long long row0, long long rows, long long begin, long long end, int wave, int lane) {
@@ -73,7 +73,7 @@ template <typename T, int W, bool OUTER> struct DmaOperand {
         const int c = lane % CHUNKS ^ exchange(row);
         voff[i] = row0 + c * EPC < rows ? (unsigned)(row * ld * ES + c * 16) : kOutside;
       } else {
-        const int row = (wave + 4 * i) * 16 + lane / 4;
+        const int row = (wave + NW * i) * 16 + lane / 4;
         chunk = lane % 4 ^ swizzle(row);
         voff[i] = row0 + row < rows ? (unsigned)(row * ld * ES + chunk * 16) : kOutside;
       }
@@ -94,7 +94,7 @@ template <typename T, int W, bool OUTER> struct DmaOperand {
   }
   // queues load i of them, into LDS at `lds` and `lds2`
   template <bool PAIR> __device__ __forceinline__ void queue(unsigned lds, unsigned lds2, int wave, int i) const {
-    const unsigned to = (OUTER ? wave * LOADS + i : wave + 4 * i) * 1024;
+    const unsigned to = (OUTER ? wave * LOADS + i : wave + NW * i) * 1024;
     dma16(d, voff[i] | out, lds + to);
     if constexpr (PAIR) dma16(d2, voff[i] | out2, lds2 + to);
   }
@@ -229,34 +229,35 @@ __device__ __forceinline__ void finish_blocks(const LinearEpilogue& e, const f32
   }
 }
 
-// Template of a product: blocks of a wavefront, stages of the ring, whether the first half of a stage is read while the last one of the stage before
-// is multiplied (a wavefront alone on its SIMD waits for every read that is not ahead)
-template <int WM_, int WN_, int RING_, bool AHEAD_> struct Shape {
-  static constexpr int WM = WM_, WN = WN_, RING = RING_;
+// Template of a product: blocks of a wavefront, wavefronts, stages of the ring, whether the first half of a stage is read while the last one of the
+// stage before is multiplied (a wavefront alone on its SIMD waits for every read that is not ahead)
+template <int WM_, int WN_, int NWM_, int NWN_, int RING_, bool AHEAD_> struct Shape {
+  static constexpr int WM = WM_, WN = WN_, NWM = NWM_, NWN = NWN_, RING = RING_, NW = NWM * NWN, BM = 32 * WM * NWM, BN = 32 * WN * NWN;
   static constexpr bool AHEAD = AHEAD_;
-  static constexpr size_t STAGE = 64 * 64 * (WM + WN), EPILOGUE = 4 * 32 * (WN * 32 + 4) * 4;
+  static constexpr size_t STAGE = 64 * (BM + BN), EPILOGUE = NW * 32 * (WN * 32 + 4) * 4;
 };
 
 template <typename T, typename SH, bool AO, bool BO>
 __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, unsigned char* lds) {
   constexpr int WM = SH::WM, WN = SH::WN, kRing = SH::RING;
   constexpr bool AHEAD = SH::AHEAD;
-  using A = DmaOperand<T, WM, AO>;
-  using B = DmaOperand<T, WN, BO>;
-  constexpr int STAGE = A::BYTES + B::BYTES, L = WM + WN;
+  constexpr int NWM = SH::NWM, NWN = SH::NWN, BM = SH::BM, BN = SH::BN;
+  using A = DmaOperand<T, BM, NWM * NWN, AO>;
+  using B = DmaOperand<T, BN, NWM * NWN, BO>;
+  constexpr int STAGE = A::BYTES + B::BYTES, L = A::LOADS + B::LOADS;
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   const int blk = xcd_remap(hw_block, g.per_xcd);
   if (blk >= g.n_blocks) return;
   // a band of tiles along M, then along N: the workgroups of an XCD that run together share the rows of few tiles of either operand
   const int tiles = g.tiles_m * g.tiles_n, s = blk / tiles, t = blk % tiles;
   const int band = t / (kBand * g.tiles_n), in_band = t % (kBand * g.tiles_n), high = min(kBand, g.tiles_m - band * kBand);
-  const long long m0 = (long long)(band * kBand + in_band % high) * (64 * WM), n0 = (long long)(in_band / high) * (64 * WN);
+  const long long m0 = (long long)(band * kBand + in_band % high) * BM, n0 = (long long)(in_band / high) * BN;
   const LinearProduct& p = g.p;
   const long long begin = s * g.R_part, end = min(p.R, begin + g.R_part);
   const int nk = end > begin ? (int)((end - begin + kDeep<T> - 1) / kDeep<T>) : 0;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / NWN, wn = wave % NWN;
   A a;
   B b;
   a.start(p.a, p.lda, m0, p.M, begin, end, wave, lane);
@@ -267,8 +268,8 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   auto after = [](int slot) { return slot + 1 == kRing ? 0 : slot + 1; };
   auto queue = [&](int q) {                         // load q of the L of a stage, or of two
     const unsigned at = lds0 + to * STAGE, at2 = lds0 + after(to) * STAGE;
-    if (q < WM) a.template queue<PAIR>(at, at2, wave, q);
-    else b.template queue<PAIR>(at + A::BYTES, at2 + A::BYTES, wave, q - WM);
+    if (q < A::LOADS) a.template queue<PAIR>(at, at2, wave, q);
+    else b.template queue<PAIR>(at + A::BYTES, at2 + A::BYTES, wave, q - A::LOADS);
   };
   auto aim = [&] {
     a.template aim<PAIR>(left);
@@ -431,7 +432,7 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   __syncthreads();                                          // the ring is done with
   float* const stage = reinterpret_cast<float*>(lds) + wave * 32 * (WN * 32 + 4);
   auto finish = [&](auto act, auto more) {
-    if (m0 + 64 * WM <= p.M && n0 + 64 * WN <= p.N) finish_blocks<T, act(), true, more(), WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
+    if (m0 + BM <= p.M && n0 + BN <= p.N) finish_blocks<T, act(), true, more(), WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
     else finish_blocks<T, act(), false, more(), WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
   };
   // (a gradient has no epilogue, and the largest tiles, whose epilogue nothing runs beside, are left to products without a heavy one)
@@ -447,10 +448,10 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   }
 }
 
-template <typename SH> constexpr int kMinWaves = SH::WM * SH::WN > 8 ? 1 : 2;
+template <typename SH> constexpr int kMinWaves = SH::AHEAD ? 1 : 2;
 
 template <typename T, typename SH, bool AO, bool BO>
-__global__ __launch_bounds__(256, kMinWaves<SH>) void product_dma_kernel(DmaArgs g) {
+__global__ __launch_bounds__(64 * SH::NW, kMinWaves<SH>) void product_dma_kernel(DmaArgs g) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   product_block<T, SH, AO, BO>(g, blockIdx.x, lds);
 }
@@ -485,12 +486,22 @@ size_t lds_of(const DmaArgs& g) {
 }
 template <typename SH> constexpr size_t kMostLds = SH::RING * SH::STAGE > SH::EPILOGUE ? SH::RING * SH::STAGE : SH::EPILOGUE;
 
+// 256 x 256 with a heavy epilogue takes two wavefronts to a SIMD, one of which finishes results while the other waits for its own.  us, bf16
+// 8192 x 2048 -> 8192, gelu with z: four wavefronts 343, eight 309 (128 x 128 349); 4096 x 4096 -> 4096, bias alone 122, 128 (153)
+using Tile256 = Shape<4, 4, 2, 2, 4, true>;
+using Tile256Heavy = Shape<4, 2, 2, 4, 5, false>;
+using Tile128 = Shape<2, 2, 2, 2, 5, false>;
+using Tile64 = Shape<1, 1, 2, 2, 5, false>;
+
 template <typename T, typename SH>
 int launch(const DmaArgs& g, void* stream) {
   const LinearProduct& p = g.p;
-  auto fn = p.a_outer ? &product_dma_kernel<T, SH, true, true> : p.b_outer ? &product_dma_kernel<T, SH, false, true> : &product_dma_kernel<T, SH, false, false>;
+  auto fn = &product_dma_kernel<T, SH, false, false>;
+  if constexpr (!std::is_same<SH, Tile256Heavy>::value) {      // (gradients have no epilogue)
+    if (p.b_outer) fn = p.a_outer ? &product_dma_kernel<T, SH, true, true> : &product_dma_kernel<T, SH, false, true>;
+  }
   if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(fn), kMostLds<SH>)) return rc;
-  hipLaunchKernelGGL(fn, dim3((unsigned)(g.per_xcd * kXcds)), dim3(256), (lds_of<T, SH>(g)), as_stream(stream), g);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(g.per_xcd * kXcds)), dim3(64 * SH::NW), (lds_of<T, SH>(g)), as_stream(stream), g);
   WC_CHECK_LAUNCH("product_dma_kernel");
   return WC_OK;
 }
@@ -503,10 +514,6 @@ int launch_pair(const DmaArgs& g, const DmaArgs& g2, void* stream) {
   WC_CHECK_LAUNCH("product_pair_kernel");
   return WC_OK;
 }
-
-using Tile256 = Shape<4, 4, 4, true>;
-using Tile128 = Shape<2, 2, 5, false>;
-using Tile64 = Shape<1, 1, 5, false>;
 
 }  // namespace
 
@@ -524,7 +531,7 @@ int product_dma(const LinearProduct& p, const ProductPlan& plan, float* parts, i
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     if constexpr (sizeof(T) == 2) {
-      if (plan.tile.m == 256) return launch<T, Tile256>(g, stream);
+      if (plan.tile.m == 256) return linear_heavy(p.e) ? launch<T, Tile256Heavy>(g, stream) : launch<T, Tile256>(g, stream);
     }
     return plan.tile.m == 128 ? launch<T, Tile128>(g, stream) : launch<T, Tile64>(g, stream);
   });

@@ -122,31 +122,108 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
     }
 }
 
+// Few rows (at most 16 of M, 16-bit types, both operands with the reduction innermost): one pass over B, which bounds it.  A workgroup of 16 wavefronts takes 16
+// rows of B, whose reduction the wavefronts share, 64 elements at a time - 32 bytes a lane, straight into the operand of a 16 x 16 x 32 instruction, with the
+// same ones of A beside them -; their sums meet in LDS, so there are no parts and no second launch.  us, LDS-DMA and parts | this: bf16 1 x 4096 -> 1000
+// 11.2 | 10.
+constexpr int kFewWaves = 16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(LinearProduct p) {
+  __shared__ float sums[kFewWaves][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
+  const long long n0 = (long long)blockIdx.x * 16;
+  const T* const w = static_cast<const T*>(p.b) + min(n0 + r, p.N - 1) * p.ldb + c * 16;
+  const T* const x = static_cast<const T*>(p.a) + min((long long)r, p.M - 1) * p.lda + c * 16;
+  const bool row = r < p.M;
+  const int chunks = (int)((p.R + 63) / 64);
+  using V = Pack<T, 8>;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int AT_ONCE = 4;
+  V zero;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) zero.v[e] = static_cast<T>(0.f);
+  auto multiply = [&](const V& a, const V& b) {
+    if constexpr (std::is_same<T, half_t>::value) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+    else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  };
+  for (int k0 = wave; k0 < chunks; k0 += AT_ONCE * kFewWaves) {
+    V wv[AT_ONCE][2], xv[AT_ONCE][2];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long k = (long long)(k0 + u * kFewWaves) * 64 + h * 8;
+        const bool in = k + c * 16 < p.R;           // (R is a multiple of eight, or rows have zeros up to one)
+        wv[u][h] = in ? *reinterpret_cast<const V*>(w + k) : zero;
+        xv[u][h] = in && row ? *reinterpret_cast<const V*>(x + k) : zero;
+      }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) multiply(wv[u][h], xv[u][h]);
+  }
+  // register e of a lane: row 4 c + e of B, row r of A
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[wave][r][4 * c + e] = acc[e];
+  __syncthreads();
+  const int m = threadIdx.x >> 4, n = threadIdx.x & 15;
+  if (m >= p.M || n0 + n >= p.N) return;            // (m of the first 256 threads is below 16, p.M is at most that)
+  float v = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewWaves; ++s) v += sums[s][m][n];
+  finish<T>(p.e, m, n0 + n, p.N, v);
+}
+// ... for a B of up to 16 MB: parts have more loads in flight (205 MB: 43.9 | 67)
+bool few_rows_pay(const LinearProduct& p, int dtype) {
+  return dtype != WC_F32 && !p.a_outer && !p.b_outer && p.M <= 16 && p.N * p.R <= 8 << 20;
+}
+
 long long tiles_of(const LinearProduct& p, ProductTile t) { return ceil_div_ll(p.M, t.m) * ceil_div_ll(p.N, t.n); }
 
-// beside: steps of 64 elements of another product's tiles that run beside this one's
-ProductPlan plan_of(const LinearProduct& p, bool dma, int dtype, long long beside) {
-  ProductPlan l = {dma, {64, 64}, 1, 0};
+// What 64 elements of the reduction take a workgroup, alone on its compute unit and with as many as it holds, and what the epilogue takes, plain and
+// heavy, in us; measured on 16-bit products of 4096 and 8192 squared (fp32 instructions: 128 x 128 seven times, 64 x 64 five times that, alone four times)
+struct TileCost { ProductTile tile; int slots; double alone, full, plain, heavy; };
+constexpr TileCost kTileCosts[] = {{{64, 64}, 4, 0.55, 1.1, 1, 3}, {{128, 128}, 2, 0.6, 1.17, 2, 6}, {{256, 256}, 1, 1.85, 1.85, 5, 18}};
+constexpr TileCost kGeneralCost = {{64, 64}, 4, 2, 2, 2, 4};
+
+// The least estimate over tiles and numbers of parts; parts' sums cost their way to memory and back, and the launch that adds them.  beside: us that another
+// product keeps the chip busy in the same launch, which leaves the tile as it is and makes parts fewer
+ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, double beside, double* busy = nullptr) {
+  ProductPlan l = {dma, false, {64, 64}, 1, 0};
   const int forced = test_gemm_config();
-  const bool heavy = p.e.act != WC_ACT_NONE || p.e.z || p.e.res;
-  if (forced >= 32 && forced <= 34 && dma) {
-    const ProductTile tiles[] = {{64, 64}, {128, 128}, {256, 256}};
-    l.tile = tiles[std::min(forced - 32, dtype == WC_F32 || heavy ? 1 : 2)];
-  } else if (dma) {
-    if (dtype != WC_F32 && !heavy && tiles_of(p, {256, 256}) >= kCus && p.R >= 2048) l.tile = {256, 256};
-    else if (tiles_of(p, {128, 128}) * std::max(1ll, p.R / 512) >= 3 * kCus / 2) l.tile = {128, 128};
+  if (forced < 0 && dma && few_rows_pay(p, dtype)) {
+    l.few = true;
+    l.R_part = std::max(p.R, 1ll);
+    return l;
   }
-  // Parts: the number with the least estimate.  Two tiles of 128 x 128 or four of 64 x 64 are on a compute unit at a time, whose workgroups take some 0.5
-  // or 0.35 us for 64 elements then (product_general_kernel's 2); a part's sums cost their way to memory and back, and the launch that adds them
-  const long long tiles = tiles_of(p, l.tile), steps = std::max(1ll, ceil_div_ll(p.R, 64)), slots = (l.tile.m == 128 ? 2 : 4) * kCus;
-  const double step_us = (l.tile.m == 128 ? 0.5 : dma ? 0.35 : 2) * (dtype == WC_F32 ? 4 : 1);
-  double least = 0;
+  const long long steps = std::max(1ll, ceil_div_ll(p.R, 64)), room = std::max(1ll, (256ll << 20) / std::max(4 * p.M * p.N, 1ll));      // 256 MB of sums
+  double least = -1;
   long long best = 1;
-  const long long most = l.tile.m == 256 ? 1 : std::min(steps, std::max(1ll, (256ll << 20) / std::max(4 * p.M * p.N, 1ll)));
-  for (long long s = 1; s <= most && s <= 4 * kCus; s += 1 + s / 8) {
-    const long long each = ceil_div_ll(steps, s), rounds = ceil_div_ll(tiles * ceil_div_ll(steps, each), slots);
-    const double us = std::max((double)(rounds * each), (double)(tiles * steps + beside) / slots) * step_us + (s > 1 ? 4 + 8e-6 * s * p.M * p.N / 4 : 0);
-    if (s == 1 || us < least) { least = us; best = s; }
+  auto consider = [&](const TileCost& c, double beside) {
+    const double f = dtype == WC_F32 ? (c.tile.m == 64 ? 5 : 7) : 1, f_alone = dtype == WC_F32 ? 4 : 1;
+    const long long tiles = tiles_of(p, c.tile), slots = (long long)c.slots * kCus, most = c.tile.m == 256 ? 1 : std::min({steps, room, 4ll * kCus});
+    for (long long s = 1; s <= most; s += 1 + s / 8) {
+      const long long each = ceil_div_ll(steps, s), n = tiles * ceil_div_ll(steps, each);
+      const double end = heavy && s == 1 ? c.heavy : c.plain;
+      const double rounds = n <= slots ? (double)n / slots : (double)ceil_div_ll(n, slots);
+      const double us = std::max({each * c.alone * f_alone + end, rounds * (each * c.full * f + end), rounds * (each * c.full * f + end) * 0.9 + beside}) + (s > 1 ? 8 + 2e-6 * s * p.M * p.N : 0);
+      if (least >= 0 && us >= least) continue;
+      least = us;
+      best = s;
+      l.tile = c.tile;
+      if (busy) *busy = c.tile.m == 256 ? 0 : rounds * (each * c.full * f + end);      // (the largest tiles share no launch)
+    }
+  };
+  if (!dma) consider(kGeneralCost, 0);
+  else if (forced >= 32 && forced <= 34) consider(kTileCosts[std::min(forced - 32, dtype == WC_F32 ? 1 : 2)], 0);
+  else
+    for (const TileCost& c : kTileCosts)
+      if (c.tile.m < 256 || dtype != WC_F32) consider(c, 0);
+  if (beside > 0 && l.tile.m < 256) {
+    const TileCost c = dma ? kTileCosts[l.tile.m / 128] : kGeneralCost;
+    least = -1;
+    consider(c, beside);
   }
   l.R_part = ceil_div_ll(steps, best) * 64;
   l.s = (int)std::max(1ll, ceil_div_ll(p.R, l.R_part));
@@ -157,22 +234,36 @@ ProductPlan plan_of(const LinearProduct& p, bool dma, int dtype, long long besid
 
 ProductPlan product_plan(const LinearProduct& p, int dtype, const LinearProduct* beside) {
   const bool dma = test_gemm_config() != 31 && product_dma_fits(p, dtype);
-  if (!beside) return plan_of(p, dma, dtype, 0);
-  const ProductPlan other = plan_of(*beside, dma, dtype, 0);
-  const long long per = other.tile.m == 128 ? 1 : 4;           // (a step of a 64 x 64 tile is a quarter of one of 128 x 128)
-  const ProductPlan own = plan_of(p, dma, dtype, 0);
-  return plan_of(p, dma, dtype, tiles_of(*beside, other.tile) * ceil_div_ll(beside->R, 64) * (own.tile.m == 128 ? 1 : 4) / per);
+  double busy = 0;
+  if (beside) plan_of(*beside, dma, false, dtype, 0, &busy);
+  return plan_of(p, dma, linear_heavy(p.e), dtype, busy);
 }
 
-size_t product_parts_bytes(const LinearProduct& p, int dtype) {
-  // (what runs beside makes parts fewer)
-  const int s = std::max(plan_of(p, true, dtype, 0).s, plan_of(p, false, dtype, 0).s);
+size_t product_parts_bytes(const LinearProduct& p, int dtype, const LinearProduct* beside) {
+  double busy = 0;
+  long long s = 1;
+  for (const bool dma : {true, false}) {
+    if (beside) plan_of(*beside, dma, false, dtype, 0, &busy);
+    for (const bool heavy : {true, false}) s = std::max<long long>(s, plan_of(p, dma, heavy, dtype, busy).s);
+  }
   return s > 1 ? (size_t)s * p.M * p.N * 4 : 0;
 }
 
 int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream) {
   const long long tiles = tiles_of(p, plan.tile);
   if (tiles * plan.s >= (1ll << 31) - 8) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
+  if (plan.few) {
+    return dispatch_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      if constexpr (sizeof(T) == 2) {
+        hipLaunchKernelGGL(product_few_kernel<T>, dim3((unsigned)ceil_div_ll(p.N, 16)), dim3(64 * kFewWaves), 0, as_stream(stream), p);
+        WC_CHECK_LAUNCH("product_few_kernel");
+        return WC_OK;
+      } else {
+        return fail(WC_ERR_UNSUPPORTED, "product_few_kernel: 16-bit types");
+      }
+    });
+  }
   if (plan.dma) return product_dma(p, plan, parts, dtype, stream);
   GeneralArgs g;
   g.p = p;

@@ -128,3 +128,21 @@ def test_the_oracle_of_8_bits_is_half_a_step_off():
         assert torch.equal(lo.pack(v.to(t))[0], codes) and torch.equal(lo.pack(v.to(t))[1], exps)
     codes, exps = lo.pack(torch.tensor([[3e-45, 0.0, 1.0], [float("inf"), 1.0, 0.0], [0.0, 0.0, 0.0]]), keep_sign=True)
     assert codes.tolist() == [[1, 0, 64], [0, 0, 0], [0, 0, 0]] and exps.tolist() == [[-6], [127], [-126]]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: where there is no GPU a launch fails and nothing is read")
+def test_a_workspace_of_the_stated_size_is_enough():
+    """Whatever stands in the epilogue and wherever the operands start, which the sizes are asked for without."""
+    import random
+    lib, rng, n = _lib.load(), random.Random(7), ctypes.c_size_t()
+    for _ in range(1500):
+        d = _lib.LinearDesc(rng.choice([1, 3, 8, 16, 17, 64, 300, 777, 5000, 200000]), rng.choice([1, 8, 40, 77, 264, 1000, 4096, 25088]),
+                            rng.choice([1, 8, 77, 264, 328, 1000, 4096]), rng.randrange(3), rng.randrange(5), rng.randrange(2))
+        at = lambda p=1.0: (1 << 30) + rng.choice([0, 0, 2]) if rng.random() < p else None  # noqa: E731
+        assert lib.wc_linear_workspace_bytes(ctypes.byref(d), ctypes.byref(n)) == 0
+        rc = lib.wc_linear_forward(ctypes.byref(d), at(), at(), at(0.5), at(0.5), at(), at(0.5), ctypes.c_void_p(1 << 40), n.value, None)
+        assert rc == -4, (rc, lib.wc_last_error(), d.rows, d.C, d.K)
+        g = _lib.LinearGradients(dy=at(), x=at(), x_exponents=at(0.3), w=at(), z=at(), z_exponents=at(0.3), dx=at(0.7), dw=at(), dw_dtype=0, db=at(0.5), db_dtype=0, dz=at(0.3))
+        assert lib.wc_linear_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(g), ctypes.byref(n)) == 0
+        rc = lib.wc_linear_backward(ctypes.byref(d), ctypes.byref(g), ctypes.c_void_p(1 << 40), n.value, None)
+        assert rc == -4, (rc, lib.wc_last_error(), d.rows, d.C, d.K)
