@@ -122,24 +122,25 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
     }
 }
 
-// Few rows (at most 16 of M, 16-bit types, both operands with the reduction innermost): one pass over B, which bounds it.  A workgroup of 16 wavefronts takes 16
-// rows of B, whose reduction the wavefronts share, 64 elements at a time - 32 bytes a lane, straight into the operand of a 16 x 16 x 32 instruction, with the
-// same ones of A beside them -; their sums meet in LDS, so there are no parts and no second launch.  us, LDS-DMA and parts | this: bf16 1 x 4096 -> 1000
-// 11.2 | 10.
+// Few rows (at most 16 of M, 16-bit types, both operands with the reduction innermost): one pass over B, which bounds it.  A workgroup of 16 wavefronts takes NR
+// rows of B (4, 8 or 16, no less than there are of A: few, so that every compute unit has some), whose reduction the wavefronts share, 64 elements
+// at a time - both halves of a line of the L2, one after the other, straight into the operands of two 16 x 16 x 32 instructions.  The 16 rows of
+// an instruction are NR rows at 16 / NR places of the reduction, of A as of B; of its results those of two equal places count.  The sums meet in LDS, so there
+// are no parts and no second launch.
 constexpr int kFewWaves = 16;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-template <typename T>
+template <typename T, int NR>
 __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(LinearProduct p) {
-  __shared__ float sums[kFewWaves][16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
-  const long long n0 = (long long)blockIdx.x * 16;
-  const T* const w = static_cast<const T*>(p.b) + min(n0 + r, p.N - 1) * p.ldb + c * 16;
-  const T* const x = static_cast<const T*>(p.a) + min((long long)r, p.M - 1) * p.lda + c * 16;
+  constexpr int PLACES = 16 / NR, AT_ONCE = 4;
+  __shared__ float sums[kFewWaves * PLACES][NR][NR + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane % NR, place = (lane & 15) / NR, c = lane >> 4;
+  const long long n0 = (long long)blockIdx.x * NR;
+  const T* const w = static_cast<const T*>(p.b) + min(n0 + r, p.N - 1) * p.ldb;
+  const T* const x = static_cast<const T*>(p.a) + min((long long)r, p.M - 1) * p.lda;
   const bool row = r < p.M;
-  const int chunks = (int)((p.R + 63) / 64);
+  const int chunks = (int)((p.R + 64 * PLACES - 1) / (64 * PLACES));
   using V = Pack<T, 8>;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  constexpr int AT_ONCE = 4;
   V zero;
 #pragma unroll
   for (int e = 0; e < 8; ++e) zero.v[e] = static_cast<T>(0.f);
@@ -153,8 +154,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(LinearProdu
     for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long long k = (long long)(k0 + u * kFewWaves) * 64 + h * 8;
-        const bool in = k + c * 16 < p.R;           // (R is a multiple of eight, or rows have zeros up to one)
+        const long long k = ((long long)(k0 + u * kFewWaves) * PLACES + place) * 64 + h * 32 + c * 8;
+        const bool in = k < p.R;                    // (R is a multiple of eight, or rows have zeros up to one)
         wv[u][h] = in ? *reinterpret_cast<const V*>(w + k) : zero;
         xv[u][h] = in && row ? *reinterpret_cast<const V*>(x + k) : zero;
       }
@@ -163,20 +164,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(LinearProdu
 #pragma unroll
       for (int h = 0; h < 2; ++h) multiply(wv[u][h], xv[u][h]);
   }
-  // register e of a lane: row 4 c + e of B, row r of A
+  // register e of a lane: row 4 c + e of B's sixteen, row lane % 16 of A's
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sums[wave][r][4 * c + e] = acc[e];
+  for (int e = 0; e < 4; ++e)
+    if ((4 * c + e) / NR == place) sums[wave * PLACES + place][r][(4 * c + e) % NR] = acc[e];
   __syncthreads();
-  const int m = threadIdx.x >> 4, n = threadIdx.x & 15;
-  if (m >= p.M || n0 + n >= p.N) return;            // (m of the first 256 threads is below 16, p.M is at most that)
+  const int m = threadIdx.x / NR, n = threadIdx.x % NR;
+  if (m >= NR || m >= p.M || n0 + n >= p.N) return;
   float v = 0.f;
-#pragma unroll
-  for (int s = 0; s < kFewWaves; ++s) v += sums[s][m][n];
+#pragma unroll 16
+  for (int s = 0; s < kFewWaves * PLACES; ++s) v += sums[s][m][n];
   finish<T>(p.e, m, n0 + n, p.N, v);
 }
-// ... for a B of up to 16 MB: parts have more loads in flight (205 MB: 43.9 | 67)
+// ... for a B of up to 4 MB, which is over before a second launch would begin; more loads are in flight in parts of tiles.  us, fp16, tiles and parts | this:
+// 1 x 1024 -> 1024 10.2 | 6.3, 8 x 2048 -> 2048 10.3 | 10.5, 8 x 4096 -> 4096 12.4 | 20.4
 bool few_rows_pay(const LinearProduct& p, int dtype) {
-  return dtype != WC_F32 && !p.a_outer && !p.b_outer && p.M <= 16 && p.N * p.R <= 8 << 20;
+  return dtype != WC_F32 && !p.a_outer && !p.b_outer && p.M <= 16 && p.N * p.R <= 2 << 20;
 }
 
 long long tiles_of(const LinearProduct& p, ProductTile t) { return ceil_div_ll(p.M, t.m) * ceil_div_ll(p.N, t.n); }
@@ -256,7 +259,9 @@ int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, i
     return dispatch_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
       if constexpr (sizeof(T) == 2) {
-        hipLaunchKernelGGL(product_few_kernel<T>, dim3((unsigned)ceil_div_ll(p.N, 16)), dim3(64 * kFewWaves), 0, as_stream(stream), p);
+        const int nr = p.M <= 4 ? 4 : p.M <= 8 ? 8 : 16;
+        auto fn = nr == 4 ? &product_few_kernel<T, 4> : nr == 8 ? &product_few_kernel<T, 8> : &product_few_kernel<T, 16>;
+        hipLaunchKernelGGL(fn, dim3((unsigned)ceil_div_ll(p.N, nr)), dim3(64 * kFewWaves), 0, as_stream(stream), p);
         WC_CHECK_LAUNCH("product_few_kernel");
         return WC_OK;
       } else {

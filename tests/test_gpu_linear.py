@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 # rows, C, K: one of everything, odd, around tiles and stages, long reductions, few and many rows
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (2, 31, 65), (8, 64, 64), (16, 512, 40), (33, 40, 72), (64, 64, 64), (65, 33, 17), (130, 257, 96), (200, 72, 264), (7, 1000, 3),
           (513, 16, 300), (257, 136, 520), (1, 4096, 24), (5, 2056, 1000), (17, 3000, 128), (1025, 8, 8), (300, 300, 301), (1000, 520, 776),
-          (2000, 96, 640), (600, 501, 403), (600, 504, 403), (600, 501, 408)]
+          (2000, 96, 640), (600, 501, 403), (600, 504, 403), (600, 501, 408), (4, 4104, 1001), (6, 136, 50), (9, 1032, 333), (16, 8, 17)]
 
 
 def _inputs(rows, C, K, t, seed, bias=True):
