@@ -205,8 +205,8 @@ ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, dou
   long long best = 1;
   auto consider = [&](const TileCost& c, double beside) {
     const double f = dtype == WC_F32 ? (c.tile.m == 64 ? 5 : 7) : 1, f_alone = dtype == WC_F32 ? 4 : 1;
-    const long long tiles = tiles_of(p, c.tile), slots = (long long)c.slots * kCus, most = c.tile.m == 256 ? 1 : std::min({steps, room, 4ll * kCus});
-    for (long long s = 1; s <= most; s += 1 + s / 8) {
+    const long long tiles = tiles_of(p, c.tile), slots = (long long)c.slots * kCus, most = c.tile.m == 256 || tiles >= slots ? 1 : std::min({steps, room, 4ll * kCus});
+    for (long long s = 1; s <= most; s += 1 + s / 4) {
       const long long each = ceil_div_ll(steps, s), n = tiles * ceil_div_ll(steps, each);
       const double end = heavy && s == 1 ? c.heavy : c.plain;
       const double rounds = n <= slots ? (double)n / slots : (double)ceil_div_ll(n, slots);

@@ -180,6 +180,33 @@ def test_strides_starts_and_axes(dev, t):
         lo.within(a, *full[k], k)
 
 
+def test_offsets_beyond_32_bits(dev):
+    """More than 2^31 elements of x, and of its codes: rows at the very end, forward, both gradients and 8 bits."""
+    t, C, K, rows = torch.float16, 64, 8, (1 << 25) + 1000
+    x = torch.zeros(rows, C, dtype=t, device=dev)
+    dy = torch.zeros(rows, K, dtype=t, device=dev)
+    tail = slice(rows - 700, rows)
+    xs, w, _, _, ds = _inputs(700, C, K, t, 3)
+    x[tail], dy[tail] = xs.cuda(), ds.cuda()
+    y, _, by, _ = lo.forward(xs, w, None, None, "relu", False)
+    got = matrix_linear.linear_forward(x, w.cuda(), activation="relu")
+    lo.within(got[tail], y, by, "y")
+    assert not bool(got[:4096].any())
+    del got
+    p = checkpoint8.pack8(x)
+    codes, exps = lo.pack(xs)
+    assert torch.equal(p.codes[tail].cpu(), codes) and torch.equal(p.exponents[tail].cpu(), exps)
+    back = checkpoint8.unpack8(p)
+    assert torch.equal(back[tail].cpu().double(), lo.unpack(codes, exps)) and not bool(back[:4096].any())
+    del p, back
+    dx, dw, db, _ = matrix_linear.linear_backward(dy, x, w.cuda())
+    want = lo.backward(ds, xs, w, xs, "none")
+    lo.within(dx[tail], *want["dx"], "dx")
+    # (zeros add no roundings but those of the sums of parts)
+    lo.within(dw, *want["dw"], "dw")
+    lo.within(db, *want["db"], "db")
+
+
 def test_no_rows(dev, host_layer):
     w = torch.randn(5, 4, device=dev)
     for lead in ((0,), (3, 0)):
