@@ -185,7 +185,7 @@ bool few_rows_pay(const LinearProduct& p, int dtype) {
 long long tiles_of(const LinearProduct& p, ProductTile t) { return ceil_div_ll(p.M, t.m) * ceil_div_ll(p.N, t.n); }
 
 // What 64 elements of the reduction take a workgroup, alone on its compute unit and with as many as it holds, and what the epilogue takes, plain and
-// heavy, in us; measured on 16-bit products of 4096 and 8192 squared (fp32 instructions: 128 x 128 seven times, 64 x 64 five times that, alone four times)
+// heavy, in us; measured on 16-bit products of 4096 and 8192 squared (fp32 instructions: 128 x 128 seven times, 64 x 64 five times that, alone three times)
 struct TileCost { ProductTile tile; int slots; double alone, full, plain, heavy; };
 constexpr TileCost kTileCosts[] = {{{64, 64}, 4, 0.55, 1.1, 1, 3}, {{128, 128}, 2, 0.6, 1.17, 2, 6}, {{256, 256}, 1, 1.85, 1.85, 5, 18}};
 constexpr TileCost kGeneralCost = {{64, 64}, 4, 2, 2, 2, 4};
@@ -204,13 +204,13 @@ ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, dou
   double least = -1;
   long long best = 1;
   auto consider = [&](const TileCost& c, double beside) {
-    const double f = dtype == WC_F32 ? (c.tile.m == 64 ? 5 : 7) : 1, f_alone = dtype == WC_F32 ? 4 : 1;
+    const double f = dtype == WC_F32 ? (c.tile.m == 64 ? 5 : 7) : 1, f_alone = dtype == WC_F32 ? 3 : 1;
     const long long tiles = tiles_of(p, c.tile), slots = (long long)c.slots * kCus, most = c.tile.m == 256 || tiles >= slots ? 1 : std::min({steps, room, 4ll * kCus});
     for (long long s = 1; s <= most; s += 1 + s / 4) {
       const long long each = ceil_div_ll(steps, s), n = tiles * ceil_div_ll(steps, each);
       const double end = heavy && s == 1 ? c.heavy : c.plain;
       const double rounds = n <= slots ? (double)n / slots : (double)ceil_div_ll(n, slots);
-      const double us = std::max({each * c.alone * f_alone + end, rounds * (each * c.full * f + end), rounds * (each * c.full * f + end) * 0.9 + beside}) + (s > 1 ? 8 + 2e-6 * s * p.M * p.N : 0);
+      const double us = std::max({each * c.alone * f_alone + end, rounds * (each * c.full * f + end), rounds * (each * c.full * f + end) * 0.9 + beside}) + (s > 1 ? 8 + 1e-6 * s * p.M * p.N : 0);
       if (least >= 0 && us >= least) continue;
       least = us;
       best = s;
