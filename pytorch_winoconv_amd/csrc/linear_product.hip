@@ -35,11 +35,14 @@ __device__ __forceinline__ void finish(const LinearEpilogue& e, long long m, lon
   else static_cast<T*>(e.y)[i] = static_cast<T>(v);
 }
 
+template <typename T> constexpr int kGeneralPitch = 80 / sizeof(T);      // of a row of 64 bytes in LDS
+template <typename T> struct GeneralLds { T tile[2][2][64 * kGeneralPitch<T>]; };
+
 template <typename T, bool AO, bool BO>
-__global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
-  constexpr int EPC = 16 / sizeof(T), BK = 4 * EPC, PITCH = BK + EPC, AHEAD = 4;
-  __shared__ __attribute__((aligned(16))) T tile[2][2][64 * PITCH];
-  const int blk = xcd_remap(blockIdx.x, g.per_xcd);
+__device__ __forceinline__ void general_block(const GeneralArgs& g, int hw_block, GeneralLds<T>& shared) {
+  constexpr int EPC = 16 / sizeof(T), BK = 4 * EPC, PITCH = kGeneralPitch<T>, AHEAD = 4;
+  static_assert(PITCH == BK + EPC, "rows of 64 bytes, 16 apart");
+  const int blk = xcd_remap(hw_block, g.per_xcd);
   if (blk >= g.n_blocks) return;
   const int tn = blk % g.tiles_n, tm = blk / g.tiles_n % g.tiles_m, s = blk / (g.tiles_n * g.tiles_m);
   const LinearProduct& p = g.p;
@@ -88,7 +91,7 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
         load(OA{}, p.a, p.lda, m0, p.M, ks + AHEAD - 1, va[(u + AHEAD - 1) % AHEAD]);
         load(OB{}, p.b, p.ldb, n0, p.N, ks + AHEAD - 1, vb[(u + AHEAD - 1) % AHEAD]);
       }
-      T(&lds)[2][64 * PITCH] = tile[u & 1];
+      T(&lds)[2][64 * PITCH] = shared.tile[u & 1];
       store(OA{}, lds[0], va[u]);
       store(OB{}, lds[1], vb[u]);
       __syncthreads();                             // and nobody multiplies from the other buffer any more
@@ -120,6 +123,21 @@ __global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
       if (g.parts) g.parts[(s * p.M + m) * p.N + n] = acc[4 * q + e];
       else finish<T>(p.e, m, n, p.N, acc[4 * q + e]);
     }
+}
+
+template <typename T, bool AO, bool BO>
+__global__ __launch_bounds__(256) void product_general_kernel(GeneralArgs g) {
+  __shared__ __attribute__((aligned(16))) GeneralLds<T> shared;
+  general_block<T, AO, BO>(g, blockIdx.x, shared);
+}
+
+// Both gradients of a layer in one launch
+template <typename T>
+__global__ __launch_bounds__(256) void product_general_pair_kernel(GeneralArgs g, GeneralArgs g2) {
+  __shared__ __attribute__((aligned(16))) GeneralLds<T> shared;
+  const int n = g.per_xcd * kXcds;
+  if ((int)blockIdx.x < n) general_block<T, false, true>(g, blockIdx.x, shared);
+  else general_block<T, true, true>(g2, blockIdx.x - n, shared);
 }
 
 // Few rows (at most 16 of M, 16-bit types, both operands with the reduction innermost): one pass over B, which bounds it.  A workgroup of 16 wavefronts takes NR
@@ -252,6 +270,17 @@ size_t product_parts_bytes(const LinearProduct& p, int dtype, const LinearProduc
   return s > 1 ? (size_t)s * p.M * p.N * 4 : 0;
 }
 
+static GeneralArgs general_args(const LinearProduct& p, const ProductPlan& plan, float* parts) {
+  GeneralArgs g;
+  g.p = p;
+  g.parts = plan.s > 1 ? parts : nullptr;
+  g.R_part = plan.R_part;
+  g.tiles_m = (int)ceil_div_ll(p.M, 64); g.tiles_n = (int)ceil_div_ll(p.N, 64);
+  g.n_blocks = (int)(tiles_of(p, plan.tile) * plan.s);
+  g.per_xcd = ceil_div(g.n_blocks, kXcds);
+  return g;
+}
+
 int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream) {
   const long long tiles = tiles_of(p, plan.tile);
   if (tiles * plan.s >= (1ll << 31) - 8) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
@@ -270,13 +299,7 @@ int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, i
     });
   }
   if (plan.dma) return product_dma(p, plan, parts, dtype, stream);
-  GeneralArgs g;
-  g.p = p;
-  g.parts = plan.s > 1 ? parts : nullptr;
-  g.R_part = plan.R_part;
-  g.tiles_m = (int)ceil_div_ll(p.M, 64); g.tiles_n = (int)ceil_div_ll(p.N, 64);
-  g.n_blocks = (int)(tiles * plan.s);
-  g.per_xcd = ceil_div(g.n_blocks, kXcds);
+  const GeneralArgs g = general_args(p, plan, parts);
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     auto fn = p.a_outer ? &product_general_kernel<T, true, true> : p.b_outer ? &product_general_kernel<T, false, true> : &product_general_kernel<T, false, false>;
@@ -289,6 +312,14 @@ int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, i
 int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream) {
   const bool few = tiles_of(p, plan.tile) * plan.s + tiles_of(p2, plan2.tile) * plan2.s < (1ll << 31) - 16;
   if (few && product_dma_pairs(plan, plan2)) return product_dma_pair(p, plan, parts, p2, plan2, parts2, dtype, stream);
+  if (few && !plan.dma && !plan2.dma) {
+    const GeneralArgs g = general_args(p, plan, parts), g2 = general_args(p2, plan2, parts2);
+    return dispatch_dtype(dtype, [&](auto t) -> int {
+      hipLaunchKernelGGL(product_general_pair_kernel<decltype(t)>, dim3((unsigned)((g.per_xcd + g2.per_xcd) * kXcds)), dim3(256), 0, as_stream(stream), g, g2);
+      WC_CHECK_LAUNCH("product_general_pair_kernel");
+      return WC_OK;
+    });
+  }
   if (int rc = product_run(p, plan, parts, dtype, stream)) return rc;
   return product_run(p2, plan2, parts2, dtype, stream);
 }
