@@ -139,6 +139,13 @@ struct DmaArgs {
   int vec;                    // rows of the parts' sums are multiples of 16 bytes
 };
 
+// What the lanes of a wavefront wrote to LDS is there for its other lanes, and what they read may be overwritten
+__device__ __forceinline__ void exchange_done() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A wavefront's WM x WN blocks through 32 rows of LDS of its own, a lane finishing eight neighbouring results of some rows, which start anywhere.
 // ALL: the tile is whole, no lane asks whether its results are there - a branch at every access leaves none to overlap.  MORE: there may be a
 // residual or z.
@@ -168,6 +175,7 @@ __device__ __forceinline__ void finish_blocks(const LinearEpilogue& e, const f32
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(stage + l32 * PITCH + j * 32 + 8 * q + 4 * lhi) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    exchange_done();
 #pragma unroll
     for (int r0 = 0; r0 < RUNS; r0 += AT_ONCE) {
       T res[AT_ONCE][8];
@@ -226,6 +234,7 @@ __device__ __forceinline__ void finish_blocks(const LinearEpilogue& e, const f32
         store(e.y);
       }
     }
+    if (i + 1 < WM) exchange_done();
   }
 }
 
