@@ -65,6 +65,19 @@ __device__ __forceinline__ float through(float dy, float z, int act) {
   }
 }
 
+// ---- launches -----------------------------------------------------------------------------------
+// A launch has fewer than 2^32 threads along an axis.  Workgroups, of at most 512 threads, that one takes; work of more goes in several
+constexpr long long kMostBlocks = (1ll << 23) - kXcds;
+// launch(first, n) over workgroups first .. first + n - 1 of `blocks`
+template <typename F>
+int in_launches(long long blocks, F&& launch) {
+  for (long long first = 0; first < blocks; first += kMostBlocks) {
+    const long long left = blocks - first;
+    if (int rc = launch(first, (unsigned)(left < kMostBlocks ? left : kMostBlocks))) return rc;
+  }
+  return WC_OK;
+}
+
 // ---- products -----------------------------------------------------------------------------------
 // What becomes of a sum v of a product: v + bias[n] (+ r) is rounded to z where that is asked for, act(it) (+ r) to y.
 struct LinearEpilogue {

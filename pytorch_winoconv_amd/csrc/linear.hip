@@ -13,7 +13,7 @@ size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 bool known(int dtype) { return dtype == WC_F32 || dtype == WC_F16 || dtype == WC_BF16; }
 int size_of(int dtype) { return dtype == WC_F32 ? 4 : 2; }
 
-// extents whose products stay far inside 63 bits and whose launches inside 31
+// extents whose products stay far inside 63 bits
 int check_extents(long long rows, int C, int K, int dtype, const char* who) {
   WC_CHECK_ARG(rows >= 0 && C > 0 && K > 0 && known(dtype), "%s: rows %lld, C %d, K %d, dtype %d", who, rows, C, K, dtype);
   if (rows > (1ll << 31) - 1 || C > (1 << 24) || K > (1 << 24))

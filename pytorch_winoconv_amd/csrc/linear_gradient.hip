@@ -120,6 +120,7 @@ __device__ __forceinline__ void slope_block(const SlopeArgs& a, int block, int t
 }
 
 struct PrepareArgs {
+  long long first;                     // workgroup of this launch
   SlopeArgs slope;
   int slope_blocks, slope_tiles;       // none: 0
   WideCopy copies[2];
@@ -131,7 +132,7 @@ struct PrepareArgs {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void prepare_kernel(PrepareArgs a) {
   __shared__ float sums[kThreads * (VEC + 1)];
-  long long b = blockIdx.x;
+  long long b = a.first + blockIdx.x;
   const long long n = (long long)a.slope_blocks * a.slope_tiles;
   if (b < n) return slope_block<T>(a.slope, (int)(b / a.slope_tiles), (int)(b % a.slope_tiles), sums);
   b -= n;
@@ -254,16 +255,17 @@ int linear_prepare(const LinearPrepare& p, int dtype, float* sums, void* stream)
   long long n = (long long)a.slope_blocks * a.slope_tiles + a.copy_blocks[0] + a.copy_blocks[1];
   if (p.codes) {
     const int rg = (int)pack_groups(p.x_C);
-    a.unpack = {p.codes, p.exps, p.x, p.x_rows * rg, p.x_ld, p.x_C, rg};
+    a.unpack = {0, p.codes, p.exps, p.x, p.x_rows * rg, p.x_ld, p.x_C, rg};
     a.line = p.x_ld == p.x_C && on_a_line(p.x_C, p.x, p.codes);
     n += unpack_blocks(a.unpack, a.line != 0);
   }
-  if (n == 0) return WC_OK;
-  if (n >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "%lld rows of %d and %d elements are too many", p.slope.rows, p.slope.K, p.x_C);
-  return dispatch_dtype(dtype, [&](auto t) -> int {
-    hipLaunchKernelGGL(prepare_kernel<decltype(t)>, dim3((unsigned)n), dim3(kThreads), 0, as_stream(stream), a);
-    WC_CHECK_LAUNCH("prepare_kernel");
-    return WC_OK;
+  return dispatch_dtype(dtype, [&](auto t) {
+    return in_launches(n, [&](long long first, unsigned blocks) -> int {
+      a.first = first;
+      hipLaunchKernelGGL(prepare_kernel<decltype(t)>, dim3(blocks), dim3(kThreads), 0, as_stream(stream), a);
+      WC_CHECK_LAUNCH("prepare_kernel");
+      return WC_OK;
+    });
   });
 }
 
@@ -281,8 +283,7 @@ int linear_join(const LinearJoin* joins, int n, const LinearSlope* slope, const 
     a.sum_rows = slope_plan(slope->rows, slope->K).blocks;
     blocks += ceil_div(slope->K, 16);
   }
-  if (blocks == 0) return WC_OK;
-  if (blocks >= (1ll << 31)) return fail(WC_ERR_UNSUPPORTED, "%lld x %lld results are too many", joins[0].M, joins[0].N);
+  if (blocks == 0) return WC_OK;      // (parts are of few results, and the columns no more than 2^24: one launch holds them)
   return dispatch_dtype(dtype, [&](auto t) -> int {
     hipLaunchKernelGGL(join_kernel<decltype(t)>, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), a);
     WC_CHECK_LAUNCH("join_kernel");

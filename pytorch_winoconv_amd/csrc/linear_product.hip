@@ -281,9 +281,26 @@ static GeneralArgs general_args(const LinearProduct& p, const ProductPlan& plan,
   return g;
 }
 
+// Rows m0 .. m0 + M - 1 of a product's results
+static LinearProduct rows_of(const LinearProduct& p, long long m0, long long M, int dtype) {
+  const long long es = dtype == WC_F32 ? 4 : 2;
+  LinearProduct q = p;
+  q.M = M;
+  q.a = static_cast<const char*>(p.a) + (p.a_outer ? m0 : m0 * p.lda) * es;
+  if (p.e.res) q.e.res = static_cast<const char*>(p.e.res) + m0 * p.N * es;
+  if (p.e.z) q.e.z = static_cast<char*>(p.e.z) + m0 * p.N * es;
+  q.e.y = static_cast<char*>(p.e.y) + m0 * p.N * (p.e.y_f32 ? 4 : es);
+  return q;
+}
+
 int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, int dtype, void* stream) {
-  const long long tiles = tiles_of(p, plan.tile);
-  if (tiles * plan.s >= (1ll << 31) - 8) return fail(WC_ERR_UNSUPPORTED, "a product of %lld x %lld has too many tiles", p.M, p.N);
+  // (few results are left to parts: those have few tiles)
+  const long long most = kMostBlocks / ceil_div_ll(p.N, plan.tile.n) * plan.tile.m;
+  if (p.M > most && plan.s == 1) {
+    for (long long m0 = 0; m0 < p.M; m0 += most)
+      if (int rc = product_run(rows_of(p, m0, std::min(most, p.M - m0), dtype), plan, nullptr, dtype, stream)) return rc;
+    return WC_OK;
+  }
   if (plan.few) {
     return dispatch_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
@@ -310,7 +327,7 @@ int product_run(const LinearProduct& p, const ProductPlan& plan, float* parts, i
 }
 
 int product_run_pair(const LinearProduct& p, const ProductPlan& plan, float* parts, const LinearProduct& p2, const ProductPlan& plan2, float* parts2, int dtype, void* stream) {
-  const bool few = tiles_of(p, plan.tile) * plan.s + tiles_of(p2, plan2.tile) * plan2.s < (1ll << 31) - 16;
+  const bool few = tiles_of(p, plan.tile) * plan.s + tiles_of(p2, plan2.tile) * plan2.s <= kMostBlocks - kXcds;
   if (few && product_dma_pairs(plan, plan2)) return product_dma_pair(p, plan, parts, p2, plan2, parts2, dtype, stream);
   if (few && !plan.dma && !plan2.dma) {
     const GeneralArgs g = general_args(p, plan, parts), g2 = general_args(p2, plan2, parts2);

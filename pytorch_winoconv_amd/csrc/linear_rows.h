@@ -42,6 +42,7 @@ __device__ __forceinline__ void store_run(void* to, long long i, int have, const
 
 // Workgroup `block` of 256 threads: rows of 8 bits back to T in rows of ld, zeros behind C; eight threads a group, four elements each
 struct UnpackArgs {
+  long long first;           // workgroup of the launch, where it does nothing else
   const signed char* codes; const signed char* exps;
   void* out;
   long long groups, ld;      // groups of all rows

@@ -20,6 +20,7 @@ namespace wc {
 namespace {
 
 struct PackArgs {
+  long long first;           // workgroup of the launch
   const void* x;
   signed char* codes; signed char* exps;
   long long groups;          // of all rows
@@ -51,7 +52,7 @@ __device__ __forceinline__ int group_exponent(const T (&x)[N]) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void pack8_line_kernel(PackArgs a) {
-  const long long total = a.groups * kPackGroup, first = (long long)blockIdx.x * kLine + threadIdx.x * 8;
+  const long long total = a.groups * kPackGroup, first = (a.first + blockIdx.x) * kLine + threadIdx.x * 8;
   T x[4][8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) load_run<T, 8>(a.x, first + j * 2048, first + j * 2048 < total ? 8 : 0, x[j]);
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(256) void pack8_line_kernel(PackArgs a) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void pack8_kernel(PackArgs a) {
-  const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
+  const long long g = ((a.first + blockIdx.x) * 256 + threadIdx.x) >> 3;
   const int part = threadIdx.x & 7;
   const long long row = g / a.row_groups;
   const int c0 = (int)(g - row * a.row_groups) * kPackGroup + part * 4;
@@ -87,34 +88,39 @@ __global__ __launch_bounds__(256) void pack8_kernel(PackArgs a) {
 
 template <typename T, bool LINE>
 __global__ __launch_bounds__(256) void unpack8_kernel(UnpackArgs a) {
-  if constexpr (LINE) unpack_line_block<T>(a, blockIdx.x);
-  else unpack_block<T>(a, blockIdx.x);
+  if constexpr (LINE) unpack_line_block<T>(a, a.first + blockIdx.x);
+  else unpack_block<T>(a, a.first + blockIdx.x);
 }
 
 }  // namespace
 
 int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, bool keep_sign, int dtype, void* stream) {
   const int rg = (int)pack_groups(C);
-  const PackArgs a = {x, codes, exps, rows * rg, C, rg, keep_sign};
+  PackArgs a = {0, x, codes, exps, rows * rg, C, rg, keep_sign};
   const bool line = on_a_line(C, x, codes);
-  return dispatch_dtype(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((line ? &pack8_line_kernel<T> : &pack8_kernel<T>), dim3((unsigned)(line ? ceil_div_ll(a.groups * kPackGroup, kLine) : ceil_div_ll(a.groups, 32))), dim3(256), 0,
-                       as_stream(stream), a);
-    WC_CHECK_LAUNCH("pack8_kernel");
-    return WC_OK;
+    return in_launches(line ? ceil_div_ll(a.groups * kPackGroup, kLine) : ceil_div_ll(a.groups, 32), [&](long long first, unsigned blocks) -> int {
+      a.first = first;
+      hipLaunchKernelGGL((line ? &pack8_line_kernel<T> : &pack8_kernel<T>), dim3(blocks), dim3(256), 0, as_stream(stream), a);
+      WC_CHECK_LAUNCH("pack8_kernel");
+      return WC_OK;
+    });
   });
 }
 
 int unpack8(const signed char* codes, const signed char* exps, void* x, long long rows, int C, int dtype, void* stream) {
   const int rg = (int)pack_groups(C);
-  const UnpackArgs a = {codes, exps, x, rows * rg, C, C, rg};
+  UnpackArgs a = {0, codes, exps, x, rows * rg, C, C, rg};
   const bool line = on_a_line(C, x, codes);
-  return dispatch_dtype(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((line ? &unpack8_kernel<T, true> : &unpack8_kernel<T, false>), dim3((unsigned)unpack_blocks(a, line)), dim3(256), 0, as_stream(stream), a);
-    WC_CHECK_LAUNCH("unpack8_kernel");
-    return WC_OK;
+    return in_launches(unpack_blocks(a, line), [&](long long first, unsigned blocks) -> int {
+      a.first = first;
+      hipLaunchKernelGGL((line ? &unpack8_kernel<T, true> : &unpack8_kernel<T, false>), dim3(blocks), dim3(256), 0, as_stream(stream), a);
+      WC_CHECK_LAUNCH("unpack8_kernel");
+      return WC_OK;
+    });
   });
 }
 
