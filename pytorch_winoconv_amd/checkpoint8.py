@@ -15,6 +15,12 @@ from ._lib import check
 GROUP = 32
 
 
+def check_channels(n, who):
+    """The C ABI takes channels as an int, which ctypes would cut to 32 bits."""
+    if n > 1 << 24:
+        raise ValueError("%s: %d channels, at most 2^24" % (who, n))
+
+
 class Packed8:
     """A tensor in 8 bits: `codes` int8 of its shape, `exponents` int8 of its shape with ceil(C / 32) groups in the place of
     its C channels, both contiguous, and the type that it reads as."""
@@ -56,9 +62,10 @@ def pack8(x, keep_sign=False):
         parts = engine._ext.pack8(x, bool(keep_sign))
         if parts is not None:
             return _made(*parts, x.dtype)
-    engine._require_gpu(x)
     if x.dim() < 1:
         raise ValueError("pack8: a tensor of at least one axis, its channels last")
+    check_channels(x.shape[-1], "pack8")
+    engine._require_gpu(x)
     x = x.detach().contiguous()
     C = x.shape[-1]
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
@@ -72,6 +79,7 @@ def pack8(x, keep_sign=False):
 
 def unpack8(packed):
     """The tensor that a Packed8 stands for, contiguous, in its type."""
+    check_channels(packed.shape[-1], "unpack8")
     if not packed.codes.is_cuda:
         raise ValueError("winoconv runs on the GPU only: got a %s tensor" % packed.device)
     if engine.USE_EXT:

@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
-from .checkpoint8 import Packed8, pack8
+from .checkpoint8 import Packed8, check_channels, pack8
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -71,6 +71,7 @@ def linear_forward(x, w, bias=None, residual=None, activation="none", residual_a
             return y
     _check_weight(x.shape, w, "x")
     K, C = w.shape
+    check_channels(max(K, C), "linear_forward")
     shape = tuple(x.shape[:-1]) + (K,)
     _check_like(w, (K, C), x.dtype, x.device, "the weight")
     _check_like(bias, (K,), x.dtype, x.device, "the bias")
@@ -101,6 +102,7 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     if (need_dx and w is None) or (need_dw and x is None):
         raise ValueError("linear_backward: dx needs w, dw needs x")
     C = w.shape[-1] if w is not None else x.shape[-1] if x is not None else 1
+    check_channels(max(K, C), "linear_backward")
     if w is not None:
         _check_weight((C,), w, "x")
         _check_like(w, (K, C), dtype, device, "the weight")
