@@ -395,7 +395,8 @@ int wc_linear_backward(const wc_linear_desc* desc, const wc_linear_gradients* gr
  * (rows, ceil(C / 32)): the groups of 32 neighbouring channels of a row share a step 2^e, e = floor(log2(largest magnitude)) - 6 but at least -126;
  * a value is the whole number nearest to its share of the step, ties to even, at most 127 either way.  It reads as code times 2^e, exact in x's
  * type.  A group with an infinity or a NaN has the exponent 127 and reads as NaN.  keep_sign: values other than zero have a code other
- * than zero (a step), for what is read by its sign alone. */
+ * than zero (a step), for what is read by its sign alone.  keep_sign 2, for z of relu in wc_linear_backward: also in a group with an infinity or a NaN,
+ * whose codes are 1 for what is above zero, -1 for what is not and 0 for NaN; as a tensor such a group still reads as NaN. */
 int wc_pack8(const void* x, signed char* codes, signed char* exponents, long long rows, int C, int dtype, int keep_sign, void* stream);
 int wc_unpack8(const signed char* codes, const signed char* exponents, void* x, long long rows, int C, int dtype, void* stream);
 #ifdef __cplusplus

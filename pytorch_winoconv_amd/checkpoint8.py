@@ -58,8 +58,18 @@ def _made(codes, exponents, dtype):
 def pack8(x, keep_sign=False):
     """x (..., C) in 8 bits.  `keep_sign`: values other than zero keep a code other than zero (one step), for tensors that are read by
     their sign alone, as a ReLU's gradient reads them."""
+    return _pack(x, int(bool(keep_sign)))
+
+
+def pack_gates(z):
+    """z in 8 bits for the gradient of a ReLU and nothing else: pack8 with `keep_sign`, and in groups with an infinity or a NaN the other channels
+    keep their gates too."""
+    return _pack(z, 2)
+
+
+def _pack(x, keep_sign):
     if engine.USE_EXT:
-        parts = engine._ext.pack8(x, bool(keep_sign))
+        parts = engine._ext.pack8(x, keep_sign)
         if parts is not None:
             return _made(*parts, x.dtype)
     if x.dim() < 1:
@@ -73,7 +83,7 @@ def pack8(x, keep_sign=False):
     if x.numel():
         with engine._on_device(x):
             check(_lib.load().wc_pack8(engine._ptr(x), engine._ptr(codes), engine._ptr(exponents), x.numel() // C, C, engine._DTYPES[x.dtype],
-                                       int(bool(keep_sign)), engine._stream(x)))
+                                       keep_sign, engine._stream(x)))
     return Packed8(codes, exponents, x.dtype)
 
 

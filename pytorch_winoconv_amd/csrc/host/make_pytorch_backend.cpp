@@ -736,7 +736,7 @@ py::tuple linear_backward(const at::Tensor& dy_, const MaybeTensor& x, const May
   return py::make_tuple(or_none(dx), or_none(dw), or_none(db), or_none(dz));
 }
 
-py::object pack8(const at::Tensor& x_, bool keep_sign) {
+py::object pack8(const at::Tensor& x_, int keep_sign) {
   const int64_t nd = x_.dim();
   if (!linear_type(x_) || nd < 1 || x_.numel() == 0 || !fits(x_.size(nd - 1))) return py::none();
   const c10::DeviceGuard guard(x_.device());

@@ -147,7 +147,10 @@ constexpr int kPackNoNumber = 127, kPackLeast = -126;
 __device__ __forceinline__ float pack_step(int e) {
   return e == kPackNoNumber ? __builtin_nanf("") : __uint_as_float((unsigned)(e + 127) << 23);
 }
-int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, bool keep_sign, int dtype, void* stream);
+constexpr int kPackSigns = 1, kPackGates = 2;                // of keep_sign
+// what relu's gate is read from: codes of a group with an infinity or a NaN as pack8.hip leaves them for it, where 0 (times an infinity) is no number
+__device__ __forceinline__ float gate_step(int e) { return e == kPackNoNumber ? __builtin_inff() : pack_step(e); }
+int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, int keep_sign, int dtype, void* stream);
 int unpack8(const signed char* codes, const signed char* exps, void* x, long long rows, int C, int dtype, void* stream);
 inline long long wide_row(long long C, int dtype) { const int epc = dtype == WC_F32 ? 4 : 8; return (C + epc - 1) / epc * epc; }
 

@@ -207,7 +207,7 @@ int wc_pack8(const void* x, signed char* codes, signed char* exponents, long lon
   if (rows == 0) return WC_OK;
   WC_CHECK_ARG(x && codes && exponents, "wc_pack8: null pointer");
   if (rows * pack_groups(C) >= (1ll << 36)) return fail(WC_ERR_UNSUPPORTED, "wc_pack8: rows %lld, C %d", rows, C);
-  return pack8(x, codes, exponents, rows, C, keep_sign != 0, dtype, stream);
+  return pack8(x, codes, exponents, rows, C, keep_sign == kPackGates ? kPackGates : keep_sign ? kPackSigns : 0, dtype, stream);
 }
 
 int wc_unpack8(const signed char* codes, const signed char* exponents, void* x, long long rows, int C, int dtype, void* stream) {

@@ -59,7 +59,7 @@ __device__ __forceinline__ void slope_rows(const SlopeArgs& a, int k, long long 
       const long long r = r0 + j * a.groups;
       T dz[VEC];
       float step = 0.f;
-      if constexpr (ACT != WC_ACT_NONE && PACKED) step = pack_step(e8[j]);
+      if constexpr (ACT != WC_ACT_NONE && PACKED) step = ACT == WC_ACT_RELU ? gate_step(e8[j]) : pack_step(e8[j]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         float z = 0.f;

@@ -7,7 +7,9 @@
 // largest, but for those above 127.5 steps, which are off by less than one, 2^-7 of themselves.  Against a floating type of 8 bits with three
 // bits of mantissa (off by 2^-4 of the value) the large values of a group, which are most of the sums they enter, are eight times as exact.
 // A group with an infinity or a NaN has the exponent 127 and reads as NaN throughout, so that such values still show in the gradients.
-// keep_sign: values other than zero keep a code other than zero, one step - for what is read by its sign alone (the gate of a ReLU).
+// keep_sign: values other than zero keep a code other than zero, one step - for what is read by its sign alone.
+// kPackGates, for the gate of a ReLU: the codes of a group with an infinity or a NaN are 1 above zero, -1 for the rest and 0 for a NaN, so that its
+// other channels keep their gates.
 //
 // Bound by memory.  Rows of whole groups are one line of groups: a thread takes eight neighbouring elements four times, 16 bytes a load, and
 // four threads a group.  Other rows take eight threads a group, four elements each, wherever they start.
@@ -32,9 +34,9 @@ __device__ __forceinline__ int pack_exponent(float top) {
   const int bits = (int)(__float_as_uint(top) >> 23);          // top >= 0
   return bits == 255 ? kPackNoNumber : max(bits - 127 - 6, kPackLeast);
 }
-// 2^-e is a normal number for every e there is but NoNumber, whose codes are not read
-__device__ __forceinline__ int pack_code(float v, int e, bool keep_sign) {
-  if (e == kPackNoNumber) return 0;
+// 2^-e is a normal number for every e there is but NoNumber, whose codes are read as gates alone
+__device__ __forceinline__ int pack_code(float v, int e, int keep_sign) {
+  if (e == kPackNoNumber) return keep_sign == kPackGates ? (v > 0.f ? 1 : v <= 0.f ? -1 : 0) : 0;
   const float q = fminf(fmaxf(rintf(v * __uint_as_float((unsigned)(127 - e) << 23)), -127.f), 127.f);
   return keep_sign && q == 0.f && v != 0.f ? (v > 0.f ? 1 : -1) : (int)q;
 }
@@ -94,7 +96,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(UnpackArgs a) {
 
 }  // namespace
 
-int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, bool keep_sign, int dtype, void* stream) {
+int pack8(const void* x, signed char* codes, signed char* exps, long long rows, int C, int keep_sign, int dtype, void* stream) {
   const int rg = (int)pack_groups(C);
   PackArgs a = {0, x, codes, exps, rows * rg, C, rg, keep_sign};
   const bool line = on_a_line(C, x, codes);

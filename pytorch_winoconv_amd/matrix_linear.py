@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
-from .checkpoint8 import Packed8, check_channels, pack8
+from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -182,7 +182,7 @@ class LinearFunction(torch.autograd.Function):
         ctx.x_shape = x.shape
         kept = [None if not need_w else x, None if not need_x else w, z]
         if checkpoint is not None:
-            packed = [None if t is None else pack8(t, s) for t, s in ((kept[0], False), (z, by_sign))]
+            packed = [None if t is None else pack(t) for t, pack in ((kept[0], pack8), (z, pack_gates if by_sign else pack8))]
             kept = [packed[0] and packed[0].codes, kept[1], packed[1] and packed[1].codes, packed[0] and packed[0].exponents, packed[1] and packed[1].exponents]
         ctx.save_for_backward(*kept)
         return y
