@@ -11,6 +11,7 @@ import ctypes
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, engine
@@ -204,7 +205,7 @@ class LinearFunction(torch.autograd.Function):
 def linear(x, w, bias=None, residual=None, activation="none", residual_after=False, checkpoint=None, channel_axis=-1):
     """linear_forward with gradients.  checkpoint="int8" keeps x and z in 8 bits for the backward pass (checkpoint8); relu's gradient
     stays exact.  channel_axis: the axis of the channels in x and the residual, so that 1 takes the (N, C, H, W) tensors of the convolutions; a
-    tensor in channel-last memory is used as it is, and the result is one."""
+    tensor in channel-last memory is used as it is, and the result is one.  Reverse mode, once: operands with a forward-mode tangent are refused."""
     _check_checkpoint(checkpoint)
     act = _activation(activation)
     if channel_axis not in (-1, x.dim() - 1):
@@ -212,6 +213,9 @@ def linear(x, w, bias=None, residual=None, activation="none", residual_after=Fal
         residual = None if residual is None else residual.movedim(channel_axis, -1)
         return linear(x, w, bias, residual, activation, residual_after, checkpoint).movedim(-1, channel_axis)
     given = [t for t in (x, w, bias, residual) if t is not None]
+    # (asked of torch for each tensor only within a level of forward mode: 3 us)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise NotImplementedError("linear has no forward-mode derivative: a tangent of its operands would be lost")
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return LinearFunction.apply(x, w, bias, residual, activation, bool(residual_after), checkpoint)
     own = lambda t: t if t is None or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731

@@ -1,7 +1,9 @@
 """Arguments of linear layers and 8 bits that the C ABI could not tell apart from others, refused on the CPU before any launch."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+import pytorch_winoconv_amd as pkg
 from pytorch_winoconv_amd import checkpoint8, matrix_linear
 
 
@@ -22,3 +24,25 @@ def test_channels_beyond_an_int(host_layer):
         matrix_linear.linear_backward(wide, None, None, need_dx=False, need_dw=False)
     with pytest.raises(ValueError, match="linear_backward: 4294967328 channels"):
         matrix_linear.linear_backward(wide[:, :1], wide, None, need_dx=False)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_is_refused(which):
+    """A tangent would be dropped without a word, gradients asked for or not."""
+    ts = [torch.randn(s) for s in ((3, 4), (5, 4), (5,), (3, 5))]
+    with forward_ad.dual_level():
+        ts[which] = forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+        for t in (ts[0], ts[0].detach().requires_grad_() if which else ts[0]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                matrix_linear.linear(t, *ts[1:])
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            matrix_linear.linear(*ts)
+        if which == 0:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                pkg.MatrixLinear(4, 5, channel_axis=1)(ts[0].view(1, 3, 4).movedim(2, 1))
+    # outside of a level, and within one without tangents, it goes on to the checks of the layer
+    ts = [torch.randn(s) for s in ((3, 4), (5, 4), (5,), (3, 5))]
+    with pytest.raises(ValueError, match="GPU only"):
+        matrix_linear.linear(*ts)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="GPU only"):
+        matrix_linear.linear(*ts)
