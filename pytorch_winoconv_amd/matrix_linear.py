@@ -102,6 +102,9 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     K, lead = dy.shape[-1], tuple(dy.shape[:-1])
     if (need_dx and w is None) or (need_dw and x is None):
         raise ValueError("linear_backward: dx needs w, dw needs x")
+    for t, what in ((w, "w"), (x, "x")):
+        if t is not None and len(t.shape) < 1:
+            raise ValueError("%s of shape (): expected %s" % (what, "(K, C)" if what == "w" else "(..., C)"))
     C = w.shape[-1] if w is not None else x.shape[-1] if x is not None else 1
     check_channels(max(K, C), "linear_backward")
     if w is not None:
@@ -209,6 +212,8 @@ def linear(x, w, bias=None, residual=None, activation="none", residual_after=Fal
     _check_checkpoint(checkpoint)
     act = _activation(activation)
     if channel_axis not in (-1, x.dim() - 1):
+        if residual is not None and residual.dim() != x.dim():
+            raise ValueError("the residual has shape %r, expected that of the result: %d axes" % (tuple(residual.shape), x.dim()))
         x = x.movedim(channel_axis, -1)
         residual = None if residual is None else residual.movedim(channel_axis, -1)
         return linear(x, w, bias, residual, activation, residual_after, checkpoint).movedim(-1, channel_axis)

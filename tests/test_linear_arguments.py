@@ -46,3 +46,13 @@ def test_forward_mode_is_refused(which):
         matrix_linear.linear(*ts)
     with forward_ad.dual_level(), pytest.raises(ValueError, match="GPU only"):
         matrix_linear.linear(*ts)
+
+
+def test_operands_without_axes_are_named():
+    dy, x, w, point = torch.randn(3, 5), torch.randn(3, 4), torch.randn(5, 4), torch.tensor(1.0)
+    with pytest.raises(ValueError, match="w of shape"):
+        matrix_linear.linear_backward(dy, x, point)
+    with pytest.raises(ValueError, match="x of shape"):
+        matrix_linear.linear_backward(dy, point, None, need_dx=False)
+    with pytest.raises(ValueError, match="the residual has shape"):
+        matrix_linear.linear(torch.randn(2, 4, 3, 3), w, None, torch.randn(5), channel_axis=1)
