@@ -183,7 +183,6 @@ class LinearFunction(torch.autograd.Function):
             y = linear_forward(x, w, bias, residual, activation, residual_after)
             if slope:
                 z = y
-        ctx.x_shape = x.shape
         kept = [None if not need_w else x, None if not need_x else w, z]
         if checkpoint is not None:
             packed = [None if t is None else pack(t) for t, pack in ((kept[0], pack8), (z, pack_gates if by_sign else pack8))]
