@@ -376,7 +376,7 @@ int wc_linear_forward(const wc_linear_desc* desc, const void* x, const void* w, 
 /* The gradients of that layer: dz = dy act'(z), dx = dz w, dw = dzT x, db = the column sums of dz (before dz's rounding).  Those that are null
  * are not computed; dz is also the gradient of a residual before the activation (of one behind it: dy).  dw and db in the operands' type
  * or unrounded in fp32.  x and z of the operands' type, or, where their exponents are given, in 8 bits (wc_pack8); for relu anything with
- * the sign of z does, y among it where no residual was added behind it.  relu's gradient is 0 at z = 0.  w and z may be null where nothing asks for them.  Sums in
+ * the sign of z does, y among it where no residual was added behind it.  relu's gradient is 0 at z = 0 and NaN where z is.  w and z may be null where nothing asks for them.  Sums in
  * fp32 and a fixed order; dz is rounded to the operands' type, which the matrix cores take, before the products.  rows > 0. */
 typedef struct {
   const void* dy;

@@ -2,7 +2,7 @@
 
 The groups of 32 neighbouring channels (the last axis) share a step 2^e, e = floor(log2(largest magnitude)) - 6 but at least -126;
 a value is kept as the nearest whole number of steps, ties to even, at most 127 either way, and reads as that number times the step, which
-every type it came from holds exactly.  It is off by at most 2^-7 of its group's largest.  Groups with an infinity or a NaN read as NaN.
+every type it came from holds exactly.  It is off by at most 2^-7 of its group's largest, or 2^-127 where that is more.  Groups with an infinity or a NaN read as NaN.
 Memory: 1 + 1/32 bytes a value.  WinoConv2d / WinoConv3d and MatrixLinear keep their inputs so with checkpoint="int8".
 """
 import ctypes

@@ -220,7 +220,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(JoinArgs a) {
 }
 
 struct SlopePlan { int cols, col_tiles, groups, blocks; long long rows_per_block; };
-// As many columns side by side as leave four workgroups to a compute unit
+// As many columns side by side as leave four workgroups to a compute unit; two of them run at a time, since the bodies of all activations in one kernel
+// take 231 registers
 SlopePlan slope_plan(long long rows, int K) {
   SlopePlan p;
   for (p.cols = kThreads;; p.cols /= 2) {

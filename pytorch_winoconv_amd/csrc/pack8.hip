@@ -4,7 +4,8 @@
 // The steps are powers of two, so v 2^-e is exact, q does not hang on how a division rounds, and q 2^e is exact in every type a group came
 // from: it has seven bits, lies between the type's smallest number and its largest (127 2^(e) is below 2^(e + 7), where the group's largest
 // value has its exponent), which steps rounded up to hold 128 2^e would exceed.  A value is off by at most half a step, 2^-7 of the group's
-// largest, but for those above 127.5 steps, which are off by less than one, 2^-7 of themselves.  Against a floating type of 8 bits with three
+// largest, but for those above 127.5 steps, which are off by less than one, 2^-7 of themselves; half a step is no less than 2^-127, so that groups
+// whose largest is below 2^-120 (fp32 and bf16) lose more of it and those of up to 2^-127 read as 0.  Against a floating type of 8 bits with three
 // bits of mantissa (off by 2^-4 of the value) the large values of a group, which are most of the sums they enter, are eight times as exact.
 // A group with an infinity or a NaN has the exponent 127 and reads as NaN throughout, so that such values still show in the gradients.
 // keep_sign: values other than zero keep a code other than zero, one step - for what is read by its sign alone.

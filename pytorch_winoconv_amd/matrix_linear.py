@@ -4,7 +4,9 @@ with bias, activation and residual in the epilogue of the product, and their gra
     z = x wT + bias (+ residual),   y = act(z) (+ residual)
 
 act is one of "none", "relu", "gelu", "gelu_tanh" and "silu"; the residual stands before the activation, or behind it with
-residual_after=True.  Sums and activations are fp32, y is rounded once.  float32, float16 and bfloat16; tensors that are not contiguous
+residual_after=True.  Sums and activations are fp32, y is rounded once.  In the gradients of an activation dz = dy act'(z) is rounded to
+the type of the tensors before both products, which the matrix cores take: with 16-bit types and gelu or silu their error in the 2-norm is 1.4 times that
+of an unrounded dz (bf16 0.0023 of 0.0017).  float32, float16 and bfloat16; tensors that are not contiguous
 are copied first.  The GPU only.
 """
 import ctypes
@@ -93,7 +95,8 @@ def linear_forward(x, w, bias=None, residual=None, activation="none", residual_a
 def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=True, need_db=True, need_dz=False, w_type=None, b_type=None):
     """(dx, dw, db, dz) of linear_forward, None for those not asked for, from dy (..., K), x (..., C), w (K, C) and, with an
     activation, z; x and z may be Packed8.  For relu anything with z's sign does, y among it where no residual stands behind the activation.
-    dw and db come in `w_type` and `b_type` (x's type; float32 sums unrounded).  dz is the gradient of z and so of a residual before
+    dw and db come in `w_type` and `b_type` (x's type; float32 sums unrounded, of products with the rounded dz; db's are of dz before
+    that).  relu's gradient is 0 at z = 0 and NaN where z is.  dz is the gradient of z and so of a residual before
     the activation; without an activation that is dy itself.  x may be None without need_dw, w without need_dx."""
     act = _activation(activation)
     dtype, device = dy.dtype, dy.device
@@ -205,8 +208,8 @@ class LinearFunction(torch.autograd.Function):
 
 
 def linear(x, w, bias=None, residual=None, activation="none", residual_after=False, checkpoint=None, channel_axis=-1):
-    """linear_forward with gradients.  checkpoint="int8" keeps x and z in 8 bits for the backward pass (checkpoint8); relu's gradient
-    stays exact.  channel_axis: the axis of the channels in x and the residual, so that 1 takes the (N, C, H, W) tensors of the convolutions; a
+    """linear_forward with gradients.  checkpoint="int8" keeps x and z in 8 bits for the backward pass (checkpoint8); relu's gate
+    stays z's own, so that of its gradients the weight's alone differs.  channel_axis: the axis of the channels in x and the residual, so that 1 takes the (N, C, H, W) tensors of the convolutions; a
     tensor in channel-last memory is used as it is, and the result is one.  Reverse mode, once: operands with a forward-mode tangent are refused."""
     _check_checkpoint(checkpoint)
     act = _activation(activation)
