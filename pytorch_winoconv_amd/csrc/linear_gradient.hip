@@ -3,8 +3,9 @@
 // Before them, dz = dy act'(z) in the storage type - the operand of both products, and the gradient of the layer's residual - and the column sums
 // of dz before that rounding (the bias gradient), in one read of dy and z, which bounds it: a workgroup takes a run of rows and some
 // columns, a thread eight neighbouring ones (16 bytes of 16-bit types, wherever they start) with fp32 sums in registers; the threads of a column
-// meet in LDS.  The rounding of dz is what the matrix cores take; two products with an unrounded one would be fp32's, at a tenth of the rate.  It makes the
-// error of the 16-bit gradients of gelu and silu 1.4 times as large (2-norm, bf16 0.0017 -> 0.0023); relu's and a plain layer's dz are not rounded by it.  Beside it the copies of operands whose rows are no multiple of 16 bytes, and activations that were kept in 8 bits.
+// meet in LDS.  The rounding of dz is what the matrix cores take; two products with an unrounded one would be fp32's, at a ninth of the rate.  It makes the
+// error of the 16-bit gradients of gelu and silu 1.4 times as large (2-norm, bf16 0.0017 -> 0.0023); relu's and a plain layer's dz are not rounded by it.
+// Beside it the copies of operands whose rows are no multiple of 16 bytes, and activations that were kept in 8 bits.
 // Behind them, the sums of the parts of a product's reduction and of the workgroups' columns, all in a fixed order.
 #include "linear_rows.h"
 
