@@ -399,6 +399,26 @@ int wc_linear_backward(const wc_linear_desc* desc, const wc_linear_gradients* gr
  * whose codes are 1 for what is above zero, -1 for what is not and 0 for NaN; as a tensor such a group still reads as NaN. */
 int wc_pack8(const void* x, signed char* codes, signed char* exponents, long long rows, int C, int dtype, int keep_sign, void* stream);
 int wc_unpack8(const signed char* codes, const signed char* exponents, void* x, long long rows, int C, int dtype, void* stream);
+
+/* Tensors in 4 bits, the OCP microscaling formats' MXFP4 (no counterpart in the reference).  The groups of 32 neighbouring channels of a row share a
+ * scale 2^e, e = floor(log2(largest magnitude)) - 2 but at least -127; a value is the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it, ties to
+ * the even code, at most 6.  A group with an infinity or a NaN has the scale 255 and reads as NaN.  Rows are padded with zeros to Cp, the next
+ * multiple of 128 channels: codes (rows, Cp / 2), the lower channel in a byte's low half; scales, e + 127, (ceil(rows / 32), Cp / 128, 32, 4):
+ * those of row r and group g at [r / 32][g / 4][r % 32][g % 4], zeros behind the last of either.  wc_packed4_bytes gives both sizes.  Both start at
+ * multiples of 16 bytes.  wc_unpack4 rounds to its type where that does not hold the value (fp16 below 2^-24 and above 65504).  C at most 2^22. */
+typedef struct {
+  const unsigned char* codes;
+  const unsigned char* scales;
+} wc_packed4;
+int wc_packed4_bytes(long long rows, int C, size_t* codes, size_t* scales);
+int wc_pack4(const void* x, unsigned char* codes, unsigned char* scales, long long rows, int C, int dtype, void* stream);
+int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x, long long rows, int C, int dtype, void* stream);
+
+/* A linear layer (wc_linear_forward, without z) whose weight w (K, C) is in 4 bits; x (rows, C) is of the descriptor's type, or packed as well (the
+ * other of the two null).  x of its type meets w's values in that type; of two packed operands the products are exact.  Sums fp32, one rounding. */
+int wc_linear4_workspace_bytes(const wc_linear_desc* desc, int x_packed, size_t* bytes);
+int wc_linear4_forward(const wc_linear_desc* desc, const void* x, const wc_packed4* x4, const wc_packed4* w, const void* bias, const void* residual, void* y,
+                       void* workspace, size_t workspace_bytes, void* stream);
 #ifdef __cplusplus
 }
 #endif

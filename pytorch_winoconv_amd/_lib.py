@@ -49,11 +49,16 @@ class LinearGradients(ctypes.Structure):
                 ("dw_dtype", ctypes.c_int), ("db", ctypes.c_void_p), ("db_dtype", ctypes.c_int), ("dz", ctypes.c_void_p)]
 
 
+class Packed4Parts(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/winoconv.h declares
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _desc_p, _plan_p = ctypes.POINTER(ConvDesc), ctypes.POINTER(Plan)
 _i64_5 = ctypes.POINTER(ctypes.c_int64)
 _linear_p, _linear_grads_p, _ll = ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearGradients), ctypes.c_longlong
+_packed4_p = ctypes.POINTER(Packed4Parts)
 SIGNATURES = {
     "wc_version": (ctypes.c_char_p, []),
     "wc_last_error": (ctypes.c_char_p, []),
@@ -95,6 +100,11 @@ SIGNATURES = {
     "wc_linear_backward": (_i, [_linear_p, _linear_grads_p, _vp, _sz, _vp]),
     "wc_pack8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "wc_unpack8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
+    "wc_packed4_bytes": (_i, [_ll, _i, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "wc_pack4": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
+    "wc_unpack4": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
+    "wc_linear4_workspace_bytes": (_i, [_linear_p, _i, ctypes.POINTER(_sz)]),
+    "wc_linear4_forward": (_i, [_linear_p, _vp, _packed4_p, _packed4_p, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -767,6 +767,73 @@ py::object unpack8(const at::Tensor& codes, const at::Tensor& exps, const py::ob
   return py::cast(x);
 }
 
+// ---- tensors in 4 bits (packed4.py) and linear layers over them
+unsigned char* bytes_of(const at::Tensor& t) { return t.data_ptr<uint8_t>(); }
+
+py::object pack4(const at::Tensor& x_) {
+  const int64_t nd = x_.dim();
+  if (!linear_type(x_) || nd < 1 || x_.numel() == 0 || !fits(x_.size(nd - 1))) return py::none();
+  const c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = x_.contiguous();
+  const int64_t C = x.size(nd - 1), rows = x.numel() / C, stages = (C + 127) / 128;
+  at::DimVector shape(x.sizes());
+  shape[nd - 1] = stages * 64;
+  const auto options = x.options().dtype(at::kByte);
+  at::Tensor codes = at::empty(shape, options), scales = at::empty({(rows + 31) / 32, stages, 32, 4}, options);
+  void* stream = stream_of(x);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_pack4(x.data_ptr(), bytes_of(codes), bytes_of(scales), rows, (int)C, dtype_of(x), stream));
+  }
+  return py::make_tuple(codes, scales);
+}
+
+// codes and scales of a Packed4 with elements
+at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
+  const c10::DeviceGuard guard(codes.device());
+  at::DimVector shape(codes.sizes());
+  shape[shape.size() - 1] = C;
+  at::Tensor x = at::empty(shape, codes.options().dtype(torch::python::detail::py_object_to_dtype(type)));
+  void* stream = stream_of(codes);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_unpack4(bytes_of(codes), bytes_of(scales), x.data_ptr(), x.numel() / C, (int)C, dtype_of(x), stream));
+  }
+  return x;
+}
+
+// x as it is, or the codes and scales of a Packed4 that reads as `type`; codes and scales of w (K, C)
+py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, const MaybeTensor& x_scales, const py::object& type, const at::Tensor& w_codes,
+                           const at::Tensor& w_scales, int64_t C, const MaybeTensor& bias_, const MaybeTensor& residual_, int activation, bool residual_after) {
+  const at::Tensor& first = x_ ? *x_ : *x_codes;
+  const int64_t nd = first.dim(), K = w_codes.size(0);
+  const at::ScalarType st = x_ ? first.scalar_type() : torch::python::detail::py_object_to_dtype(type);
+  const auto own = [&](const MaybeTensor& t) { return !t || (t->scalar_type() == st && t->device() == first.device() && t->layout() == at::kStrided); };
+  if ((x_ && (!linear_type(first) || nd < 1 || first.size(nd - 1) != C)) || first.numel() == 0 || w_codes.device() != first.device() || !own(bias_) || !own(residual_) ||
+      (bias_ && (bias_->dim() != 1 || bias_->size(0) != K)))
+    return py::none();
+  at::DimVector shape(first.sizes());
+  const int64_t rows = first.numel() / shape[nd - 1];
+  shape[nd - 1] = K;
+  if (residual_ && residual_->sizes() != at::IntArrayRef(shape)) return py::none();
+  const c10::DeviceGuard guard(first.device());
+  const MaybeTensor x = packed_rows(x_), bias = packed_rows(bias_), residual = packed_rows(residual_);
+  at::Tensor y = at::empty(shape, first.options().dtype(st));
+  const wc_linear_desc d = {rows, (int)C, (int)K, dtype_of(y), activation, residual_after};
+  const wc_packed4 w4 = {bytes_of(w_codes), bytes_of(w_scales)}, x4 = x ? wc_packed4{nullptr, nullptr} : wc_packed4{bytes_of(*x_codes), bytes_of(*x_scales)};
+  size_t bytes = 0;
+  check(wc_linear4_workspace_bytes(&d, !x, &bytes));
+  void* stream = stream_of(first);
+  at::Tensor ws;
+  if (bytes) ws = workspace_for(y, bytes, stream);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_linear4_forward(&d, data_or_null(x), x ? nullptr : &x4, &w4, data_or_null(bias), data_or_null(residual), y.data_ptr(), bytes ? ws.data_ptr() : nullptr,
+                             bytes, stream));
+  }
+  return py::cast(y);
+}
+
 bool channel_last_memory(const at::Tensor& t) {
   std::vector<int64_t> last{0};
   for (int64_t a = 2; a < t.dim(); ++a) last.push_back(a);
@@ -1300,5 +1367,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("activation"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"), py::arg("need_dz"), py::arg("w_type"), py::arg("b_type"));
   m.def("pack8", &pack8, py::arg("x"), py::arg("keep_sign"));
   m.def("unpack8", &unpack8, py::arg("codes"), py::arg("exponents"), py::arg("type"));
+  m.def("pack4", &pack4, py::arg("x"));
+  m.def("unpack4", &unpack4, py::arg("codes"), py::arg("scales"), py::arg("C"), py::arg("type"));
+  m.def("linear4_forward", &linear4_forward, py::arg("x"), py::arg("x_codes"), py::arg("x_scales"), py::arg("type"), py::arg("w_codes"), py::arg("w_scales"),
+        py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"));
   m.def("version", []() { return std::string(wc_version()); });
 }

@@ -1,0 +1,129 @@
+// Entry points of linear layers with operands in 4 bits (packed4.h): argument checks, which kernel, what goes where in the workspace.
+#include "packed4.h"
+
+#include <algorithm>
+
+using namespace wc;
+
+namespace {
+
+bool known(int dtype) { return dtype == WC_F32 || dtype == WC_F16 || dtype == WC_BF16; }
+
+int check_extents4(long long rows, int C, int dtype, const char* who) {
+  WC_CHECK_ARG(rows >= 0 && C > 0 && known(dtype), "%s: rows %lld, C %d, dtype %d", who, rows, C, dtype);
+  if (rows > (1ll << 31) - 1 || C > kMostChannels4)
+    return fail(WC_ERR_UNSUPPORTED, "%s: rows %lld, C %d (at most 2^31 - 1 and 2^22)", who, rows, C);
+  return WC_OK;
+}
+
+int check_packed(const wc_packed4* t, const char* what, const char* who) {
+  WC_CHECK_ARG(t && t->codes && t->scales, "%s: %s is null", who, what);
+  WC_CHECK_ARG(reinterpret_cast<uintptr_t>(t->codes) % 16 == 0 && reinterpret_cast<uintptr_t>(t->scales) % 16 == 0, "%s: %s must start at multiples of 16 bytes", who, what);
+  return WC_OK;
+}
+
+size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
+
+int check_desc4(const wc_linear_desc* d, const char* who) {
+  WC_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
+  if (int rc = check_extents4(d->rows, d->C, d->dtype, who)) return rc;
+  WC_CHECK_ARG(d->K > 0 && d->activation >= WC_ACT_NONE && d->activation <= WC_ACT_SILU, "%s: K %d, activation %d", who, d->K, d->activation);
+  if (d->K > kMostChannels4) return fail(WC_ERR_UNSUPPORTED, "%s: K %d (at most 2^22)", who, d->K);
+  return WC_OK;
+}
+
+LinearProduct product_of(const wc_linear_desc* d, const void* x, const void* bias, const void* res, void* y) {
+  return {x, nullptr, d->C, padded4(d->C), false, false, d->rows, d->K, d->C, {bias, res, y, nullptr, d->activation, d->residual_after != 0, 0}};
+}
+
+// Rows of x over which a pass over the packed weight takes the layer; above, the weight is widened first, or, x packed as well, tiles take it
+bool few(const wc_linear_desc* d) { return d->rows <= kMostFew4; }
+
+// the product of two packed operands, its reduction padded
+LinearProduct tiled(LinearProduct p) {
+  p.R = padded4(p.R);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wc_packed4_bytes(long long rows, int C, size_t* codes, size_t* scales) {
+  WC_CHECK_ARG(codes && scales, "wc_packed4_bytes: null output");
+  if (int rc = check_extents4(rows, C, WC_F32, "wc_packed4_bytes")) return rc;
+  *codes = (size_t)(rows * (padded4(C) / 2));
+  *scales = (size_t)scale_bytes4(rows, C);
+  return WC_OK;
+}
+
+int wc_pack4(const void* x, unsigned char* codes, unsigned char* scales, long long rows, int C, int dtype, void* stream) {
+  if (int rc = check_extents4(rows, C, dtype, "wc_pack4")) return rc;
+  if (rows == 0) return WC_OK;
+  WC_CHECK_ARG(x && codes && scales, "wc_pack4: null pointer");
+  return pack4(x, codes, scales, rows, C, dtype, stream);
+}
+
+int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x, long long rows, int C, int dtype, void* stream) {
+  if (int rc = check_extents4(rows, C, dtype, "wc_unpack4")) return rc;
+  if (rows == 0) return WC_OK;
+  WC_CHECK_ARG(x && codes && scales, "wc_unpack4: null pointer");
+  return unpack4(codes, scales, x, rows, C, dtype, stream);
+}
+
+int wc_linear4_workspace_bytes(const wc_linear_desc* d, int x_packed, size_t* bytes) {
+  WC_CHECK_ARG(bytes != nullptr, "wc_linear4_workspace_bytes: null output");
+  if (int rc = check_desc4(d, "wc_linear4_workspace_bytes")) return rc;
+  *bytes = 0;
+  if (d->rows == 0 || few(d)) return WC_OK;
+  if (x_packed) {
+    // (a plan goes by whether the epilogue is heavy: the larger of both)
+    LinearProduct p = tiled(product_of(d, nullptr, nullptr, nullptr, nullptr));
+    int s = 1;
+    for (const int after : {0, 1}) {
+      p.e.res = after ? d : nullptr;
+      s = std::max(s, product4_plan(p).s);
+    }
+    *bytes = s > 1 ? rounded((size_t)s * d->rows * d->K * 4) : 0;
+    return WC_OK;
+  }
+  size_t inner = 0;
+  if (int rc = wc_linear_workspace_bytes(d, &inner)) return rc;
+  *bytes = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2)) + inner;
+  return WC_OK;
+}
+
+int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4* x4, const wc_packed4* w4, const void* bias, const void* residual, void* y,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  if (int rc = wc_linear4_workspace_bytes(d, x4 != nullptr, &need)) return rc;
+  if (d->rows == 0) return WC_OK;
+  WC_CHECK_ARG((x != nullptr) != (x4 != nullptr) && y, "wc_linear4_forward: x is given as it is or packed, and y");
+  if (int rc = check_packed(w4, "w", "wc_linear4_forward")) return rc;
+  if (x4)
+    if (int rc = check_packed(x4, "x", "wc_linear4_forward")) return rc;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: workspace must be 256-byte aligned");
+  const LinearProduct p = product_of(d, x, bias, residual, y);
+  const Operand4 w = {w4->codes, w4->scales};
+  if (few(d)) {
+    const Operand4 xp = x4 ? Operand4{x4->codes, x4->scales} : Operand4{nullptr, nullptr};
+    return product4_few(p, x4 ? &xp : nullptr, w, d->dtype, stream);
+  }
+  if (x4) {
+    const LinearProduct t = tiled(p);
+    const ProductPlan plan = product4_plan(t);
+    if (plan.s > 1 && (size_t)plan.s * t.M * t.N * 4 > need) return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: %d parts do not fit the workspace", plan.s);
+    float* const parts = static_cast<float*>(workspace);
+    if (int rc = product4_dma(t, {x4->codes, x4->scales}, w, plan, parts, d->dtype, stream)) return rc;
+    const LinearJoin join = {t.e, parts, plan.s, t.M, t.N};
+    return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
+  }
+  char* const ws = static_cast<char*>(workspace);
+  const size_t wide = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2));
+  if (int rc = unpack4(w.codes, w.scales, ws, d->K, d->C, d->dtype, stream)) return rc;
+  return wc_linear_forward(d, x, ws, bias, residual, y, nullptr, ws + wide, need - wide, stream);
+}
+
+}  // extern "C"

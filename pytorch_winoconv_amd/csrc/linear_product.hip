@@ -22,19 +22,6 @@ struct GeneralArgs {
   int tiles_m, tiles_n, n_blocks, per_xcd;
 };
 
-template <typename T>
-__device__ __forceinline__ void finish(const LinearEpilogue& e, long long m, long long n, long long N, float v) {
-  const long long i = m * N + n;
-  if (e.bias) v += static_cast<float>(static_cast<const T*>(e.bias)[n]);
-  const float r = e.res ? static_cast<float>(static_cast<const T*>(e.res)[i]) : 0.f;
-  if (!e.res_after) v += r;
-  if (e.z) static_cast<T*>(e.z)[i] = static_cast<T>(v);
-  v = activate(v, e.act);
-  if (e.res_after) v += r;
-  if (e.y_f32) static_cast<float*>(e.y)[i] = v;
-  else static_cast<T*>(e.y)[i] = static_cast<T>(v);
-}
-
 template <typename T> constexpr int kGeneralPitch = 80 / sizeof(T);      // of a row of 64 bytes in LDS
 template <typename T> struct GeneralLds { T tile[2][2][64 * kGeneralPitch<T>]; };
 
@@ -121,7 +108,7 @@ __device__ __forceinline__ void general_block(const GeneralArgs& g, int hw_block
       const long long n = n0 + wn + 8 * q + 4 * lhi + e;
       if (n >= p.N) continue;
       if (g.parts) g.parts[(s * p.M + m) * p.N + n] = acc[4 * q + e];
-      else finish<T>(p.e, m, n, p.N, acc[4 * q + e]);
+      else finish_one<T>(p.e, m, n, p.N, acc[4 * q + e]);
     }
 }
 
@@ -192,7 +179,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(LinearProdu
   float v = 0.f;
 #pragma unroll 16
   for (int s = 0; s < kFewWaves * PLACES; ++s) v += sums[s][m][n];
-  finish<T>(p.e, m, n0 + n, p.N, v);
+  finish_one<T>(p.e, m, n0 + n, p.N, v);
 }
 // ... for a B of up to 4 MB, which is over before a second launch would begin; more loads are in flight in parts of tiles.  us, fp16, tiles and parts | this:
 // 1 x 1024 -> 1024 10.2 | 6.3, 8 x 2048 -> 2048 10.3 | 10.5, 8 x 4096 -> 4096 12.4 | 20.4
@@ -210,10 +197,10 @@ constexpr TileCost kGeneralCost = {{64, 64}, 4, 2, 2, 2, 4};
 
 // The least estimate over tiles and numbers of parts; parts' sums cost their way to memory and back, and the launch that adds them.  beside: us that another
 // product keeps the chip busy in the same launch, which leaves the tile as it is and makes parts fewer
-ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, double beside, double* busy = nullptr) {
+ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, double beside, double* busy = nullptr, bool few = true) {
   ProductPlan l = {dma, false, {64, 64}, 1, 0};
   const int forced = test_gemm_config();
-  if (forced < 0 && dma && few_rows_pay(p, dtype)) {
+  if (few && forced < 0 && dma && few_rows_pay(p, dtype)) {
     l.few = true;
     l.R_part = std::max(p.R, 1ll);
     return l;
@@ -252,6 +239,9 @@ ProductPlan plan_of(const LinearProduct& p, bool dma, bool heavy, int dtype, dou
 }
 
 }  // namespace
+
+// (codes of 4 bits lie in rows of a quarter as many 16-bit elements, which take the matrix instructions as long)
+ProductPlan product_plan4(const LinearProduct& p, bool heavy) { return plan_of(p, true, heavy, WC_F16, 0, nullptr, false); }
 
 ProductPlan product_plan(const LinearProduct& p, int dtype, const LinearProduct* beside) {
   const bool dma = test_gemm_config() != 31 && product_dma_fits(p, dtype);

@@ -40,6 +40,20 @@ __device__ __forceinline__ void store_run(void* to, long long i, int have, const
   }
 }
 
+// What becomes of one sum of a product
+template <typename T>
+__device__ __forceinline__ void finish_one(const LinearEpilogue& e, long long m, long long n, long long N, float v) {
+  const long long i = m * N + n;
+  if (e.bias) v += static_cast<float>(static_cast<const T*>(e.bias)[n]);
+  const float r = e.res ? static_cast<float>(static_cast<const T*>(e.res)[i]) : 0.f;
+  if (!e.res_after) v += r;
+  if (e.z) static_cast<T*>(e.z)[i] = static_cast<T>(v);
+  v = activate(v, e.act);
+  if (e.res_after) v += r;
+  if (e.y_f32) static_cast<float*>(e.y)[i] = v;
+  else static_cast<T*>(e.y)[i] = static_cast<T>(v);
+}
+
 // Workgroup `block` of 256 threads: rows of 8 bits back to T in rows of ld, zeros behind C; eight threads a group, four elements each
 struct UnpackArgs {
   long long first;           // workgroup of the launch, where it does nothing else

@@ -8,6 +8,9 @@ residual_after=True.  Sums and activations are fp32, y is rounded once.  In the 
 the type of the tensors before both products, which the matrix cores take: with 16-bit types and gelu or silu their error in the 2-norm is 1.4 times that
 of an unrounded dz (bf16 0.0023 of 0.0017).  float32, float16 and bfloat16; tensors that are not contiguous
 are copied first.  The GPU only.
+
+A frozen weight may be in 4 bits (packed4.Packed4): x then meets its values in x's type, or, in 4 bits itself, its values as they are; gradients
+pass through it to x, bias and residual.
 """
 import ctypes
 
@@ -19,6 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
 from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
+from .packed4 import Packed4, _made as _made4, linear4_forward, pack4, unpack4
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -30,7 +34,7 @@ def _activation(name):
 
 
 def _check_weight(shape, w, what):
-    if w.dim() != 2 or len(shape) < 1 or shape[-1] != w.shape[1] or not w.shape[0] or not w.shape[1]:
+    if len(w.shape) != 2 or len(shape) < 1 or shape[-1] != w.shape[1] or not w.shape[0] or not w.shape[1]:
         raise ValueError("%s of shape %r and a weight of shape %r: expected (..., C) and (K, C), neither of them 0" % (what, tuple(shape), tuple(w.shape)))
 
 
@@ -66,8 +70,11 @@ def _desc(rows, C, K, dtype, activation, residual_after=False):
 
 
 def linear_forward(x, w, bias=None, residual=None, activation="none", residual_after=False, keep_z=False):
-    """y (..., K) for x (..., C) and w (K, C); with keep_z (y, z).  bias (K) and residual (..., K) of x's type, or None."""
+    """y (..., K) for x (..., C) and w (K, C); with keep_z (y, z).  bias (K) and residual (..., K) of x's type, or None.  w may be a
+    Packed4, and then x too, whose result is of the type that x reads as."""
     act = _activation(activation)
+    if isinstance(w, Packed4) or isinstance(x, Packed4):
+        return _linear4(x, w, bias, residual, activation, residual_after, keep_z)
     if engine.USE_EXT:
         y = engine._ext.linear_forward(x, w, bias, residual, act, bool(residual_after), bool(keep_z))
         if y is not None:
@@ -92,12 +99,30 @@ def linear_forward(x, w, bias=None, residual=None, activation="none", residual_a
     return (y, z) if keep_z else y
 
 
+def _linear4(x, w, bias, residual, activation, residual_after, keep_z):
+    """linear_forward over a Packed4 w."""
+    if not isinstance(w, Packed4):
+        raise TypeError("linear_forward: x in 4 bits takes a weight in 4 bits, got a tensor")
+    _check_weight(x.shape, w, "x")
+    K = w.shape[0]
+    shape = tuple(x.shape[:-1]) + (K,)
+    if keep_z:
+        # z is for a backward pass, which wants many rows: the weight is widened for them all the same
+        if isinstance(x, Packed4):
+            raise NotImplementedError("linear_forward: no z of an x in 4 bits, which has no gradient")
+        return linear_forward(x, unpack4(w, x.dtype), bias, residual, activation, residual_after, True)
+    _check_like(bias, (K,), x.dtype, x.device, "the bias")
+    _check_like(residual, shape, x.dtype, x.device, "the residual")
+    return linear4_forward(x, w, bias, residual, ACTIVATIONS[activation], residual_after)
+
+
 def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=True, need_db=True, need_dz=False, w_type=None, b_type=None):
     """(dx, dw, db, dz) of linear_forward, None for those not asked for, from dy (..., K), x (..., C), w (K, C) and, with an
     activation, z; x and z may be Packed8.  For relu anything with z's sign does, y among it where no residual stands behind the activation.
     dw and db come in `w_type` and `b_type` (x's type; float32 sums unrounded, of products with the rounded dz; db's are of dz before
     that).  relu's gradient is 0 at z = 0 and NaN where z is.  dz is the gradient of z and so of a residual before
-    the activation; without an activation that is dy itself.  x may be None without need_dw, w without need_dx."""
+    the activation; without an activation that is dy itself.  x may be None without need_dw, w without need_dx.  w may be a Packed4, whose values
+    are read in dy's type."""
     act = _activation(activation)
     dtype, device = dy.dtype, dy.device
     if dy.dim() < 1 or not dy.shape[-1]:
@@ -112,7 +137,7 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     check_channels(max(K, C), "linear_backward")
     if w is not None:
         _check_weight((C,), w, "x")
-        _check_like(w, (K, C), dtype, device, "the weight")
+        _check_like(w, (K, C), w.dtype if isinstance(w, Packed4) else dtype, device, "the weight")
     if need_dw:
         if not C:
             raise ValueError("x of shape %r: expected (..., C)" % (tuple(x.shape),))
@@ -124,6 +149,8 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     if not dy.is_cuda:
         raise ValueError("winoconv runs on the GPU only: got a %s tensor" % device)
     engine._require_gpu(dy)
+    if isinstance(w, Packed4):
+        w = unpack4(w, dtype) if need_dx and dy.numel() else None
     w_type, b_type = w_type or dtype, b_type or dtype
     w_own, b_own = (t if t == torch.float32 else dtype for t in (w_type, b_type))
     if need_dz and not act:
@@ -168,14 +195,15 @@ def _check_checkpoint(checkpoint):
 
 class LinearFunction(torch.autograd.Function):
     """linear_forward with gradients.  Parameters of another type than x's are cast for the products, and their gradients come back in
-    theirs, float32 ones unrounded."""
+    theirs, float32 ones unrounded.  A Packed4 w has none."""
 
     @staticmethod
     def forward(ctx, x, w, bias, residual, activation, residual_after, checkpoint):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         ctx.types = (w.dtype, None if bias is None else bias.dtype)
+        ctx.channels4 = w.channels if isinstance(w, Packed4) else None
         ctx.conf = (activation, residual_after, checkpoint is not None)
-        own = lambda t: t if t is None or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731
+        own = lambda t: t if t is None or isinstance(t, Packed4) or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731
         w, bias = own(w), own(bias)
         slope = activation != "none" and (need_x or need_w or need_b or (need_r and not residual_after))
         by_sign = activation == "relu"
@@ -190,6 +218,8 @@ class LinearFunction(torch.autograd.Function):
         if checkpoint is not None:
             packed = [None if t is None else pack(t) for t, pack in ((kept[0], pack8), (z, pack_gates if by_sign else pack8))]
             kept = [packed[0] and packed[0].codes, kept[1], packed[1] and packed[1].codes, packed[0] and packed[0].exponents, packed[1] and packed[1].exponents]
+        if ctx.channels4 is not None:
+            kept[1:2] = [None, None] if kept[1] is None else [kept[1].codes, kept[1].scales]
         ctx.save_for_backward(*kept)
         return y
 
@@ -198,9 +228,12 @@ class LinearFunction(torch.autograd.Function):
     def backward(ctx, dy):
         activation, residual_after, packed = ctx.conf
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        x, w, z = ctx.saved_tensors[:3]
+        kept = list(ctx.saved_tensors)
+        if ctx.channels4 is not None:
+            kept[1:3] = [None if kept[1] is None else _made4(kept[1], kept[2], ctx.channels4, dy.dtype)]
+        x, w, z = kept[:3]
         if packed:
-            x_exp, z_exp = ctx.saved_tensors[3:]
+            x_exp, z_exp = kept[3:]
             x, z = (None if c is None else Packed8(c, e, dy.dtype) for c, e in ((x, x_exp), (z, z_exp)))
         w_type, b_type = ctx.types
         dx, dw, db, dz = linear_backward(dy, x, w, z, activation, need_x, need_w, need_b, need_r and not residual_after, w_type, b_type)
@@ -210,22 +243,29 @@ class LinearFunction(torch.autograd.Function):
 def linear(x, w, bias=None, residual=None, activation="none", residual_after=False, checkpoint=None, channel_axis=-1):
     """linear_forward with gradients.  checkpoint="int8" keeps x and z in 8 bits for the backward pass (checkpoint8); relu's gate
     stays z's own, so that of its gradients the weight's alone differs.  channel_axis: the axis of the channels in x and the residual, so that 1 takes the (N, C, H, W) tensors of the convolutions; a
-    tensor in channel-last memory is used as it is, and the result is one.  Reverse mode, once: operands with a forward-mode tangent are refused."""
+    tensor in channel-last memory is used as it is, and the result is one.  Reverse mode, once: operands with a forward-mode tangent are refused.
+    w may be a Packed4, through which gradients pass to x, bias and residual; with an x in 4 bits too there are none."""
     _check_checkpoint(checkpoint)
-    act = _activation(activation)
+    _activation(activation)
+    if isinstance(x, Packed4):
+        if channel_axis not in (-1, len(x.shape) - 1):
+            raise ValueError("linear: channel_axis %r of an x in 4 bits, whose channels are last" % (channel_axis,))
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual)):
+            raise NotImplementedError("linear: no gradient passes a layer whose x is in 4 bits")
+        return linear_forward(x, w, bias, residual, activation, residual_after)
     if channel_axis not in (-1, x.dim() - 1):
         if residual is not None and residual.dim() != x.dim():
             raise ValueError("the residual has shape %r, expected that of the result: %d axes" % (tuple(residual.shape), x.dim()))
         x = x.movedim(channel_axis, -1)
         residual = None if residual is None else residual.movedim(channel_axis, -1)
         return linear(x, w, bias, residual, activation, residual_after, checkpoint).movedim(-1, channel_axis)
-    given = [t for t in (x, w, bias, residual) if t is not None]
+    given = [t for t in (x, w, bias, residual) if t is not None and not isinstance(t, Packed4)]
     # (asked of torch for each tensor only within a level of forward mode: 3 us)
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
         raise NotImplementedError("linear has no forward-mode derivative: a tangent of its operands would be lost")
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return LinearFunction.apply(x, w, bias, residual, activation, bool(residual_after), checkpoint)
-    own = lambda t: t if t is None or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731
+    own = lambda t: t if t is None or isinstance(t, Packed4) or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731
     return linear_forward(x, own(w), own(bias), residual, activation, residual_after)
 
 
@@ -252,3 +292,55 @@ class MatrixLinear(nn.Module):
 
     def extra_repr(self):
         return "%d, %d, bias=%s, activation=%r" % (self.in_features, self.out_features, self.bias is not None, self.activation)
+
+    def pack4(self, x4=False):
+        """This layer for serving or behind trained ones: a MatrixLinear4 whose weight is this one's in 4 bits.  x4: its inputs are put into 4
+        bits too, which many rows take to the matrix cores' 4-bit rate; gradients do not pass it then."""
+        layer = MatrixLinear4.__new__(MatrixLinear4)
+        nn.Module.__init__(layer)
+        w4 = pack4(self.weight)
+        layer._hold(w4, self.bias, self.activation, self.residual_after, self.channel_axis, x4)
+        return layer
+
+
+class MatrixLinear4(nn.Module):
+    """A linear layer whose weight is frozen, in 4 bits (MatrixLinear.pack4, or of a Packed4 w (out_features, in_features)): 1/2 + 1/32 bytes a
+    weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales`; the bias is a parameter."""
+
+    def __init__(self, weight, bias=None, activation="none", residual_after=False, channel_axis=-1, x4=False):
+        super().__init__()
+        _activation(activation)
+        if not isinstance(weight, Packed4) or len(weight.shape) != 2:
+            raise TypeError("MatrixLinear4: the weight is a Packed4 of two axes")
+        self._hold(weight, bias, activation, residual_after, channel_axis, x4)
+
+    def _hold(self, w4, bias, activation, residual_after, channel_axis, x4):
+        self.out_features, self.in_features = w4.shape
+        self.activation, self.residual_after, self.channel_axis, self.x4 = activation, residual_after, channel_axis, bool(x4)
+        self.dtype = w4.dtype
+        self.register_buffer("codes", w4.codes)
+        self.register_buffer("scales", w4.scales)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=bias.requires_grad)
+
+    @property
+    def weight(self):
+        """The Packed4 of the buffers as they are now."""
+        return Packed4(self.codes, self.scales, self.in_features, self.dtype)
+
+    def forward(self, x, residual=None):
+        w = self.weight
+        if not self.x4:
+            return linear(x, w, self.bias, residual, self.activation, self.residual_after, None, self.channel_axis)
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise NotImplementedError("MatrixLinear4: no gradient passes a layer that puts its inputs into 4 bits")
+        axis = self.channel_axis
+        if axis not in (-1, x.dim() - 1):
+            return self._last(x.movedim(axis, -1), w, None if residual is None else residual.movedim(axis, -1)).movedim(-1, axis)
+        return self._last(x, w, residual)
+
+    def _last(self, x, w, residual):
+        bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
+        return linear(pack4(x), w, bias, residual, self.activation, self.residual_after)
+
+    def extra_repr(self):
+        return "%d, %d, bias=%s, activation=%r, x4=%r" % (self.in_features, self.out_features, self.bias is not None, self.activation, self.x4)
