@@ -419,6 +419,56 @@ int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x,
 int wc_linear4_workspace_bytes(const wc_linear_desc* desc, int x_packed, size_t* bytes);
 int wc_linear4_forward(const wc_linear_desc* desc, const void* x, const wc_packed4* x4, const wc_packed4* w, const void* bias, const void* residual, void* y,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Joins of a block to its stream, over rows of channels (no counterpart in the reference):
+ *   n = post(f),  d = drop(n),  s = stream_scale x + block_scale gate d,  y = pre(s)
+ * f (rows, C) is what the block gave, x (rows, C) or null the stream, post and pre the norms behind this block and before the next one: RMS
+ * v w / sqrt(mean(v^2) + eps), layer (v - mean) w / sqrt(var + eps) + bias, over a row; weight and bias null: 1 and 0.  gate null, or of 1 row or one a
+ * sample; the rows belong to `samples` samples in equal shares.  Parameters and gate of the tensors' type or fp32.  In fp32, s and y rounded
+ * once (y of s before that).  s or y may be null; y needs its norm.  f alone with pre and y: a norm; with drop and s: dropout.
+ *
+ * drop: channel c of row i is kept where word c % 8 of eight of 16 bits is at least drop_level, and then divided by 1 - drop_level / 65536; what is not
+ * kept is 0 whatever it was.  The words are those of Philox4x32-10 (Salmon et al., SC 2011), low halves first, with the counter (c / 8, i, the
+ * halves of the offset) and the key (the halves of the seed); drop_per_sample: word 0 of counter (0, sample, ...) for a sample's every value.  The mask is never
+ * stored: the backward pass draws it again.  drop_state, if not null: seed and offset in device memory, read by the kernel.
+ *
+ * post_stats, pre_stats (rows, 2), or null: mean and inverse deviation of either norm (RMS: 0), which the backward pass wants. */
+typedef enum { WC_NORM_NONE = 0, WC_NORM_RMS = 1, WC_NORM_LAYER = 2 } wc_norm_kind;
+typedef struct {
+  int kind;
+  float eps;
+  const void* weight;
+  const void* bias;
+  int dtype;
+} wc_norm;
+typedef struct {
+  long long rows, samples;
+  int C;
+  int dtype;
+  float stream_scale, block_scale;
+  long long gate_rows;              /* 0: no gate */
+  int gate_dtype;
+  int drop_level;
+  int drop_per_sample;
+  unsigned long long drop_seed, drop_offset;
+  const void* drop_state;
+  wc_norm post, pre;
+} wc_join_desc;
+int wc_join_forward(const wc_join_desc* desc, const void* f, const void* x, const void* gate, void* s, void* y, float* post_stats, float* pre_stats,
+                    void* stream);
+
+/* Its gradients.  ds, dy: of s and y, one of them may be null.  f is wanted by post and the gate's gradient, s by pre (as it was rounded).  Results that are null
+ * are not computed; those of parameters and gate come in their types.  Sums fp32 in a fixed order.  rows > 0.  Workspace 256-byte aligned; its size goes
+ * by which pointers are null. */
+typedef struct {
+  const void* ds; const void* dy;
+  const void* f; const void* s; const void* gate;
+  const float* post_stats; const float* pre_stats;
+  void* df; void* dx;
+  void* dpre_weight; void* dpre_bias; void* dpost_weight; void* dpost_bias; void* dgate;
+} wc_join_gradients;
+int wc_join_backward_workspace_bytes(const wc_join_desc* desc, const wc_join_gradients* gradients, size_t* bytes);
+int wc_join_backward(const wc_join_desc* desc, const wc_join_gradients* gradients, void* workspace, size_t workspace_bytes, void* stream);
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,8 @@ except ImportError:
     from .backend import AddGPU, Foo, WinoSplit, WinoConcat, DWM, winograd_conv, split_and_concat  # noqa: F401
 from .Add import add_gpu  # noqa: F401
 from .Split_and_Concat import wino_split, wino_concat  # noqa: F401
-from . import dwm, matrix_conv, matrix_conv3d, matrix_linear, checkpoint8, packed4, WinoConv, network, engine  # noqa: F401
+from . import dwm, matrix_conv, matrix_conv3d, matrix_linear, checkpoint8, packed4, residual, WinoConv, network, engine  # noqa: F401
 from .WinoConv import Wino, WinoConv2d, WinoConv3d  # noqa: F401
 from .matrix_linear import MatrixLinear, MatrixLinear4  # noqa: F401
+from .residual import BlockNorm, Dropout, ResidualStack  # noqa: F401
 from .network import Dwm  # noqa: F401

@@ -53,12 +53,29 @@ class Packed4Parts(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
 
 
+class NormParts(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int)]
+
+
+class JoinDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_longlong), ("samples", ctypes.c_longlong), ("C", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("stream_scale", ctypes.c_float), ("block_scale", ctypes.c_float), ("gate_rows", ctypes.c_longlong), ("gate_dtype", ctypes.c_int),
+                ("drop_level", ctypes.c_int), ("drop_per_sample", ctypes.c_int), ("drop_seed", ctypes.c_ulonglong), ("drop_offset", ctypes.c_ulonglong),
+                ("drop_state", ctypes.c_void_p), ("post", NormParts), ("pre", NormParts)]
+
+
+class JoinGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("ds", "dy", "f", "s", "gate", "post_stats", "pre_stats", "df", "dx", "dpre_weight", "dpre_bias",
+                                                     "dpost_weight", "dpost_bias", "dgate")]
+
+
 # name -> (restype, argtypes); every symbol include/winoconv.h declares
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _desc_p, _plan_p = ctypes.POINTER(ConvDesc), ctypes.POINTER(Plan)
 _i64_5 = ctypes.POINTER(ctypes.c_int64)
 _linear_p, _linear_grads_p, _ll = ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearGradients), ctypes.c_longlong
 _packed4_p = ctypes.POINTER(Packed4Parts)
+_join_p, _join_grads_p = ctypes.POINTER(JoinDesc), ctypes.POINTER(JoinGradients)
 SIGNATURES = {
     "wc_version": (ctypes.c_char_p, []),
     "wc_last_error": (ctypes.c_char_p, []),
@@ -105,6 +122,9 @@ SIGNATURES = {
     "wc_unpack4": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp]),
     "wc_linear4_workspace_bytes": (_i, [_linear_p, _i, ctypes.POINTER(_sz)]),
     "wc_linear4_forward": (_i, [_linear_p, _vp, _packed4_p, _packed4_p, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "wc_join_forward": (_i, [_join_p] + [_vp] * 8),
+    "wc_join_backward_workspace_bytes": (_i, [_join_p, _join_grads_p, ctypes.POINTER(_sz)]),
+    "wc_join_backward": (_i, [_join_p, _join_grads_p, _vp, _sz, _vp]),
 }
 
 _lib = None

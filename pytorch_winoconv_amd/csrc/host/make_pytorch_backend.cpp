@@ -834,6 +834,91 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
   return py::cast(y);
 }
 
+// ---- joins of blocks to their stream (residual.py): None, as above, for operands that do not fit together
+bool own_or_wide(const MaybeTensor& t, const at::Tensor& like) {
+  return !t || ((t->scalar_type() == like.scalar_type() || t->scalar_type() == at::kFloat) && t->device() == like.device() && t->layout() == at::kStrided);
+}
+MaybeTensor dense(const MaybeTensor& t) { return t ? MaybeTensor(t->contiguous()) : t; }
+bool channels_of(const MaybeTensor& t, int64_t C) { return !t || (t->dim() == 1 && t->size(0) == C); }
+wc_norm norm_of(int kind, double eps, const MaybeTensor& w, const MaybeTensor& b, const at::Tensor& like) {
+  return {kind, (float)eps, data_or_null(w), data_or_null(b), dtype_of(w ? *w : b ? *b : like)};
+}
+bool norm_fits(const MaybeTensor& w, const MaybeTensor& b, const at::Tensor& f, int64_t C) {
+  return own_or_wide(w, f) && own_or_wide(b, f) && channels_of(w, C) && channels_of(b, C) && !(w && b && w->scalar_type() != b->scalar_type());
+}
+wc_join_desc join_desc(const at::Tensor& f, const MaybeTensor& gate, double a, double b, const wc_norm& post, const wc_norm& pre, int level, bool per_sample, uint64_t seed,
+                       uint64_t offset, const MaybeTensor& state) {
+  const int64_t C = f.size(f.dim() - 1);
+  return {f.numel() / C, f.dim() > 1 ? f.size(0) : 1, (int)C, dtype_of(f), (float)a, (float)b, gate ? gate->numel() / C : 0, gate ? dtype_of(*gate) : dtype_of(f), level, per_sample,
+          seed, offset, data_or_null(state), post, pre};
+}
+
+py::object join_forward(const at::Tensor& f_, const MaybeTensor& x_, const MaybeTensor& gate_, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_,
+                        const MaybeTensor& post_b_, int pre_kind, double pre_eps, const MaybeTensor& pre_w_, const MaybeTensor& pre_b_, int level, bool per_sample, uint64_t seed,
+                        uint64_t offset, const MaybeTensor& state, bool need_s, bool keep) {
+  const int64_t nd = f_.dim();
+  if (!linear_type(f_) || nd < 1 || f_.numel() == 0 || f_.size(nd - 1) > 1 << 24) return py::none();
+  const int64_t C = f_.size(nd - 1), samples = nd > 1 ? f_.size(0) : 1;
+  if (!same_kind(x_, f_) || (x_ && x_->sizes() != f_.sizes()) || !own_or_wide(gate_, f_) || !norm_fits(post_w_, post_b_, f_, C) || !norm_fits(pre_w_, pre_b_, f_, C) ||
+      (state && state->device() != f_.device()))
+    return py::none();
+  if (gate_ && !(gate_->dim() == 1 && gate_->size(0) == C) && !(gate_->dim() == 2 && gate_->size(0) == samples && gate_->size(1) == C)) return py::none();
+  const c10::DeviceGuard guard(f_.device());
+  const at::Tensor f = f_.contiguous();
+  const MaybeTensor x = dense(x_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_), pre_b = dense(pre_b_);
+  const wc_join_desc d = join_desc(f, gate, a, b, norm_of(post_kind, post_eps, post_w, post_b, f), norm_of(pre_kind, pre_eps, pre_w, pre_b, f), level, per_sample, seed, offset, state);
+  at::Tensor s, y, post_stats, pre_stats;
+  const auto wide = f.options().dtype(at::kFloat);
+  if (need_s) s = at::empty(f.sizes(), f.options());
+  if (pre_kind) y = at::empty(f.sizes(), f.options());
+  if (keep && post_kind) post_stats = at::empty({d.rows, 2}, wide);
+  if (keep && pre_kind) pre_stats = at::empty({d.rows, 2}, wide);
+  auto at_or_null = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  void* stream = stream_of(f);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_join_forward(&d, f.data_ptr(), data_or_null(x), data_or_null(gate), at_or_null(s), at_or_null(y), static_cast<float*>(at_or_null(post_stats)),
+                          static_cast<float*>(at_or_null(pre_stats)), stream));
+  }
+  return py::make_tuple(or_none(s), or_none(y), or_none(post_stats), or_none(pre_stats));
+}
+
+// operands that the Python layer has checked; rows > 0
+py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& gate_, const MaybeTensor& post_stats,
+                        const MaybeTensor& pre_stats, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_, const MaybeTensor& post_b_, int pre_kind,
+                        double pre_eps, const MaybeTensor& pre_w_, const MaybeTensor& pre_b_, int level, bool per_sample, uint64_t seed, uint64_t offset,
+                        const MaybeTensor& state, bool need_f, bool need_x, bool need_gate, bool need_post, bool need_pre) {
+  const at::Tensor& like = ds_ ? *ds_ : *dy_;
+  const c10::DeviceGuard guard(like.device());
+  const MaybeTensor ds = dense(ds_), dy = dense(dy_), f = dense(f_), s = dense(s_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_),
+                    pre_b = dense(pre_b_);
+  const wc_join_desc d = join_desc(like, gate, a, b, norm_of(post_kind, post_eps, post_w, post_b, like), norm_of(pre_kind, pre_eps, pre_w, pre_b, like), level, per_sample, seed, offset,
+                                   state);
+  at::Tensor df, dx, dpost_w, dpost_b, dgate, dpre_w, dpre_b;
+  auto fresh = [](const at::Tensor& t) { return at::empty(t.sizes(), t.options()); };
+  if (need_f) df = fresh(like);
+  if (need_x) dx = fresh(like);
+  if (need_gate && gate) dgate = fresh(*gate);
+  if (need_post && post_w) dpost_w = fresh(*post_w);
+  if (need_post && post_b) dpost_b = fresh(*post_b);
+  if (need_pre && pre_w) dpre_w = fresh(*pre_w);
+  if (need_pre && pre_b) dpre_b = fresh(*pre_b);
+  auto at_or_null = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  auto stats = [](const MaybeTensor& t) { return t ? t->data_ptr<float>() : nullptr; };
+  const wc_join_gradients q = {data_or_null(ds), data_or_null(dy), data_or_null(f), data_or_null(s), data_or_null(gate), stats(post_stats), stats(pre_stats), at_or_null(df),
+                               at_or_null(dx), at_or_null(dpre_w), at_or_null(dpre_b), at_or_null(dpost_w), at_or_null(dpost_b), at_or_null(dgate)};
+  size_t bytes = 0;
+  check(wc_join_backward_workspace_bytes(&d, &q, &bytes));
+  void* stream = stream_of(like);
+  at::Tensor ws;
+  if (bytes) ws = workspace_for(like, bytes, stream);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_join_backward(&d, &q, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  }
+  return py::make_tuple(or_none(df), or_none(dx), or_none(dpre_w), or_none(dpre_b), or_none(dpost_w), or_none(dpost_b), or_none(dgate));
+}
+
 bool channel_last_memory(const at::Tensor& t) {
   std::vector<int64_t> last{0};
   for (int64_t a = 2; a < t.dim(); ++a) last.push_back(a);
@@ -1371,5 +1456,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack4", &unpack4, py::arg("codes"), py::arg("scales"), py::arg("C"), py::arg("type"));
   m.def("linear4_forward", &linear4_forward, py::arg("x"), py::arg("x_codes"), py::arg("x_scales"), py::arg("type"), py::arg("w_codes"), py::arg("w_scales"),
         py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"));
+  m.def("join_forward", &join_forward);
+  m.def("join_backward", &join_backward);
   m.def("version", []() { return std::string(wc_version()); });
 }

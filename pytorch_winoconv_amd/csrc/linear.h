@@ -68,12 +68,12 @@ __device__ __forceinline__ float through(float dy, float z, int act) {
 // ---- launches -----------------------------------------------------------------------------------
 // A launch has fewer than 2^32 threads along an axis.  Workgroups, of at most 512 threads, that one takes; work of more goes in several
 constexpr long long kMostBlocks = (1ll << 23) - kXcds;
-// launch(first, n) over workgroups first .. first + n - 1 of `blocks`
+// launch(first, n) over workgroups first .. first + n - 1 of `blocks` (most: half of it for workgroups of 1024)
 template <typename F>
-int in_launches(long long blocks, F&& launch) {
-  for (long long first = 0; first < blocks; first += kMostBlocks) {
+int in_launches(long long blocks, F&& launch, long long most = kMostBlocks) {
+  for (long long first = 0; first < blocks; first += most) {
     const long long left = blocks - first;
-    if (int rc = launch(first, (unsigned)(left < kMostBlocks ? left : kMostBlocks))) return rc;
+    if (int rc = launch(first, (unsigned)(left < most ? left : most))) return rc;
   }
   return WC_OK;
 }
