@@ -62,6 +62,7 @@ enum { kPreWeight, kPreBias, kPostWeight, kPostBias, kGateSum };
 struct Random8 { unsigned w[4]; };
 __device__ __forceinline__ Random8 philox(unsigned c0, unsigned c1, unsigned long long offset, unsigned long long seed) {
   unsigned x0 = c0, x1 = c1, x2 = (unsigned)offset, x3 = (unsigned)(offset >> 32), k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+  asm volatile("" : "+s"(k0), "+s"(k1));         // (the rounds' keys, kept over the loop over rows, would be spilled)
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long p = 0xD2511F53ull * x0, q = 0xCD9E8D57ull * x2;
@@ -75,7 +76,15 @@ __device__ __forceinline__ Random8 philox(unsigned c0, unsigned c1, unsigned lon
   return {{x0, x1, x2, x3}};
 }
 struct Keys { unsigned long long seed, offset; };
-__device__ __forceinline__ Keys keys_of(const Dropout& d) { return d.state ? Keys{d.state[0], d.state[1]} : Keys{d.seed, d.offset}; }
+// (the same for all: in scalar registers)
+__device__ __forceinline__ unsigned long long uniform(unsigned long long v) {
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ __forceinline__ Keys keys_of(const Dropout& d) {
+  Keys k = {d.seed, d.offset};
+  if (d.state) k = {uniform(d.state[0]), uniform(d.state[1])};
+  return k;
+}
 
 // what channels 8 j .. of a row are multiplied by is `scale` where the bit of the mask is set, and 0 - whatever the value - where it is not
 __device__ __forceinline__ unsigned kept8(const Dropout& d, const Keys& k, unsigned j, unsigned row) {
@@ -96,11 +105,19 @@ struct Team {
   int lanes;
   float* lds;                  // WAVES above 1: two rows of 2 WAVES
   int turn;
+  // (exchanges within 16 lanes are operands of the additions; mirrored, not across, which is the same once the halves agree)
+  template <int CONTROL> static __device__ __forceinline__ void add_across(float& u) {
+    u += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(u), CONTROL, 0xf, 0xf, true));
+  }
   __device__ __forceinline__ void sum(float& u, float& v) {
-    for (int d = 1; d < (WAVES > 1 ? 64 : lanes); d <<= 1) {
-      u += __shfl_xor(u, d);
-      v += __shfl_xor(v, d);
-    }
+    const int n = WAVES > 1 ? 64 : lanes;
+    constexpr int kPairs = 0xB1, kQuads = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+    if (n > 1) { add_across<kPairs>(u); add_across<kPairs>(v); }
+    if (n > 2) { add_across<kQuads>(u); add_across<kQuads>(v); }
+    if (n > 4) { add_across<kHalfMirror>(u); add_across<kHalfMirror>(v); }
+    if (n > 8) { add_across<kMirror>(u); add_across<kMirror>(v); }
+    if (n > 16) { u += __shfl_xor(u, 16); v += __shfl_xor(v, 16); }
+    if (n > 32) { u += __shfl_xor(u, 32); v += __shfl_xor(v, 32); }
     if constexpr (WAVES > 1) {
       // (the two rows take turns, so that one barrier is enough: before a row is written again everyone has passed the other's)
       float* const row = lds + turn * 2 * WAVES;
@@ -124,6 +141,69 @@ struct Team {
     return u;
   }
 };
+
+// Channels c .. c + 7 of a row of C, zeros behind its end: one 16-byte load (fp32: two) wherever it starts.  That of the row's last channels starts
+// before them, and what is in front is shifted out; no lane takes a branch to loads of single elements, which all would wait for.
+// EVEN: C is a multiple of eight.  `there`: the row is, else zeros.
+template <typename T> struct Raw8 { uint32_t w[2 * sizeof(T)]; };
+template <typename T, bool EVEN>
+__device__ __forceinline__ Raw8<T> load8(const void* p, long long row, int c, int C, bool there) {
+  constexpr int W = 2 * sizeof(T);
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < W; ++i) r.w[i] = 0u;
+  if (EVEN || C < 8) {
+    if (EVEN && (!there || c >= C)) return r;
+    T v[8];
+    load_run<T, 8>(p, row * C + c, EVEN ? 8 : there ? max(min(C - c, 8), 0) : 0, v);
+    __builtin_memcpy(&r, v, sizeof(r));
+    return r;
+  }
+  if (!there || c >= C) return r;
+  const int at = min(c, C - 8);
+  int k = c - at;
+  const Run<T, 8> v = *reinterpret_cast<const Run<T, 8>*>(static_cast<const T*>(p) + row * C + at);
+  __builtin_memcpy(&r, &v, sizeof(r));
+  if (k > 0) {
+    asm volatile("" : "+v"(k));                        // (compared anew: its bits as masks, kept over the loop over rows, would be spilled)
+    // by whole words, then by half a one
+    constexpr int ONE = sizeof(T) == 4 ? 1 : 0;        // words of a shift by one element
+#pragma unroll
+    for (int bit = 4; bit >= (ONE ? 1 : 2); bit /= 2) {
+      const int words = bit * (int)sizeof(T) / 4;
+#pragma unroll
+      for (int i = 0; i < W; ++i) r.w[i] = k & bit ? (i + words < W ? r.w[i + words] : 0u) : r.w[i];
+    }
+    if constexpr (!ONE) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint32_t next = i + 1 < W ? r.w[i + 1] : 0u;
+        r.w[i] = k & 1 ? r.w[i] >> 16 | next << 16 : r.w[i];
+      }
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void floats_of(const Raw8<T>& r, float (&v)[8]) {
+  T t[8];
+  __builtin_memcpy(t, &r, sizeof(r));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
+}
+template <typename T, bool EVEN>
+__device__ __forceinline__ void parameter8(const void* p, int wide, long long row, int c, int C, float (&v)[8], float otherwise) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = otherwise;
+  } else if (wide) {
+    floats_of<float>(load8<float, EVEN>(p, row, c, C, true), v);
+  } else {
+    floats_of<T>(load8<T, EVEN>(p, row, c, C, true), v);
+  }
+}
+// x where element e of `have` is there, 0 where it is not; EVEN: eight are there or none, whose x is 0 as it is
+template <bool EVEN> __device__ __forceinline__ float kept_element(float x, int e, int have) { return EVEN || e < have ? x : 0.f; }
 
 template <typename T>
 __device__ __forceinline__ void load_floats(const void* p, long long i, int have, float (&v)[8]) {
@@ -160,8 +240,10 @@ struct TeamShape { int vectors, waves, lanes; };
 
 int join_forward(const JoinArgs& a, int dtype, void* stream);
 int join_backward(const JoinGradients& g, int dtype, void* stream);
+template <typename T> int join_backward_of(const JoinGradients& g, void* stream);      // residual_backward.inc
+TeamShape back_shape(int C);
 // how many workgroups, and in how many parts a segment, a backward pass takes
-void join_plan(JoinGradients* g, bool gate_sums);
+void join_plan(JoinGradients* g);
 // dst[which] = the sums of part[which] over the workgroups (gate of a sample: over a sample's)
 struct JoinSum { const float* part; void* dst; int wide; long long segments; int parts; };
 int join_sums(const JoinSum* sums, int n, int C, int dtype, void* stream);

@@ -55,7 +55,7 @@ Backward backward_plan(const wc_join_desc* d, const wc_join_gradients* q, char* 
   if (!q->dy) g.pre.kind = WC_NORM_NONE;
   if (g.gate_rows == kGateRow) g.dgate_rows = q->dgate;
   void* const to[5] = {q->dpre_weight, q->dpre_bias, q->dpost_weight, q->dpost_bias, g.dgate_rows ? nullptr : q->dgate};
-  join_plan(&g, to[kGateSum] != nullptr);
+  join_plan(&g);
   size_t at = 0;
   for (int k = 0; k < 5; ++k) {
     g.part[k] = nullptr;

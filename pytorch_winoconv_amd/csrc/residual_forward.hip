@@ -6,7 +6,7 @@ namespace wc {
 namespace {
 
 // (v - mean) / deviation, in place; zeros behind `have`
-template <int NV, int WAVES>
+template <bool EVEN, int NV, int WAVES>
 __device__ __forceinline__ void normalise(Team<WAVES>& team, float (&v)[NV][8], const int (&have)[NV], const Norm& n, int C, float* stats, long long row, bool first) {
   float mean = 0.f;
   if (n.kind == WC_NORM_LAYER) {
@@ -22,7 +22,7 @@ __device__ __forceinline__ void normalise(Team<WAVES>& team, float (&v)[NV][8], 
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[i][e] = e < have[i] ? v[i][e] - mean : 0.f;
+      v[i][e] = kept_element<EVEN>(v[i][e] - (have[i] ? mean : 0.f), e, have[i]);
       t = fmaf(v[i][e], v[i][e], t);
     }
   const float inverse = 1.f / sqrtf(team.sum(t) / C + n.eps);
@@ -42,69 +42,110 @@ __device__ __forceinline__ void scale_shift(const Norm& n, int c, int have, floa
   for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], w[e], b[e]);
 }
 
-template <typename T, int NV, int WAVES>
-__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(JoinArgs a, int lanes, long long first_block) {
+// Rows blockIdx.x, blockIdx.x + gridDim.x, ... a team; one vector a thread: the next row is on its way while one is worked on, and the parameters stay in registers
+template <typename T, int NV, int WAVES, bool EVEN, bool AHEAD, bool ALONE>
+__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(JoinArgs a, int lanes) {
   __shared__ float meet[WAVES > 1 ? 4 * WAVES : 1];
-  const int width = WAVES > 1 ? 64 * WAVES : lanes, slot = threadIdx.x & (width - 1);
-  const long long row = (first_block + blockIdx.x) * (WAVES > 1 ? 1 : 256 / lanes) + (WAVES > 1 ? 0 : threadIdx.x / lanes);
-  const bool there = row < a.rows;             // (lanes of other teams of the wavefront go on, and it takes them for its exchanges)
+  const int width = WAVES > 1 ? 64 * WAVES : lanes, slot = threadIdx.x & (width - 1), teams = WAVES > 1 ? 1 : 256 / lanes;
+  const long long step = (long long)gridDim.x * teams;
   Team<WAVES> team = {lanes, meet, 0};
-  int c[NV], have[NV];
-  float v[NV][8], r[NV][8];
+  const Keys keys = !ALONE && a.drop.level ? keys_of(a.drop) : Keys{0, 0};
+  int c[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    c[i] = (i * width + slot) * 8;
-    have[i] = there ? max(min(a.C - c[i], 8), 0) : 0;
-    load_floats<T>(a.f, row * a.C + c[i], have[i], v[i]);
-  }
+  for (int i = 0; i < NV; ++i) c[i] = (i * width + slot) * 8;
+  Raw8<T> f[NV], x[NV];
+  auto load = [&](long long row) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (a.x) {
-      load_floats<T>(a.x, row * a.C + c[i], have[i], r[i]);
-    } else {
+    for (int i = 0; i < NV; ++i) f[i] = load8<T, EVEN>(a.f, row, c[i], a.C, row < a.rows);
+    if (!ALONE && a.x) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[i][e] = 0.f;
+      for (int i = 0; i < NV; ++i) x[i] = load8<T, EVEN>(a.x, row, c[i], a.C, row < a.rows);
     }
-  }
-  if (a.post.kind) {
-    normalise<NV, WAVES>(team, v, have, a.post, a.C, a.post_stats, row, slot == 0 && there);
+  };
+  constexpr int KEPT = AHEAD ? NV : 1;
+  float post_w[KEPT][8], post_b[KEPT][8], pre_w[KEPT][8], pre_b[KEPT][8], gate[KEPT][8];
+  auto parameters = [&](const Norm& n, int c, float (&w)[8], float (&b)[8]) {
+    parameter8<T, EVEN>(n.weight, n.wide, 0, c, a.C, w, 1.f);
+    parameter8<T, EVEN>(n.bias, n.wide, 0, c, a.C, b, 0.f);
+  };
+  if constexpr (AHEAD) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) scale_shift<T>(a.post, c[i], have[i], v[i]);
+    for (int i = 0; i < KEPT; ++i) {
+      if (!ALONE && a.post.kind) parameters(a.post, c[i], post_w[i], post_b[i]);
+      if (a.pre.kind) parameters(a.pre, c[i], pre_w[i], pre_b[i]);
+      if (!ALONE && a.gate_rows == kGateChannel) parameter8<T, EVEN>(a.gate, a.gate_wide, 0, c[i], a.C, gate[i], 0.f);
+    }
+    load((long long)blockIdx.x * teams + threadIdx.x / width);
   }
-  if (a.drop.level) {
-    const Keys k = keys_of(a.drop);
-    const unsigned all = a.drop.per_sample ? kept_sample(a.drop, k, (unsigned)row / (unsigned)a.per) : 0u;
+  for (long long base = (long long)blockIdx.x * teams; base < a.rows; base += step) {
+    const long long row = base + (WAVES > 1 ? 0 : threadIdx.x / lanes);
+    const bool there = row < a.rows;           // (lanes of other teams of the wavefront go on, and it takes them for its exchanges)
+    if constexpr (!AHEAD) load(row);
+    int have[NV];
+    float v[NV][8], r[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const unsigned kept = a.drop.per_sample ? all : kept8(a.drop, k, (unsigned)c[i] / 8, (unsigned)row);
+      have[i] = there ? max(min(a.C - c[i], 8), 0) : 0;
+      asm volatile("" : "+v"(have[i]));
+      floats_of<T>(f[i], v[i]);
+      if (!ALONE && a.x) floats_of<T>(x[i], r[i]);
+      else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = kept >> e & 1 ? v[i][e] * a.drop.scale : 0.f;
+        for (int e = 0; e < 8; ++e) r[i][e] = 0.f;
+      }
     }
-  }
-  const long long g0 = a.gate_rows ? gate_row(a.gate_rows, row, a.per) * a.C : 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (a.gate_rows) {
-      float g[8];
-      load_parameter<T>(a.gate, a.gate_wide, g0 + c[i], have[i], g, 0.f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] *= g[e];
+    if constexpr (AHEAD) {
+      if (base + step < a.rows) load(row + step);
     }
+    if (!ALONE && a.post.kind) {
+      normalise<EVEN, NV, WAVES>(team, v, have, a.post, a.C, a.post_stats, row, slot == 0 && there);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] *= a.b;
-    if (a.x) {
+      for (int i = 0; i < NV; ++i) {
+        const int k = AHEAD ? i : 0;
+        if constexpr (!AHEAD) parameters(a.post, c[i], post_w[k], post_b[k]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = fmaf(a.a, r[i][e], v[i][e]);
+        for (int e = 0; e < 8; ++e) v[i][e] = fmaf(v[i][e], post_w[k][e], post_b[k][e]);
+      }
     }
-    if (a.s) store_floats<T>(a.s, row * a.C + c[i], have[i], v[i]);
-  }
-  if (!a.pre.kind) return;
-  // (of s before its rounding)
-  normalise<NV, WAVES>(team, v, have, a.pre, a.C, a.pre_stats, row, slot == 0 && there);
+    if (!ALONE && a.drop.level) {
+      const unsigned all = a.drop.per_sample ? kept_sample(a.drop, keys, (unsigned)row / (unsigned)a.per) : 0u;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    scale_shift<T>(a.pre, c[i], have[i], v[i]);
-    store_floats<T>(a.y, row * a.C + c[i], have[i], v[i]);
+      for (int i = 0; i < NV; ++i) {
+        const unsigned kept = a.drop.per_sample ? all : kept8(a.drop, keys, (unsigned)c[i] / 8, (unsigned)row);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = kept >> e & 1 ? v[i][e] * a.drop.scale : 0.f;
+      }
+    }
+    const long long g0 = !ALONE && a.gate_rows && there ? gate_row(a.gate_rows, row, a.per) : 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!ALONE && a.gate_rows) {
+        const int k = AHEAD ? i : 0;
+        if (!AHEAD || a.gate_rows != kGateChannel) parameter8<T, EVEN>(a.gate, a.gate_wide, g0, c[i], a.C, gate[k], 0.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] *= gate[k][e];
+      }
+      if (!ALONE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] *= a.b;
+      }
+      if (!ALONE && a.x) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = fmaf(a.a, r[i][e], v[i][e]);
+      }
+      if (!ALONE && a.s) store_floats<T>(a.s, row * a.C + c[i], have[i], v[i]);
+    }
+    if (!ALONE && !a.pre.kind) continue;
+    // (of s before its rounding)
+    normalise<EVEN, NV, WAVES>(team, v, have, a.pre, a.C, a.pre_stats, row, slot == 0 && there);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = AHEAD ? i : 0;
+      if constexpr (!AHEAD) parameters(a.pre, c[i], pre_w[k], pre_b[k]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = fmaf(v[i][e], pre_w[k][e], pre_b[k][e]);
+      store_floats<T>(a.y, row * a.C + c[i], have[i], v[i]);
+    }
   }
 }
 
@@ -189,29 +230,44 @@ __global__ __launch_bounds__(kLong) void join_long_kernel(JoinArgs a, long long 
 
 int join_forward(const JoinArgs& a, int dtype, void* stream) {
   const int vectors = ceil_div(a.C, 8);
+  const bool alone = a.pre.kind && !a.post.kind && !a.x && !a.gate_rows && !a.drop.level && !a.s && a.b == 1.f;
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    auto go = [&](auto nv, auto waves, int lanes) {
-      constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value;
-      return in_launches(WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), [&](long long first, unsigned blocks) -> int {
-        hipLaunchKernelGGL((join_kernel<T, NV, WAVES>), dim3(blocks), dim3(WAVES > 1 ? 64 * WAVES : 256), 0, as_stream(stream), a, lanes, first);
-        WC_CHECK_LAUNCH("join_kernel");
-        return WC_OK;
-      }, kMostBlocks / 2);
+    // as many workgroups as the compute units hold at once, or as there are rows
+    auto go = [&](auto nv, auto waves, auto ahead, int lanes) -> int {
+      constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value, THREADS = WAVES > 1 ? 64 * WAVES : 256;
+      constexpr bool AHEAD = decltype(ahead)::value;
+      const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? kCus * (2048 / THREADS) : kMostBlocks / 2;
+      constexpr bool BOTH = (NV == 1 && WAVES == 1) || (NV == 2 && WAVES == 16), ALONE = BOTH || NV == 2;      // what is there of a form
+      auto fn = a.C % 8 == 0 ? &join_kernel<T, NV, WAVES, true, AHEAD, ALONE> : &join_kernel<T, NV, WAVES, false, AHEAD, ALONE>;
+      if constexpr (BOTH) {
+        if (!alone) fn = a.C % 8 == 0 ? &join_kernel<T, NV, WAVES, true, AHEAD, false> : &join_kernel<T, NV, WAVES, false, AHEAD, false>;
+      }
+      hipLaunchKernelGGL(fn, dim3((unsigned)(wanted < most ? wanted : most)), dim3(THREADS), 0, as_stream(stream), a, lanes);
+      WC_CHECK_LAUNCH("join_kernel");
+      return WC_OK;
     };
-    // a wavefront a row waits for nobody; few rows are over sooner with more threads each
-    const bool many = a.rows >= 4 * kCus;
+    const std::true_type ahead;
+    const std::false_type whole;
     if (vectors <= 64) {
       int lanes = 1;
       while (lanes < vectors) lanes *= 2;
-      return go(ic<1>{}, ic<1>{}, lanes);
+      return go(ic<1>{}, ic<1>{}, ahead, lanes);
     }
-    if (vectors <= 128 && many) return go(ic<2>{}, ic<1>{}, 64);
-    if (vectors <= 256 && many) return go(ic<4>{}, ic<1>{}, 64);
-    if (vectors <= 256) return go(ic<1>{}, ic<4>{}, 64);
-    if (vectors <= 512) return go(ic<2>{}, ic<4>{}, 64);
-    if (vectors <= 1024) return go(ic<4>{}, ic<4>{}, 64);
-    if (vectors <= 4096) return go(ic<4>{}, ic<16>{}, 64);
+    // A norm alone takes two vectors a thread and every row a workgroup of its own: there is little to keep in registers, and fewer wait at a barrier
+    // (us, bf16 rms, two | one ahead: 65536 x 1024 46.9 | 47.3, 16384 x 4096 46.0 | 49.3, 8192 x 8192 45.2 | 57.8).  Joins the other way about (8192 x 4096 76 | 63)
+    if (alone) {
+      if (vectors <= 128) return go(ic<2>{}, ic<1>{}, whole, 64);
+      if (vectors <= 256) return go(ic<2>{}, ic<2>{}, whole, 64);
+      if (vectors <= 512) return go(ic<2>{}, ic<4>{}, whole, 64);
+      if (vectors <= 1024) return go(ic<2>{}, ic<8>{}, whole, 64);
+    } else {
+      if (vectors <= 128) return go(ic<1>{}, ic<2>{}, ahead, 64);
+      if (vectors <= 256) return go(ic<1>{}, ic<4>{}, ahead, 64);
+      if (vectors <= 512) return go(ic<1>{}, ic<8>{}, ahead, 64);
+      if (vectors <= 1024) return go(ic<1>{}, ic<16>{}, ahead, 64);
+    }
+    if (vectors <= 2048) return go(ic<2>{}, ic<16>{}, whole, 64);
     return in_launches(a.rows, [&](long long first, unsigned blocks) -> int {
       hipLaunchKernelGGL((join_long_kernel<T>), dim3(blocks), dim3(kLong), 0, as_stream(stream), a, first);
       WC_CHECK_LAUNCH("join_long_kernel");
