@@ -56,7 +56,7 @@ int unpack4(const unsigned char* codes, const unsigned char* scales, void* x, lo
 // y = act(x wT + b + r), one operand or both in 4 bits; p's a (x as it is) and b are null where they are packed
 struct Operand4 { const unsigned char* codes; const unsigned char* scales; };
 // linear4_few.hip: few rows of x, a pass over w
-constexpr int kMostFew4 = 64;
+constexpr int kMostFew4 = 16;
 int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, int dtype, void* stream);
 // linear4_dma.hip: both operands in 4 bits, on tiles.  Extents of p in channels, R padded
 ProductPlan product4_plan(const LinearProduct& p);
