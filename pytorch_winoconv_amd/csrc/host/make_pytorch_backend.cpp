@@ -883,6 +883,24 @@ py::object join_forward(const at::Tensor& f_, const MaybeTensor& x_, const Maybe
   return py::make_tuple(or_none(s), or_none(y), or_none(post_stats), or_none(pre_stats));
 }
 
+// y, or with keep (y, statistics)
+py::object norm_forward(const at::Tensor& x_, int kind, double eps, const MaybeTensor& w_, const MaybeTensor& b_, bool keep) {
+  const int64_t nd = x_.dim();
+  if (!linear_type(x_) || nd < 1 || x_.numel() == 0 || x_.size(nd - 1) > 1 << 24 || !norm_fits(w_, b_, x_, x_.size(nd - 1))) return py::none();
+  const c10::DeviceGuard guard(x_.device());
+  const at::Tensor x = x_.contiguous();
+  const MaybeTensor w = dense(w_), b = dense(b_), none;
+  const wc_join_desc d = join_desc(x, none, 1.0, 1.0, norm_of(0, 0.0, none, none, x), norm_of(kind, eps, w, b, x), 0, false, 0, 0, none);
+  at::Tensor y = at::empty(x.sizes(), x.options()), stats;
+  if (keep) stats = at::empty({d.rows, 2}, x.options().dtype(at::kFloat));
+  void* stream = stream_of(x);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_join_forward(&d, x.data_ptr(), nullptr, nullptr, nullptr, y.data_ptr(), nullptr, keep ? stats.data_ptr<float>() : nullptr, stream));
+  }
+  return keep ? py::object(py::make_tuple(y, stats)) : py::cast(y);
+}
+
 // operands that the Python layer has checked; rows > 0
 py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& gate_, const MaybeTensor& post_stats,
                         const MaybeTensor& pre_stats, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_, const MaybeTensor& post_b_, int pre_kind,
@@ -1456,6 +1474,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack4", &unpack4, py::arg("codes"), py::arg("scales"), py::arg("C"), py::arg("type"));
   m.def("linear4_forward", &linear4_forward, py::arg("x"), py::arg("x_codes"), py::arg("x_scales"), py::arg("type"), py::arg("w_codes"), py::arg("w_scales"),
         py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"));
+  m.def("norm_forward", &norm_forward);
   m.def("join_forward", &join_forward);
   m.def("join_backward", &join_backward);
   m.def("version", []() { return std::string(wc_version()); });

@@ -36,8 +36,12 @@ LinearProduct product_of(const wc_linear_desc* d, const void* x, const void* bia
   return {x, nullptr, d->C, padded4(d->C), false, false, d->rows, d->K, d->C, {bias, res, y, nullptr, d->activation, d->residual_after != 0, 0}};
 }
 
-// Rows of x over which a pass over the packed weight takes the layer; above, the weight is widened first, or, x packed as well, tiles take it
-bool few(const wc_linear_desc* d) { return d->rows <= kMostFew4; }
+// A pass over the packed weight, whose workgroups read x anew for every 16 of its rows, up to 8 rows, and up to 16 over a weight of up to 2^25 values.  us, fp16, the pass | tiles:
+// 16 x 4096 -> 4096 7.6 | 10, 16 x 8192 -> 8192 23.8 | 20.2, 16 x 25088 -> 4096 33 | 26
+bool few(const wc_linear_desc* d) { return d->rows <= 8 || (d->rows <= 16 && (long long)d->C * d->K <= 1ll << 25); }
+// Tiles that widen the codes in the registers, up to 2048 rows; above, and for fp32 and rows of x that are no whole 16 bytes, the weight is widened first, a launch and
+// a pass over it, for the product of its own type.  us, fp16 8192 -> 8192, tiles | widened first: 64 rows 23 | 64, 1024 128 | 182, 2048 247 | 270, 4096 509 | 499
+bool wide(const wc_linear_desc* d) { return d->rows <= kMostWide4 && linear4_wide_fits(nullptr, d->C, d->dtype); }
 
 // the product of two packed operands, its reduction padded
 LinearProduct tiled(LinearProduct p) {
@@ -87,6 +91,12 @@ int wc_linear4_workspace_bytes(const wc_linear_desc* d, int x_packed, size_t* by
     *bytes = s > 1 ? rounded((size_t)s * d->rows * d->K * 4) : 0;
     return WC_OK;
   }
+  if (wide(d)) {
+    const LinearProduct p = product_of(d, nullptr, nullptr, nullptr, nullptr);
+    const int s = linear4_wide_plan(p).s;
+    *bytes = s > 1 ? rounded((size_t)s * d->rows * d->K * 4) : 0;
+    return WC_OK;
+  }
   size_t inner = 0;
   if (int rc = wc_linear_workspace_bytes(d, &inner)) return rc;
   *bytes = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2)) + inner;
@@ -120,10 +130,19 @@ int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4*
     const LinearJoin join = {t.e, parts, plan.s, t.M, t.N};
     return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
   }
+  if (wide(d)) {
+    const ProductPlan plan = linear4_wide_plan(p);
+    float* const parts = static_cast<float*>(workspace);
+    if (plan.s > 1 && (size_t)plan.s * p.M * p.N * 4 > need) return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: %d parts do not fit the workspace", plan.s);
+    WC_CHECK_ARG(linear4_wide_fits(x, d->C, d->dtype), "wc_linear4_forward: x must start at a multiple of 16 bytes");
+    if (int rc = linear4_wide(p, w, plan, parts, d->dtype, stream)) return rc;
+    const LinearJoin join = {p.e, parts, plan.s, p.M, p.N};
+    return linear_join(&join, 1, nullptr, nullptr, d->dtype, stream);
+  }
   char* const ws = static_cast<char*>(workspace);
-  const size_t wide = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2));
+  const size_t wide_bytes = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2));
   if (int rc = unpack4(w.codes, w.scales, ws, d->K, d->C, d->dtype, stream)) return rc;
-  return wc_linear_forward(d, x, ws, bias, residual, y, nullptr, ws + wide, need - wide, stream);
+  return wc_linear_forward(d, x, ws, bias, residual, y, nullptr, ws + wide_bytes, need - wide_bytes, stream);
 }
 
 }  // extern "C"

@@ -43,7 +43,7 @@ template <int WM_, int WN_, int NWM_, int NWN_> struct Shape4 {
 constexpr int kBand4 = 8;
 
 template <typename T, typename SH>
-__global__ __launch_bounds__(64 * SH::NW, 2) void product4_dma_kernel(Dma4Args g) {
+__global__ __launch_bounds__(64 * SH::NW, SH::WM * SH::WN == 16 ? 1 : 2) void product4_dma_kernel(Dma4Args g) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   constexpr int WM = SH::WM, WN = SH::WN, NWM = SH::NWM, NWN = SH::NWN, BM = SH::BM, BN = SH::BN, NW = SH::NW;
   using E = half_t;           // what an element of 16 bits is called
@@ -112,29 +112,33 @@ __global__ __launch_bounds__(64 * SH::NW, 2) void product4_dma_kernel(Dma4Args g
     for (int j = 0; j < WN; ++j) fb[kk][j] = A::BYTES + B::offset(wn * WN + j, kk, lane);
   }
   const int ga = SH::CODES + (wm * WM * 32 + l32) * 4, gb = SH::CODES + BM * 4 + (wn * WN * 32 + l32) * 4;
+  // The halves of a pair's stages, 64 channels each: while one is multiplied the next is read, and with it, stage by stage, the scales
   s16x8 va[2][WM], vb[2][WN];
-  unsigned sa[WM], sb[WN];
-  auto step = [&](const unsigned char* st, bool more, int half) {
+  unsigned sa[2][WM], sb[2][WN];
+  auto read = [&](const unsigned char* st, int kk) {
+    if (kk == 0) {
 #pragma unroll
-    for (int i = 0; i < WM; ++i) sa[i] = *reinterpret_cast<const unsigned*>(st + ga + i * 128) >> (8 * lhi);
+      for (int i = 0; i < WM; ++i) sa[0][i] = *reinterpret_cast<const unsigned*>(st + ga + i * 128) >> (8 * lhi);
 #pragma unroll
-    for (int j = 0; j < WN; ++j) sb[j] = *reinterpret_cast<const unsigned*>(st + gb + j * 128) >> (8 * lhi);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-      for (int i = 0; i < WM; ++i) va[kk][i] = A::read(st + fa[kk][i]);
-#pragma unroll
-      for (int j = 0; j < WN; ++j) vb[kk][j] = B::read(st + fb[kk][j]);
+      for (int j = 0; j < WN; ++j) sb[0][j] = *reinterpret_cast<const unsigned*>(st + gb + j * 128) >> (8 * lhi);
     }
-    if (more) queue_pair(half);
+#pragma unroll
+    for (int i = 0; i < WM; ++i) va[kk][i] = A::read(st + fa[kk][i]);
+#pragma unroll
+    for (int j = 0; j < WN; ++j) vb[kk][j] = B::read(st + fb[kk][j]);
+  };
+  auto keep_scales = [&] {
+#pragma unroll
+    for (int i = 0; i < WM; ++i) sa[1][i] = sa[0][i];
+#pragma unroll
+    for (int j = 0; j < WN; ++j) sb[1][j] = sb[0][j];
+  };
+  auto multiply = [&](auto half) {
+    constexpr int H = decltype(half)::value;
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
-      for (int j = 0; j < WN; ++j) acc[i][j] = product4<0>(vb[0][j], va[0][i], acc[i][j], sb[j], sa[i]);
-#pragma unroll
-    for (int i = 0; i < WM; ++i)
-#pragma unroll
-      for (int j = 0; j < WN; ++j) acc[i][j] = product4<1>(vb[1][j], va[1][i], acc[i][j], sb[j], sa[i]);
+      for (int j = 0; j < WN; ++j) acc[i][j] = product4<H>(vb[H][j], va[H][i], acc[i][j], sb[H][j], sa[H][i]);
   };
 
   const int pairs = (nk + 1) / 2;
@@ -144,8 +148,19 @@ __global__ __launch_bounds__(64 * SH::NW, 2) void product4_dma_kernel(Dma4Args g
     // pair j has landed, and nobody reads pair j - 1 any more, which pair j + 1 overwrites
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const unsigned char* const st = lds + (j & 1) * 2 * SH::STAGE;
-    step(st, j + 1 < pairs, (j + 1) & 1);
-    if (2 * j + 1 < nk) step(st + SH::STAGE, false, 0);
+    read(st, 0);
+    keep_scales();
+    read(st, 1);
+    if (j + 1 < pairs) queue_pair((j + 1) & 1);
+    multiply(ic<0>{});
+    if (2 * j + 1 < nk) {
+      read(st + SH::STAGE, 0);
+      multiply(ic<1>{});
+      keep_scales();
+      read(st + SH::STAGE, 1);
+      multiply(ic<0>{});
+    }
+    multiply(ic<1>{});
   }
 
   const long long wm0 = m0 + wm * WM * 32, wn0 = n0 + wn * WN * 32;

@@ -12,6 +12,24 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c, half_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// (the lanes of either half hold four neighbouring reduction elements, and an fp32 instruction takes one of each half)
+__device__ __forceinline__ f32x16 product(s16x8 a, s16x8 b, f32x16 c, float) {
+  const f32x4 p = __builtin_bit_cast(f32x4, a), q = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_32x32x2f32(p[k], q[k], c, 0, 0, 0);
+  return c;
+}
+
 // reduction elements of a stage, and of a 16-byte chunk
 template <typename T> constexpr int kDeep = 64 / sizeof(T);
 template <typename T> constexpr int kChunk = 16 / sizeof(T);

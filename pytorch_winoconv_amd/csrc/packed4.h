@@ -55,9 +55,13 @@ int unpack4(const unsigned char* codes, const unsigned char* scales, void* x, lo
 
 // y = act(x wT + b + r), one operand or both in 4 bits; p's a (x as it is) and b are null where they are packed
 struct Operand4 { const unsigned char* codes; const unsigned char* scales; };
-// linear4_few.hip: few rows of x, a pass over w
-constexpr int kMostFew4 = 16;
+// linear4_few.hip: at most 16 rows of x, a pass over w
 int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, int dtype, void* stream);
+// linear4_wide.hip: more rows of 16-bit x (rows of whole 16 bytes), w's codes widened in the registers.  R_part of its plan is in stages
+constexpr int kMostWide4 = 2048;
+bool linear4_wide_fits(const void* x, long long C, int dtype);
+ProductPlan linear4_wide_plan(const LinearProduct& p);
+int linear4_wide(const LinearProduct& p, const Operand4& w, const ProductPlan& plan, float* parts, int dtype, void* stream);
 // linear4_dma.hip: both operands in 4 bits, on tiles.  Extents of p in channels, R padded
 ProductPlan product4_plan(const LinearProduct& p);
 int product4_dma(const LinearProduct& p, const Operand4& x, const Operand4& w, const ProductPlan& plan, float* parts, int dtype, void* stream);

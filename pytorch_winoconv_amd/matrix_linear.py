@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
 from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
-from .packed4 import Packed4, _made as _made4, linear4_forward, pack4, unpack4
+from .packed4 import Packed4, _made as _made4, linear4_ext, linear4_forward, pack4, unpack4
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -103,6 +103,10 @@ def _linear4(x, w, bias, residual, activation, residual_after, keep_z):
     """linear_forward over a Packed4 w."""
     if not isinstance(w, Packed4):
         raise TypeError("linear_forward: x in 4 bits takes a weight in 4 bits, got a tensor")
+    if not keep_z:
+        y = linear4_ext(x, w, bias, residual, ACTIVATIONS[activation], residual_after)
+        if y is not None:
+            return y
     _check_weight(x.shape, w, "x")
     K = w.shape[0]
     shape = tuple(x.shape[:-1]) + (K,)

@@ -139,16 +139,23 @@ def unpack4(packed, dtype=None):
     return x
 
 
+def linear4_ext(x, w, bias, residual, activation, residual_after):
+    """linear4_forward by the compiled host layer, which takes operands that fit together; None for others."""
+    if not engine.USE_EXT or not w.codes.is_cuda or w.codes.dim() != 2:
+        return None
+    if not isinstance(x, Packed4):
+        return engine._ext.linear4_forward(x, None, None, None, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after))
+    if x.channels != w.channels:
+        return None
+    return engine._ext.linear4_forward(None, x.codes, x.scales, x.dtype, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after))
+
+
 def linear4_forward(x, w, bias, residual, activation, residual_after):
     """matrix_linear.linear_forward without z for w a Packed4 (K, C) and x a tensor (..., C) or a Packed4; activation is its number."""
-    packed = isinstance(x, Packed4)
-    C = w.channels
-    if engine.USE_EXT and w.codes.is_cuda:
-        given = (None, x.codes, x.scales) if packed else (x, None, None)
-        if not packed or x.channels == C:
-            y = engine._ext.linear4_forward(*given, x.dtype, w.codes, w.scales, C, bias, residual, activation, bool(residual_after))
-            if y is not None:
-                return y
+    y = linear4_ext(x, w, bias, residual, activation, residual_after)
+    if y is not None:
+        return y
+    packed, C = isinstance(x, Packed4), w.channels
     K, shape, dtype = w.codes.shape[0], tuple(x.shape[:-1]) + (w.codes.shape[0],), x.dtype
     if packed:
         if not x.codes.is_cuda:

@@ -250,6 +250,10 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
 
 def norm_forward(x, norm, keep=False):
     """norm(x) for x (..., C); with keep (y, stats), stats for norm_backward."""
+    if engine.USE_EXT:
+        out = engine._ext.norm_forward(x, KINDS[norm.kind], norm.eps, norm.weight, norm.bias, keep)
+        if out is not None:
+            return out
     _, y, stats = _forward(x, None, None, None, norm, None, 1.0, 1.0, False, bool(keep))
     return (y, stats[1]) if keep else y
 

@@ -69,10 +69,11 @@ def test_borders_and_extremes(dev, t):
     assert _same(packed4.unpack4(p).cpu(), po.values(codes, scales, 64).to(t))
 
 
-# rows, C, K: passes over w (up to 64 rows) of four, eight and sixteen rows of w a workgroup, several stages a place, and beyond
+# rows, C, K: passes over w (up to 16 rows) of four, eight and sixteen rows of w a workgroup, several stages a place; tiles, whole and not, in parts; beyond them
 SHAPES = [(1, 1, 1), (1, 128, 4), (1, 4096, 40), (2, 31, 65), (4, 4104, 1001), (5, 2056, 24), (8, 64, 64), (8, 136, 2100), (9, 1032, 333), (16, 520, 40), (17, 300, 128),
           (33, 257, 72), (48, 1000, 31), (64, 64, 64), (65, 33, 17), (130, 257, 96), (200, 72, 264), (257, 136, 520), (1025, 8, 8), (300, 300, 301), (600, 501, 403),
-          (513, 1152, 300), (1000, 520, 776)]
+          (513, 1152, 300), (1000, 520, 776),
+          (12, 8200, 4104), (70, 1096, 700), (128, 8192, 136), (2050, 136, 72)]
 
 
 @pytest.mark.parametrize("t", lo.TYPES, ids=str)
