@@ -16,10 +16,15 @@ int check_extents4(long long rows, int C, int dtype, const char* who) {
   return WC_OK;
 }
 
+// (codes are read and written by words and 16 bytes)
+int check_starts(const unsigned char* codes, const unsigned char* scales, const char* who) {
+  WC_CHECK_ARG(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0, "%s: codes and scales must start at multiples of 16 bytes", who);
+  return WC_OK;
+}
+
 int check_packed(const wc_packed4* t, const char* what, const char* who) {
   WC_CHECK_ARG(t && t->codes && t->scales, "%s: %s is null", who, what);
-  WC_CHECK_ARG(reinterpret_cast<uintptr_t>(t->codes) % 16 == 0 && reinterpret_cast<uintptr_t>(t->scales) % 16 == 0, "%s: %s must start at multiples of 16 bytes", who, what);
-  return WC_OK;
+  return check_starts(t->codes, t->scales, who);
 }
 
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
@@ -65,6 +70,7 @@ int wc_pack4(const void* x, unsigned char* codes, unsigned char* scales, long lo
   if (int rc = check_extents4(rows, C, dtype, "wc_pack4")) return rc;
   if (rows == 0) return WC_OK;
   WC_CHECK_ARG(x && codes && scales, "wc_pack4: null pointer");
+  if (int rc = check_starts(codes, scales, "wc_pack4")) return rc;
   return pack4(x, codes, scales, rows, C, dtype, stream);
 }
 
@@ -72,6 +78,7 @@ int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x,
   if (int rc = check_extents4(rows, C, dtype, "wc_unpack4")) return rc;
   if (rows == 0) return WC_OK;
   WC_CHECK_ARG(x && codes && scales, "wc_unpack4: null pointer");
+  if (int rc = check_starts(codes, scales, "wc_unpack4")) return rc;
   return unpack4(codes, scales, x, rows, C, dtype, stream);
 }
 

@@ -29,6 +29,12 @@ int check_desc(const wc_join_desc* d, const char* who) {
   return check_norm(d->pre, d->dtype, "pre", who);
 }
 
+// (a row's two are one access)
+int check_stats(const void* a, const void* b, const char* who) {
+  WC_CHECK_ARG(reinterpret_cast<uintptr_t>(a) % 8 == 0 && reinterpret_cast<uintptr_t>(b) % 8 == 0, "%s: statistics must start at multiples of 8 bytes", who);
+  return WC_OK;
+}
+
 Norm norm_of(const wc_norm& n) { return {n.kind, n.eps, n.weight, n.bias, n.dtype == WC_F32}; }
 Dropout drop_of(const wc_join_desc* d) {
   return {(unsigned)d->drop_level, d->drop_per_sample != 0, d->drop_level == 0 ? 1.f : d->drop_level == 65536 ? 0.f : 65536.f / (float)(65536 - d->drop_level), d->drop_seed,
@@ -80,6 +86,7 @@ int wc_join_forward(const wc_join_desc* d, const void* f, const void* x, const v
   if (d->rows == 0) return WC_OK;
   WC_CHECK_ARG(f && (s || y), "wc_join_forward: null pointer");
   WC_CHECK_ARG(!d->gate_rows == !gate, "wc_join_forward: a gate and its rows go together");
+  if (int rc = check_stats(post_stats, pre_stats, "wc_join_forward")) return rc;
   JoinArgs a = {d->rows, d->rows / d->samples, d->C, f, x, gate, gate_of(d), d->gate_dtype == WC_F32, d->stream_scale, d->block_scale, norm_of(d->post), norm_of(d->pre),
                 drop_of(d), s, y, post_stats, pre_stats};
   if (!y) a.pre.kind = WC_NORM_NONE;
@@ -106,6 +113,7 @@ int wc_join_backward(const wc_join_desc* d, const wc_join_gradients* q, void* wo
   WC_CHECK_ARG(!q->dgate || q->gate, "wc_join_backward: the gradient of a gate that is not there");
   WC_CHECK_ARG(!post || q->post_stats, "wc_join_backward: post's gradient needs its statistics");
   WC_CHECK_ARG((!post && !q->dgate) || q->f, "wc_join_backward: post's gradient and the gate's need f");
+  if (int rc = check_stats(q->post_stats, q->pre_stats, "wc_join_backward")) return rc;
   if (need && (!workspace || workspace_bytes < need))
     return fail(WC_ERR_WORKSPACE, "wc_join_backward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   if (need && reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(WC_ERR_WORKSPACE, "wc_join_backward: workspace must be 256-byte aligned");

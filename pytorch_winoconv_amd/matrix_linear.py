@@ -309,7 +309,8 @@ class MatrixLinear(nn.Module):
 
 class MatrixLinear4(nn.Module):
     """A linear layer whose weight is frozen, in 4 bits (MatrixLinear.pack4, or of a Packed4 w (out_features, in_features)): 1/2 + 1/32 bytes a
-    weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales`; the bias is a parameter."""
+    weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales`; the bias is a parameter, which with x4 does not
+    learn either."""
 
     def __init__(self, weight, bias=None, activation="none", residual_after=False, channel_axis=-1, x4=False):
         super().__init__()
@@ -324,7 +325,7 @@ class MatrixLinear4(nn.Module):
         self.dtype = w4.dtype
         self.register_buffer("codes", w4.codes)
         self.register_buffer("scales", w4.scales)
-        self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=bias.requires_grad)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=bias.requires_grad and not x4)
 
     @property
     def weight(self):
@@ -332,7 +333,7 @@ class MatrixLinear4(nn.Module):
         return Packed4(self.codes, self.scales, self.in_features, self.dtype)
 
     def forward(self, x, residual=None):
-        w = self.weight
+        w = _made4(self.codes, self.scales, self.in_features, self.dtype)
         if not self.x4:
             return linear(x, w, self.bias, residual, self.activation, self.residual_after, None, self.channel_axis)
         if torch.is_grad_enabled() and x.requires_grad:

@@ -14,11 +14,11 @@ def least(t):
     return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
 
 
-def words(rows, C, seed, offset):
-    """The eight 16-bit words of Philox4x32-10 for every eight channels, (rows, 8 ceil(C / 8)), in Python's whole numbers by numpy's unsigned ones."""
+def words(rows, C, seed, offset, first=0):
+    """Of rows `first` and on, the eight 16-bit words of Philox4x32-10 for every eight channels, (rows, 8 ceil(C / 8)), in Python's whole numbers by numpy's unsigned ones."""
     width = -(-C // 8)
     low, half = np.uint64(0xFFFFFFFF), np.uint64(32)
-    x = [np.tile(np.arange(width, dtype=np.uint64), rows), np.repeat(np.arange(rows, dtype=np.uint64), width), np.full(rows * width, offset & 0xFFFFFFFF, dtype=np.uint64),
+    x = [np.tile(np.arange(width, dtype=np.uint64), rows), np.repeat(np.arange(first, first + rows, dtype=np.uint64), width), np.full(rows * width, offset & 0xFFFFFFFF, dtype=np.uint64),
          np.full(rows * width, offset >> 32, dtype=np.uint64)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
     for _ in range(10):

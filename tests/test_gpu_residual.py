@@ -305,8 +305,11 @@ def test_stack_against_torch(dev):
         assert all(isinstance(layer, pkg.MatrixLinear4) for b in stack.blocks for layer in b)
         y = stack(x.cuda())
         assert float((y.detach().cpu().double() - reference()).norm() / reference().norm()) < 1e-5
+        # inputs in 4 bits too: serving, no gradient
+        stack = pkg.ResidualStack([residual.matrix_block(40, 64) for _ in range(2)], 40, kind, gate=0.7).cuda().eval().pack4(True)
         with torch.no_grad():
-            assert stack.pack4(True)(x.cuda()).shape == x.shape
+            y = stack(x.cuda())
+        assert y.shape == x.shape and bool(torch.isfinite(y).all()) and all(layer.x4 for b in stack.blocks for layer in b)
 
 
 def test_gradients_by_differences(dev):
@@ -372,3 +375,49 @@ def test_stream_and_two_at_once(dev):
     for w, g in zip(want, got):
         for once in g:
             assert all(torch.equal(a, b) for a, b in zip(w, once))
+
+
+def test_beyond_32_bits(dev):
+    """More than 2^31 elements: the last rows are those of a call of their own, and their mask is theirs."""
+    rows, C = 300000, 8200
+    f = torch.empty(rows, C, dtype=torch.bfloat16, device="cuda").normal_()
+    n = Norm("layer", torch.randn(C).cuda(), torch.randn(C).cuda())
+    y, stats = residual.norm_forward(f, n, keep=True)
+    assert f.numel() > 1 << 31 and torch.equal(y[-5:], residual.norm_forward(f[-5:], n))
+    dx, dw, db = residual.norm_backward(y, f, stats, n)
+    assert torch.equal(dx[-5:], residual.norm_backward(y[-5:], f[-5:], stats[-5:].clone(), n)[0])
+    assert bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())
+    del dx
+    s = residual.join_forward(f, y, drop=Drop(0.3, 11, 12))[0]
+    kept = (ro.words(5, C, 11, 12, rows - 5)[:, :C] >= int(round(0.3 * 65536))).cuda()
+    scale = 65536 / (65536 - int(round(0.3 * 65536)))
+    want = y[-5:].float() + torch.where(kept, f[-5:].float() * scale, torch.zeros((), device="cuda"))
+    assert float((s[-5:].float() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("C", [40, 1000, 2056])
+def test_many_samples(dev, C):
+    """More samples than workgroups, of few rows each: the sums behind a sample's gate."""
+    for t in (torch.float32, torch.bfloat16):
+        f, x, po, pr, gt, ds, dy = _inputs((1500, 3, C), t, C, "layer", "rms", "sample")
+        how = dict(post=_cuda(po), gate=_cuda(gt), pre=_cuda(pr), drop=Drop(0.2, 1, 2, "sample"))
+        s, y, stats = residual.join_forward(f.cuda(), x.cuda(), keep=True, **how)
+        want = ro.forward(f, x, gt, po, pr, (0.2, 1, 2, "sample"), 1.0, 1.0)
+        ro.within(s, want[0], want[2], "s")
+        wanted = ro.backward(ds, dy, f, s.cpu(), gt, po, pr, (0.2, 1, 2, "sample"), 1.0, 1.0, want[0])
+        got = residual.join_backward(ds.cuda(), dy.cuda(), f.cuda(), s, stats, **how)._asdict()
+        for k, (v, bound) in wanted.items():
+            ro.within(got[k], v, bound, k)
+
+
+def test_same_bits_every_time(dev):
+    f, x, po, pr, gt, ds, dy = _inputs((4, 600, 520), torch.bfloat16, 1, "layer", "layer", "channel")
+    how = dict(post=_cuda(po), gate=_cuda(gt), pre=_cuda(pr), drop=Drop(0.2, 1, 2))
+    args = [v.cuda() for v in (f, x, ds, dy)]
+
+    def step():
+        s, y, stats = residual.join_forward(args[0], args[1], keep=True, **how)
+        return (s, y) + tuple(residual.join_backward(args[2], args[3], args[0], s, stats, **how))
+    first = step()
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))

@@ -105,6 +105,8 @@ def test_c_entry_points_refuse():
     assert lib.wc_pack4(None, None, None, 0, 4, 0, None) == 0
     assert lib.wc_pack4(None, None, None, 1, 4, 0, None) == _lib.WC_ERR_BAD_ARG
     assert lib.wc_unpack4(None, None, None, 1, 4, 7, None) == _lib.WC_ERR_BAD_ARG
+    assert lib.wc_pack4(256, 8, 256, 1, 4, 0, None) == _lib.WC_ERR_BAD_ARG
+    assert lib.wc_unpack4(256, 24, 256, 1, 4, 0, None) == _lib.WC_ERR_BAD_ARG
     d = _lib.LinearDesc(3000, 256, 64, _lib.WC_F16, 0, 0)
     n = ctypes.c_size_t()
     assert lib.wc_linear4_workspace_bytes(ctypes.byref(d), 0, ctypes.byref(n)) == 0 and n.value >= 64 * 256 * 2

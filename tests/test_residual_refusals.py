@@ -152,6 +152,7 @@ def test_c_entry_points_refuse():
     assert forward(desc(), y=at) == _lib.WC_ERR_BAD_ARG
     assert forward(desc(gate_rows=3)) == _lib.WC_ERR_BAD_ARG
     assert forward(desc(), gate=at) == _lib.WC_ERR_BAD_ARG
+    assert lib.wc_join_forward(desc(pre=rms), at, None, None, at, at, None, 260, None) == _lib.WC_ERR_BAD_ARG
     n = ctypes.c_size_t()
 
     def backward(d, ws=None, size=0, **given):
@@ -166,6 +167,7 @@ def test_c_entry_points_refuse():
     assert backward(desc(), ds=256, df=256, dpost_weight=256) == _lib.WC_ERR_BAD_ARG
     assert backward(desc(), ds=256, df=256, dpre_bias=256) == _lib.WC_ERR_BAD_ARG
     assert backward(desc(gate_rows=3), ds=256, df=256) == _lib.WC_ERR_BAD_ARG
+    assert backward(desc(post=rms), ds=256, df=256, f=256, post_stats=260) == _lib.WC_ERR_BAD_ARG
     q = _lib.JoinGradients(dy=256, s=256, pre_stats=256, df=256, dpre_weight=256)
     assert lib.wc_join_backward_workspace_bytes(desc(pre=rms), ctypes.byref(q), ctypes.byref(n)) == 0 and n.value > 0
     assert lib.wc_join_backward(desc(pre=rms), ctypes.byref(q), None, 0, None) == _lib.WC_ERR_WORKSPACE
