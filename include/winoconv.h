@@ -457,12 +457,13 @@ typedef struct {
 int wc_join_forward(const wc_join_desc* desc, const void* f, const void* x, const void* gate, void* s, void* y, float* post_stats, float* pre_stats,
                     void* stream);
 
-/* Its gradients.  ds, dy: of s and y, one of them may be null.  f is wanted by post and the gate's gradient, s by pre (as it was rounded).  Results that are null
+/* Its gradients.  ds, dy: of s and y, one of them may be null.  f is wanted by post and the gate's gradient.  pre wants s, but of 16-bit types, if f
+ * is there, f and x (null: no stream), from which s is computed again as it was before its rounding.  Results that are null
  * are not computed; those of parameters and gate come in their types.  Sums fp32 in a fixed order.  rows > 0.  Workspace 256-byte aligned; its size goes
  * by which pointers are null. */
 typedef struct {
   const void* ds; const void* dy;
-  const void* f; const void* s; const void* gate;
+  const void* f; const void* s; const void* x; const void* gate;
   const float* post_stats; const float* pre_stats;
   void* df; void* dx;
   void* dpre_weight; void* dpre_bias; void* dpost_weight; void* dpost_bias; void* dgate;

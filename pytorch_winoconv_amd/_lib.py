@@ -65,7 +65,7 @@ class JoinDesc(ctypes.Structure):
 
 
 class JoinGradients(ctypes.Structure):
-    _fields_ = [(name, ctypes.c_void_p) for name in ("ds", "dy", "f", "s", "gate", "post_stats", "pre_stats", "df", "dx", "dpre_weight", "dpre_bias",
+    _fields_ = [(name, ctypes.c_void_p) for name in ("ds", "dy", "f", "s", "x", "gate", "post_stats", "pre_stats", "df", "dx", "dpre_weight", "dpre_bias",
                                                      "dpost_weight", "dpost_bias", "dgate")]
 
 

@@ -902,13 +902,13 @@ py::object norm_forward(const at::Tensor& x_, int kind, double eps, const MaybeT
 }
 
 // operands that the Python layer has checked; rows > 0
-py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& gate_, const MaybeTensor& post_stats,
+py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& x_, const MaybeTensor& gate_, const MaybeTensor& post_stats,
                         const MaybeTensor& pre_stats, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_, const MaybeTensor& post_b_, int pre_kind,
                         double pre_eps, const MaybeTensor& pre_w_, const MaybeTensor& pre_b_, int level, bool per_sample, uint64_t seed, uint64_t offset,
                         const MaybeTensor& state, bool need_f, bool need_x, bool need_gate, bool need_post, bool need_pre) {
   const at::Tensor& like = ds_ ? *ds_ : *dy_;
   const c10::DeviceGuard guard(like.device());
-  const MaybeTensor ds = dense(ds_), dy = dense(dy_), f = dense(f_), s = dense(s_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_),
+  const MaybeTensor ds = dense(ds_), dy = dense(dy_), f = dense(f_), s = dense(s_), x = dense(x_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_),
                     pre_b = dense(pre_b_);
   const wc_join_desc d = join_desc(like, gate, a, b, norm_of(post_kind, post_eps, post_w, post_b, like), norm_of(pre_kind, pre_eps, pre_w, pre_b, like), level, per_sample, seed, offset,
                                    state);
@@ -923,7 +923,7 @@ py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const Ma
   if (need_pre && pre_b) dpre_b = fresh(*pre_b);
   auto at_or_null = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   auto stats = [](const MaybeTensor& t) { return t ? t->data_ptr<float>() : nullptr; };
-  const wc_join_gradients q = {data_or_null(ds), data_or_null(dy), data_or_null(f), data_or_null(s), data_or_null(gate), stats(post_stats), stats(pre_stats), at_or_null(df),
+  const wc_join_gradients q = {data_or_null(ds), data_or_null(dy), data_or_null(f), data_or_null(s), data_or_null(x), data_or_null(gate), stats(post_stats), stats(pre_stats), at_or_null(df),
                                at_or_null(dx), at_or_null(dpre_w), at_or_null(dpre_b), at_or_null(dpost_w), at_or_null(dpost_b), at_or_null(dgate)};
   size_t bytes = 0;
   check(wc_join_backward_workspace_bytes(&d, &q, &bytes));

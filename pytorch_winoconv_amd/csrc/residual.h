@@ -40,7 +40,7 @@ struct JoinGradients {
   long long rows, per;
   int C;
   const void* ds; const void* dy;          // null: none
-  const void* f; const void* s; const void* gate;
+  const void* f; const void* s; const void* x; const void* gate;      // pre's s null: computed again from f and x (null: there is no stream)
   int gate_rows, gate_wide;
   float a, b;
   Norm post, pre;

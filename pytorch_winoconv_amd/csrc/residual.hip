@@ -56,9 +56,10 @@ struct Backward {
 Backward backward_plan(const wc_join_desc* d, const wc_join_gradients* q, char* ws) {
   Backward b = {};
   JoinGradients& g = b.g;
-  g = {d->rows, d->rows / d->samples, d->C, q->ds, q->dy, q->f, q->s, q->gate, gate_of(d), d->gate_dtype == WC_F32, d->stream_scale, d->block_scale, norm_of(d->post),
+  g = {d->rows, d->rows / d->samples, d->C, q->ds, q->dy, q->f, q->s, q->x, q->gate, gate_of(d), d->gate_dtype == WC_F32, d->stream_scale, d->block_scale, norm_of(d->post),
        norm_of(d->pre), drop_of(d), q->post_stats, q->pre_stats, q->df, q->dx, nullptr, {}, 1, 1, 1};
   if (!q->dy) g.pre.kind = WC_NORM_NONE;
+  if (d->dtype != WC_F32 && g.f) g.s = nullptr;
   if (g.gate_rows == kGateRow) g.dgate_rows = q->dgate;
   void* const to[5] = {q->dpre_weight, q->dpre_bias, q->dpost_weight, q->dpost_bias, g.dgate_rows ? nullptr : q->dgate};
   join_plan(&g);
@@ -106,7 +107,7 @@ int wc_join_backward(const wc_join_desc* d, const wc_join_gradients* q, void* wo
   WC_CHECK_ARG(d->rows > 0, "wc_join_backward: no rows (the gradients of the parameters are zero)");
   const bool pre = d->pre.kind != WC_NORM_NONE && q->dy, post = d->post.kind != WC_NORM_NONE;
   WC_CHECK_ARG(q->ds || pre, "wc_join_backward: neither ds nor dy with its norm");
-  WC_CHECK_ARG(!pre || (q->s && q->pre_stats), "wc_join_backward: pre's gradient needs s and its statistics");
+  WC_CHECK_ARG(!pre || ((q->s || (q->f && d->dtype != WC_F32)) && q->pre_stats), "wc_join_backward: pre's gradient needs s, or in 16-bit types f, and its statistics");
   WC_CHECK_ARG(!d->gate_rows == !q->gate, "wc_join_backward: a gate and its rows go together");
   WC_CHECK_ARG((!q->dpre_weight && !q->dpre_bias) || pre, "wc_join_backward: gradients of a norm that is not there");
   WC_CHECK_ARG((!q->dpost_weight && !q->dpost_bias) || post, "wc_join_backward: gradients of a norm that is not there");

@@ -28,7 +28,7 @@ void join_plan(JoinGradients* g) {
   const long long length = g->segments > 1 ? g->per : g->rows;
   // Workgroups: what the compute units hold at once (kMinWaves: more would wait for their turn and leave more parts; us, 16384 x 2048 bf16, two norms, gate and
   // dropout, at 8 | 12 | 16 wavefronts a compute unit 135 | 171 | 138, without post and gate 82 | 79 | 74), with two rows a team where there are so many
-  const int held = g->post.kind || g->gate_rows == kGateRow ? 8 : g->pre.kind && g->gate_rows ? 12 : 16;
+  const int held = g->post.kind || g->gate_rows == kGateRow ? 8 : g->pre.kind && (g->gate_rows || !g->s) ? 12 : 16;
   const long long most = kCus * std::max(1, t.vectors == 0 ? 1 : held / (t.waves == 1 ? 4 : t.waves));
   const long long wanted = std::max(1ll, std::min(most, ceil_div_ll(g->rows, 2 * teams)));
   g->parts = (int)std::max(1ll, std::min(wanted / g->segments, ceil_div_ll(length, teams)));

@@ -5,8 +5,9 @@
 f is what a block gave, x the stream, post the norm behind the block, pre the norm before the next one; all but f may be missing, so that a
 norm alone and dropout alone are the same kernels.  Norms are over the channels (the last axis): "rms", v w / sqrt(mean(v^2) + eps), and
 "layer", (v - mean) w / sqrt(var + eps) + bias.  gate is one value a channel, (C,), or one a sample and channel, (N, C), where the samples are the first
-axis of f.  Arithmetic and sums are fp32, s and y are rounded once (y is of s before that, its gradient of s as it was rounded).  float32, float16 and
-bfloat16; parameters and gate of that type or float32.  The GPU only.
+axis of f.  Arithmetic and sums are fp32, s and y are rounded once (y is of s before that).  float32, float16 and
+bfloat16; parameters and gate of that type or float32.  The GPU only.  In 16-bit types the backward pass computes s again from f and x, since a norm's
+gradient from the rounded s is 1.4 times as far from the exact one.
 
 Dropout draws its mask from a counter-based generator, Philox4x32-10, by seed, offset, row and channel, and draws it again for the backward pass: nothing
 of it is stored, and the same numbers give the same mask whatever the strides, the launch or the type.  Each channel has 16 bits: the
@@ -190,14 +191,20 @@ def join_forward(block, stream=None, post=None, gate=None, pre=None, drop=None, 
     """(s, y, stats) for block = f (..., C) and stream = x of its shape, post and pre Norms, drop a Drop; y is None without pre.  stats is what join_backward
     wants, where keep is true."""
     s, y, stats = _forward(block, stream, post, gate, pre, drop, stream_scale, block_scale, True, bool(keep))
-    return s, y, stats if keep else None
+    return s, y, stats + ((stream,) if _again(block, pre) else ()) if keep else None
+
+
+def _again(block, pre):
+    """Whether the backward pass computes s again, unrounded, from block and stream."""
+    return pre is not None and block.dtype != torch.float32
 
 
 def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=None, stream_scale=1.0, block_scale=1.0, need_block=True, need_stream=True,
                   need_gate=True, need_post=True, need_pre=True):
     """Gradients(block, stream, post_weight, post_bias, gate, pre_weight, pre_bias) of join_forward, None for those not asked for or of what is not there, each
     of the type of what it belongs to.  ds or dy may be None, for an s or y that went nowhere; block may be None where there is neither post nor a gate that
-    wants its gradient, s without pre."""
+    wants its gradient, s without pre, or where block is given.  stats of 16-bit types with pre hold the stream, as it must still be; s is then computed again, unless
+    block is None."""
     given = ds if ds is not None else dy
     if given is None:
         raise ValueError("join_backward: neither ds nor dy")
@@ -205,16 +212,18 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
         raise ValueError("join_backward: dy without pre, whose result y is")
     through = pre if dy is not None else None
     need_gate = need_gate and gate is not None
-    post_stats, pre_stats = stats if stats is not None else (None, None)
+    post_stats, pre_stats = stats[:2] if stats is not None else (None, None)
+    again = through is not None and block is not None and stats is not None and len(stats) > 2
+    x = stats[2] if again else None
     if (post is not None or need_gate) and block is None:
         raise ValueError("join_backward: the gradients of post and the gate need block")
-    if through is not None and s is None:
-        raise ValueError("join_backward: the gradient of pre needs s")
+    if through is not None and s is None and not again:
+        raise ValueError("join_backward: the gradient of pre needs s, or block and what join_forward kept")
     rows = _rows(given.shape)
     for n, t, what in ((post, post_stats, "post"), (through, pre_stats, "pre")):
         if n is not None and (t is None or t.dtype != torch.float32 or tuple(t.shape) != (rows, 2) or t.device != given.device or not t.is_contiguous()):
             raise ValueError("join_backward: the statistics of %s are those that join_forward kept, (%d, 2) in float32" % (what, rows))
-    _check_block(given, post, gate, pre, drop, {"ds": ds, "dy": dy, "block": block, "s": s})
+    _check_block(given, post, gate, pre, drop, {"ds": ds, "dy": dy, "block": block, "s": s, "the stream": x})
     like = lambda n, name, wanted: getattr(n, name) if wanted and n is not None else None  # noqa: E731
     want = [like(through, "weight", need_pre), like(through, "bias", need_pre), like(post, "weight", need_post), like(post, "bias", need_post), gate if need_gate else None]
     # (a norm that no gradient comes through has zeros)
@@ -229,17 +238,17 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
     if not (need_block or need_stream or any(t is not None for t in want)):
         return Gradients(None, None, None, None, None, zeros(silent[0]), zeros(silent[1]))
     if engine.USE_EXT:
-        df, dx, pw, pb, qw, qb, dg = engine._ext.join_backward(ds, dy, block if post is not None or need_gate else None, s if through is not None else None, gate,
-                                                               post_stats, pre_stats, float(stream_scale), float(block_scale), *_ext_norm(post), *_ext_norm(through),
+        df, dx, pw, pb, qw, qb, dg = engine._ext.join_backward(ds, dy, block if post is not None or need_gate or again else None,
+                                                               s if through is not None and not again else None, x, gate, post_stats, pre_stats, float(stream_scale), float(block_scale), *_ext_norm(post), *_ext_norm(through),
                                                                *_ext_drop(drop), need_block, need_stream, need_gate, need_post, need_pre)
     else:
-        ds, dy, block, s, g = (_plain(t) for t in (ds, dy, block, s, gate))
+        ds, dy, block, s, x, g = (_plain(t) for t in (ds, dy, block, s, x, gate))
         d, kept = _desc(given, post, g, through, drop, stream_scale, block_scale)
         df, dx = (dense(given) if wanted else None for wanted in (need_block, need_stream))
         pw, pb, qw, qb, dg = (None if t is None else dense(t) for t in want)
         at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        q = _lib.JoinGradients(*(at(t) for t in (ds, dy, block if post is not None or need_gate else None, s if through is not None else None, g, post_stats,
-                                                 pre_stats, df, dx, pw, pb, qw, qb, dg)))
+        q = _lib.JoinGradients(*(at(t) for t in (ds, dy, block if post is not None or need_gate or again else None,
+                                                 s if through is not None and not again else None, x, g, post_stats, pre_stats, df, dx, pw, pb, qw, qb, dg)))
         lib, nbytes = _lib.load(), ctypes.c_size_t()
         check(lib.wc_join_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(q), ctypes.byref(nbytes)))
         ws = torch.empty(nbytes.value, dtype=torch.uint8, device=given.device)
@@ -290,17 +299,18 @@ class JoinFunction(torch.autograd.Function):
         s, y, (post_stats, pre_stats) = _forward(block, stream, post, gate, pre, drop, stream_scale, block_scale, need_s, True)
         need = ctx.needs_input_grad
         state = drop.seed if drop is not None and isinstance(drop.seed, torch.Tensor) else None
-        # a norm alone keeps what it normalised, a join its s; the block is kept for post and the gate alone
-        ctx.save_for_backward(block if post is not None or need[2] else None, (s if need_s else block) if pre is not None else None, gate, post_w, post_b, pre_w, pre_b,
-                              post_stats, pre_stats, state)
-        ctx.conf, ctx.like = conf, (block.shape, block.dtype, block.device)
+        # a norm alone keeps what it normalised, a join its s, or block and stream to compute it again; the block is kept for post and the gate too
+        ctx.again = need_s and _again(block, pre)
+        ctx.save_for_backward(block if post is not None or need[2] or ctx.again else None, None if pre is None or ctx.again else s if need_s else block,
+                              stream if ctx.again else None, gate, post_w, post_b, pre_w, pre_b, post_stats, pre_stats, state)
+        ctx.conf = conf
         ctx.set_materialize_grads(False)
         return (s, y) if need_s and pre is not None else s if need_s else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        block, s, gate, post_w, post_b, pre_w, pre_b, post_stats, pre_stats, state = ctx.saved_tensors
+        block, s, stream, gate, post_w, post_b, pre_w, pre_b, post_stats, pre_stats, state = ctx.saved_tensors
         post, pre, drop, stream_scale, block_scale, need_s = ctx.conf
         need = ctx.needs_input_grad
         ds, dy = grads if need_s and pre else (grads[0], None) if need_s else (None, grads[0])
@@ -310,7 +320,7 @@ class JoinFunction(torch.autograd.Function):
             drop = Drop(drop.p, state, 0, drop.per)
         post = post and Norm(post[0], post_w, post_b, post[1])
         pre = pre and Norm(pre[0], pre_w, pre_b, pre[1])
-        g = join_backward(ds, dy, block, s, (post_stats, pre_stats), post, gate, pre, drop, stream_scale, block_scale, need[0], need[1], need[2],
+        g = join_backward(ds, dy, block, s, (post_stats, pre_stats) + ((stream,) if ctx.again else ()), post, gate, pre, drop, stream_scale, block_scale, need[0], need[1], need[2],
                           need[3] or need[4], need[5] or need[6])
         return g.block, g.stream, g.gate, g.post_weight, g.post_bias, g.pre_weight, g.pre_bias, None
 

@@ -83,7 +83,7 @@ def _hat(v, n):
 
 
 def forward(f, x, gate, post, pre, drop, a, b):
-    """(s, y, bound of s, bound of y) of CPU tensors of one type, before the roundings of s and y to it, which are added here."""
+    """(s, y, bound of s, bound of y, bound of s before its rounding) of CPU tensors of one type, before the roundings of s and y to it, which are added here."""
     t, wide = f.dtype, lambda v: None if v is None else v.double()  # noqa: E731
     u, E = half_step(t), roundings(f.shape[-1])
     F, X, G = wide(f), wide(x), wide(gate)
@@ -100,36 +100,37 @@ def forward(f, x, gate, post, pre, drop, a, b):
         off = off + E * large * (hat.abs() + 1) * (w * scale * b * kept).abs() + 4 * SUM * (0 if post[2] is None else (post[2] * scale * b * kept).abs())
     by_s = off * (1 + u) + u * s.abs() + least(t)
     if pre is None:
-        return s, None, by_s, None
+        return s, None, by_s, None, off
     hat, _, inverse, large = _hat(s, pre)
     w = torch.ones(s.shape[-1], dtype=torch.float64) if pre[1] is None else pre[1]
     y = hat * w + (0 if pre[2] is None else pre[2])
     # s moves y by its own error, by that of the mean (the largest of the row's) and, times s^, by that of the deviation
     moved = inverse * off.amax(-1, keepdim=True) * (2 + 2 * hat.abs())
     off_y = (moved + E * large * (hat.abs() + 1)) * w.abs() + 4 * SUM * y.abs()
-    return s, y, by_s, off_y * (1 + u) + u * y.abs() + least(t)
+    return s, y, by_s, off_y * (1 + u) + u * y.abs() + least(t), off
 
 
-def _through(dh, dh_off, n, v, E):
-    """(gradient, its bound, dw, db and their bounds) of a norm of v with dh its result's gradient, off by dh_off."""
+def _through(dh, dh_off, n, v, E, v_off=None):
+    """(gradient, its bound, dw, db and their bounds) of a norm of v with dh its result's gradient, off by dh_off; v_off: what v is off by."""
     hat, _, inverse, large = _hat(v, n)
+    moved = 0 if v_off is None else inverse * v_off.amax(-1, keepdim=True) * (2 + 2 * hat.abs())
     w = torch.ones(v.shape[-1], dtype=torch.float64) if n[1] is None else n[1]
     g = dh * w
     out = g - hat * (g * hat).mean(-1, keepdim=True)
     if n[0] == "layer":
         out = out - g.mean(-1, keepdim=True)
     top = g.abs().amax(-1, keepdim=True) + (dh_off * w.abs()).amax(-1, keepdim=True)
-    off = inverse * (E * large * (2 + 2 * hat.abs()) * top * 2 + (dh_off * w.abs()).amax(-1, keepdim=True) * (2 + hat.abs()))
+    off = inverse * ((E * large * (2 + 2 * hat.abs()) + (0 if v_off is None else moved + moved.amax(-1, keepdim=True) * (1 + hat.abs()))) * top * 2 + (dh_off * w.abs()).amax(-1, keepdim=True) * (2 + hat.abs()))
     axes = tuple(range(v.dim() - 1))
     rows = v.numel() // v.shape[-1]
-    hat_off = E * large * (hat.abs() + 1)
+    hat_off = E * large * (hat.abs() + 1) + moved
     dw, dw_off = (dh * hat).sum(axes), (dh.abs() * hat_off + dh_off * (hat.abs() + hat_off)).sum(axes) + (rows + 8) * SUM * (dh * hat).abs().sum(axes)
     db, db_off = dh.sum(axes), dh_off.sum(axes) + (rows + 8) * SUM * dh.abs().sum(axes)
     return out * inverse, off, dw, dw_off, db, db_off
 
 
-def backward(ds, dy, f, s, gate, post, pre, drop, a, b, s_exact=None):
-    """{name: (value, bound)} of the gradients in the names of residual.Gradients, from s as it was rounded; its statistics are those of s_exact (of s where it is None)."""
+def backward(ds, dy, f, s, gate, post, pre, drop, a, b, s_exact=None, s_off=None):
+    """{name: (value, bound)} of the gradients in the names of residual.Gradients, from s, off by s_off; its statistics are those of s_exact (of s where it is None)."""
     t, wide = f.dtype, lambda v: None if v is None else v.double()  # noqa: E731
     u, E = half_step(t), roundings(f.shape[-1])
     F, G = wide(f), wide(gate)
@@ -146,7 +147,7 @@ def backward(ds, dy, f, s, gate, post, pre, drop, a, b, s_exact=None):
     off = torch.zeros_like(dr)
     if pre is not None and dy is not None:
         S = wide(s)
-        through, off, dw, dw_off, db, db_off = _through(wide(dy), torch.zeros_like(dr), pre, S, E)
+        through, off, dw, dw_off, db, db_off = _through(wide(dy), torch.zeros_like(dr), pre, S, E, s_off)
         if s_exact is not None:
             # the rounding moved s^ by u times s, which the statistics did not see
             hat, _, inverse, _ = _hat(s_exact, pre)
@@ -193,3 +194,8 @@ def within(got, want, bound, what=""):
     assert got.shape == want.shape, (what, got.shape, want.shape)
     over = (got - want).abs() - bound
     assert bool((over <= 0).all()), "%s: %g over a bound of %g at %r" % (what, float(over.max()), float(bound.flatten()[over.argmax()]), int(over.argmax()))
+
+
+def of_s(s, want):
+    """What `backward` takes for s and after it: s as it was rounded with the statistics of the exact one, or, of 16-bit types, which compute it again, the exact one."""
+    return dict(s=s.detach().cpu(), s_exact=want[0]) if s.dtype == torch.float32 else dict(s=want[0], s_off=want[4])

@@ -58,7 +58,7 @@ def test_join(dev, shape, t):
         assert torch.equal(again[0], s) and again[2] is None and (y is None or torch.equal(again[1], y))
         dy = dy if pr is not None else None
         for given in ((ds, dy), (None, dy) if pr is not None and i != 2 else (ds, None)):
-            wanted = ro.backward(*given, f, s.cpu(), gt, po, pr, drop, 0.75, 1.5, want[0])
+            wanted = ro.backward(*given, f, gate=gt, post=po, pre=pr, drop=drop, a=0.75, b=1.5, **ro.of_s(s, want))
             got = residual.join_backward(_cuda(given[0]), _cuda(given[1]), f.cuda(), s, stats, need_stream=stream, **how)._asdict()
             for k, v in got.items():
                 if k in wanted and v is not None:
@@ -213,9 +213,9 @@ def test_autograd(dev, host_layer, t):
         call = lambda: residual.join(leaves["block"], leaves.get("stream"), norms["post"], leaves.get("gate"), norms["pre"], Drop(*drop) if drop else None, 0.75, 1.5)  # noqa: E731
         out = call()
         s, y = out if pr is not None else (out, None)
-        exact = ro.forward(f, x, gt, po, pr, drop, 0.75, 1.5)[0]
+        exact = ro.forward(f, x, gt, po, pr, drop, 0.75, 1.5)
         for given in ([ds, dy], [None, dy], [ds, None]) if pr is not None else ([ds, None],):
-            wanted = ro.backward(*given, f, s.detach().cpu(), gt, po, pr, drop, 0.75, 1.5, exact)
+            wanted = ro.backward(*given, f, gate=gt, post=po, pre=pr, drop=drop, a=0.75, b=1.5, **ro.of_s(s, exact))
             pairs = [(o, v.cuda()) for o, v in zip((s, y), given) if v is not None]
             got = torch.autograd.grad([o for o, _ in pairs], list(leaves.values()), [v for _, v in pairs], retain_graph=True, allow_unused=True)
             for k, v in zip(leaves, got):
@@ -229,7 +229,27 @@ def test_autograd(dev, host_layer, t):
             out = call()
             outs = list(out) if pr is not None else [out]
             got = torch.autograd.grad(outs, [leaves[k]], [ds.cuda(), dy.cuda()][:len(outs)])[0]
-            ro.within(got, *ro.backward(ds, dy if pr is not None else None, f, s.detach().cpu(), gt, po, pr, drop, 0.75, 1.5, exact)[k], what=k)
+            ro.within(got, *ro.backward(ds, dy if pr is not None else None, f, gate=gt, post=po, pre=pr, drop=drop, a=0.75, b=1.5, **ro.of_s(s, exact))[k], what=k)
+
+
+@pytest.mark.parametrize("t", TYPES[1:], ids=str)
+def test_gradients_from_a_rounded_s(dev, host_layer, t):
+    """Without the block, pre's gradient goes by s as it is given; a norm behind a join whose s went nowhere, and one whose stream is missing, compute it again."""
+    f, x, _, pr, _, ds, dy = _inputs((3, 5, 72), t, 1, "none", "layer", "none")
+    n = _cuda(pr)
+    s, y, stats = residual.join_forward(f.cuda(), x.cuda(), pre=n, keep=True)
+    want = ro.forward(f, x, None, None, pr, None, 1.0, 1.0)
+    got = residual.join_backward(ds.cuda(), dy.cuda(), None, s, stats, pre=n)
+    for k, (v, bound) in ro.backward(ds, dy, f, s.cpu(), None, None, pr, None, 1.0, 1.0, s_exact=want[0]).items():
+        ro.within(getattr(got, k), v, bound, k)
+    again = residual.join_backward(ds.cuda(), dy.cuda(), f.cuda(), None, stats, pre=n)
+    for k, (v, bound) in ro.backward(ds, dy, f, want[0], None, None, pr, None, 1.0, 1.0, s_off=want[4]).items():
+        ro.within(getattr(again, k), v, bound, k)
+    leaf = f.cuda().requires_grad_()
+    _, y = residual.join(leaf, None, pre=n)
+    (df,) = torch.autograd.grad(y, leaf, dy.cuda())
+    want = ro.forward(f, None, None, None, pr, None, 1.0, 1.0)
+    ro.within(df, *ro.backward(None, dy, f, want[0], None, None, pr, None, 1.0, 1.0, s_off=want[4])["block"], what="alone")
 
 
 def test_nothing_to_do(dev, host_layer):
@@ -404,7 +424,7 @@ def test_many_samples(dev, C):
         s, y, stats = residual.join_forward(f.cuda(), x.cuda(), keep=True, **how)
         want = ro.forward(f, x, gt, po, pr, (0.2, 1, 2, "sample"), 1.0, 1.0)
         ro.within(s, want[0], want[2], "s")
-        wanted = ro.backward(ds, dy, f, s.cpu(), gt, po, pr, (0.2, 1, 2, "sample"), 1.0, 1.0, want[0])
+        wanted = ro.backward(ds, dy, f, gate=gt, post=po, pre=pr, drop=(0.2, 1, 2, "sample"), a=1.0, b=1.0, **ro.of_s(s, want))
         got = residual.join_backward(ds.cuda(), dy.cuda(), f.cuda(), s, stats, **how)._asdict()
         for k, (v, bound) in wanted.items():
             ro.within(got[k], v, bound, k)
