@@ -241,7 +241,7 @@ struct TeamShape { int vectors, waves, lanes; };
 int join_forward(const JoinArgs& a, int dtype, void* stream);
 int join_backward(const JoinGradients& g, int dtype, void* stream);
 template <typename T> int join_backward_of(const JoinGradients& g, void* stream);      // residual_backward.inc
-TeamShape back_shape(int C);
+TeamShape back_shape(const JoinGradients& g);
 // how many workgroups, and in how many parts a segment, a backward pass takes
 void join_plan(JoinGradients* g);
 // dst[which] = the sums of part[which] over the workgroups (gate of a sample: over a sample's)
