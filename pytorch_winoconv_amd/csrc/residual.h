@@ -142,29 +142,38 @@ struct Team {
   }
 };
 
-// Channels c .. c + 7 of a row of C, zeros behind its end: one 16-byte load (fp32: two) wherever it starts.  That of the row's last channels starts
-// before them, and what is in front is shifted out; no lane takes a branch to loads of single elements, which all would wait for.
-// EVEN: C is a multiple of eight.  `there`: the row is, else zeros.
+// Channels c .. c + 7 of a row of C, zeros behind its end: one 16-byte load (fp32: two) wherever it starts.  That of an odd row's last channels starts
+// before them, and what is in front is shifted out; lanes behind the row's end, or of no row, load something that is there.  The load stands behind no
+// branch and the shift where the values are wanted (settled8), so that all loads of a row are on their way at once.
+// `there`: the row is, else zeros.
+// Rows of whole vectors (C a multiple of eight), others, and those of fewer than eight channels
+enum { kEven, kOdd, kTiny };
 template <typename T> struct Raw8 { uint32_t w[2 * sizeof(T)]; };
-template <typename T, bool EVEN>
+template <typename T, int ROW>
 __device__ __forceinline__ Raw8<T> load8(const void* p, long long row, int c, int C, bool there) {
-  constexpr int W = 2 * sizeof(T);
   Raw8<T> r;
+  if constexpr (ROW != kOdd) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) r.w[i] = 0u;
-  if (EVEN || C < 8) {
-    if (EVEN && (!there || c >= C)) return r;
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) r.w[i] = 0u;
+    if (!there || c >= C) return r;
     T v[8];
-    load_run<T, 8>(p, row * C + c, EVEN ? 8 : there ? max(min(C - c, 8), 0) : 0, v);
+    load_run<T, 8>(p, row * C + c, ROW == kEven ? 8 : C - c, v);
     __builtin_memcpy(&r, v, sizeof(r));
-    return r;
+  } else {
+    const Run<T, 8> v = *reinterpret_cast<const Run<T, 8>*>(static_cast<const T*>(p) + (there ? row : 0) * C + min(c, C - 8));
+    __builtin_memcpy(&r, &v, sizeof(r));
   }
-  if (!there || c >= C) return r;
-  const int at = min(c, C - 8);
-  int k = c - at;
-  const Run<T, 8> v = *reinterpret_cast<const Run<T, 8>*>(static_cast<const T*>(p) + row * C + at);
-  __builtin_memcpy(&r, &v, sizeof(r));
-  if (k > 0) {
+  return r;
+}
+template <typename T, int ROW>
+__device__ __forceinline__ Raw8<T> settled8(Raw8<T> r, int c, int C, bool there) {
+  if (ROW != kOdd) return r;
+  constexpr int W = 2 * sizeof(T);
+  int k = c - (C - 8);                                 // channels in front
+  if (!there || c >= C) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = 0u;
+  } else if (k > 0) {
     asm volatile("" : "+v"(k));                        // (compared anew: its bits as masks, kept over the loop over rows, would be spilled)
     // by whole words, then by half a one
     constexpr int ONE = sizeof(T) == 4 ? 1 : 0;        // words of a shift by one element
@@ -191,19 +200,19 @@ __device__ __forceinline__ void floats_of(const Raw8<T>& r, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
 }
-template <typename T, bool EVEN>
+template <typename T, int ROW>
 __device__ __forceinline__ void parameter8(const void* p, int wide, long long row, int c, int C, float (&v)[8], float otherwise) {
   if (!p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = otherwise;
   } else if (wide) {
-    floats_of<float>(load8<float, EVEN>(p, row, c, C, true), v);
+    floats_of<float>(settled8<float, ROW>(load8<float, ROW>(p, row, c, C, true), c, C, true), v);
   } else {
-    floats_of<T>(load8<T, EVEN>(p, row, c, C, true), v);
+    floats_of<T>(settled8<T, ROW>(load8<T, ROW>(p, row, c, C, true), c, C, true), v);
   }
 }
-// x where element e of `have` is there, 0 where it is not; EVEN: eight are there or none, whose x is 0 as it is
-template <bool EVEN> __device__ __forceinline__ float kept_element(float x, int e, int have) { return EVEN || e < have ? x : 0.f; }
+// x where element e of `have` is there, 0 where it is not; of whole vectors eight are there or none, whose x is 0 as it is
+template <int ROW> __device__ __forceinline__ float kept_element(float x, int e, int have) { return ROW == kEven || e < have ? x : 0.f; }
 
 template <typename T>
 __device__ __forceinline__ void load_floats(const void* p, long long i, int have, float (&v)[8]) {

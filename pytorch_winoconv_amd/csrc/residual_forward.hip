@@ -6,7 +6,7 @@ namespace wc {
 namespace {
 
 // (v - mean) / deviation, in place; zeros behind `have`
-template <bool EVEN, int NV, int WAVES>
+template <int ROW, int NV, int WAVES>
 __device__ __forceinline__ void normalise(Team<WAVES>& team, float (&v)[NV][8], const int (&have)[NV], const Norm& n, int C, float* stats, long long row, bool first) {
   float mean = 0.f;
   if (n.kind == WC_NORM_LAYER) {
@@ -22,7 +22,7 @@ __device__ __forceinline__ void normalise(Team<WAVES>& team, float (&v)[NV][8], 
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[i][e] = kept_element<EVEN>(v[i][e] - (have[i] ? mean : 0.f), e, have[i]);
+      v[i][e] = kept_element<ROW>(v[i][e] - (have[i] ? mean : 0.f), e, have[i]);
       t = fmaf(v[i][e], v[i][e], t);
     }
   const float inverse = 1.f / sqrtf(team.sum(t) / C + n.eps);
@@ -43,7 +43,7 @@ __device__ __forceinline__ void scale_shift(const Norm& n, int c, int have, floa
 }
 
 // Rows blockIdx.x, blockIdx.x + gridDim.x, ... a team; one vector a thread: the next row is on its way while one is worked on, and the parameters stay in registers
-template <typename T, int NV, int WAVES, bool EVEN, bool AHEAD, bool ALONE>
+template <typename T, int NV, int WAVES, int ROW, bool AHEAD, bool ALONE>
 __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(JoinArgs a, int lanes) {
   __shared__ float meet[WAVES > 1 ? 4 * WAVES : 1];
   const int width = WAVES > 1 ? 64 * WAVES : lanes, slot = threadIdx.x & (width - 1), teams = WAVES > 1 ? 1 : 256 / lanes;
@@ -56,24 +56,24 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
   Raw8<T> f[NV], x[NV];
   auto load = [&](long long row) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) f[i] = load8<T, EVEN>(a.f, row, c[i], a.C, row < a.rows);
+    for (int i = 0; i < NV; ++i) f[i] = load8<T, ROW>(a.f, row, c[i], a.C, row < a.rows);
     if (!ALONE && a.x) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) x[i] = load8<T, EVEN>(a.x, row, c[i], a.C, row < a.rows);
+      for (int i = 0; i < NV; ++i) x[i] = load8<T, ROW>(a.x, row, c[i], a.C, row < a.rows);
     }
   };
   constexpr int KEPT = AHEAD ? NV : 1;
   float post_w[KEPT][8], post_b[KEPT][8], pre_w[KEPT][8], pre_b[KEPT][8], gate[KEPT][8];
   auto parameters = [&](const Norm& n, int c, float (&w)[8], float (&b)[8]) {
-    parameter8<T, EVEN>(n.weight, n.wide, 0, c, a.C, w, 1.f);
-    parameter8<T, EVEN>(n.bias, n.wide, 0, c, a.C, b, 0.f);
+    parameter8<T, ROW>(n.weight, n.wide, 0, c, a.C, w, 1.f);
+    parameter8<T, ROW>(n.bias, n.wide, 0, c, a.C, b, 0.f);
   };
   if constexpr (AHEAD) {
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) {
       if (!ALONE && a.post.kind) parameters(a.post, c[i], post_w[i], post_b[i]);
       if (a.pre.kind) parameters(a.pre, c[i], pre_w[i], pre_b[i]);
-      if (!ALONE && a.gate_rows == kGateChannel) parameter8<T, EVEN>(a.gate, a.gate_wide, 0, c[i], a.C, gate[i], 0.f);
+      if (!ALONE && a.gate_rows == kGateChannel) parameter8<T, ROW>(a.gate, a.gate_wide, 0, c[i], a.C, gate[i], 0.f);
     }
     load((long long)blockIdx.x * teams + threadIdx.x / width);
   }
@@ -87,8 +87,8 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
     for (int i = 0; i < NV; ++i) {
       have[i] = there ? max(min(a.C - c[i], 8), 0) : 0;
       asm volatile("" : "+v"(have[i]));
-      floats_of<T>(f[i], v[i]);
-      if (!ALONE && a.x) floats_of<T>(x[i], r[i]);
+      floats_of<T>(settled8<T, ROW>(f[i], c[i], a.C, there), v[i]);
+      if (!ALONE && a.x) floats_of<T>(settled8<T, ROW>(x[i], c[i], a.C, there), r[i]);
       else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[i][e] = 0.f;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
       if (base + step < a.rows) load(row + step);
     }
     if (!ALONE && a.post.kind) {
-      normalise<EVEN, NV, WAVES>(team, v, have, a.post, a.C, a.post_stats, row, slot == 0 && there);
+      normalise<ROW, NV, WAVES>(team, v, have, a.post, a.C, a.post_stats, row, slot == 0 && there);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int k = AHEAD ? i : 0;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
     for (int i = 0; i < NV; ++i) {
       if (!ALONE && a.gate_rows) {
         const int k = AHEAD ? i : 0;
-        if (!AHEAD || a.gate_rows != kGateChannel) parameter8<T, EVEN>(a.gate, a.gate_wide, g0, c[i], a.C, gate[k], 0.f);
+        if (!AHEAD || a.gate_rows != kGateChannel) parameter8<T, ROW>(a.gate, a.gate_wide, g0, c[i], a.C, gate[k], 0.f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[i][e] *= gate[k][e];
       }
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
     }
     if (!ALONE && !a.pre.kind) continue;
     // (of s before its rounding)
-    normalise<EVEN, NV, WAVES>(team, v, have, a.pre, a.C, a.pre_stats, row, slot == 0 && there);
+    normalise<ROW, NV, WAVES>(team, v, have, a.pre, a.C, a.pre_stats, row, slot == 0 && there);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k = AHEAD ? i : 0;
@@ -239,10 +239,13 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value, THREADS = WAVES > 1 ? 64 * WAVES : 256;
       constexpr bool AHEAD = decltype(ahead)::value;
       const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? kCus * (2048 / THREADS) : kMostBlocks / 2;
-      constexpr bool BOTH = (NV == 1 && WAVES == 1) || (NV == 2 && WAVES == 16), ALONE = BOTH || NV == 2;      // what is there of a form
-      auto fn = a.C % 8 == 0 ? &join_kernel<T, NV, WAVES, true, AHEAD, ALONE> : &join_kernel<T, NV, WAVES, false, AHEAD, ALONE>;
-      if constexpr (BOTH) {
-        if (!alone) fn = a.C % 8 == 0 ? &join_kernel<T, NV, WAVES, true, AHEAD, false> : &join_kernel<T, NV, WAVES, false, AHEAD, false>;
+      // (what is there of a form: two vectors a thread of even rows alone, and of joins in 16 wavefronts alone)
+      auto fn = alone ? &join_kernel<T, NV, WAVES, kEven, AHEAD, true> : &join_kernel<T, NV, WAVES, kEven, AHEAD, NV == 2 && WAVES < 16>;
+      if constexpr (NV == 1) {
+        if (!even) fn = alone ? &join_kernel<T, NV, WAVES, kOdd, AHEAD, true> : &join_kernel<T, NV, WAVES, kOdd, AHEAD, false>;
+      }
+      if constexpr (NV == 1 && WAVES == 1) {
+        if (a.C < 8) fn = alone ? &join_kernel<T, NV, WAVES, kTiny, AHEAD, true> : &join_kernel<T, NV, WAVES, kTiny, AHEAD, false>;
       }
       hipLaunchKernelGGL(fn, dim3((unsigned)(wanted < most ? wanted : most)), dim3(THREADS), 0, as_stream(stream), a, lanes);
       WC_CHECK_LAUNCH("join_kernel");
@@ -255,9 +258,9 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       while (lanes < vectors) lanes *= 2;
       return go(ic<1>{}, ic<1>{}, ahead, lanes);
     }
-    // A norm alone takes two vectors a thread and every row a workgroup of its own: there is little to keep in registers, and fewer wait at a barrier
+    // A norm alone of even rows takes two vectors a thread and every row a workgroup of its own: there is little to keep in registers, and fewer wait at a barrier
     // (us, bf16 rms, two | one ahead: 65536 x 1024 46.9 | 47.3, 16384 x 4096 46.0 | 49.3, 8192 x 8192 45.2 | 57.8).  Joins the other way about (8192 x 4096 76 | 63)
-    if (alone) {
+    if (alone && even) {
       if (vectors <= 128) return go(ic<2>{}, ic<1>{}, whole, 64);
       if (vectors <= 256) return go(ic<2>{}, ic<2>{}, whole, 64);
       if (vectors <= 512) return go(ic<2>{}, ic<4>{}, whole, 64);
