@@ -7,9 +7,9 @@
 namespace wc {
 
 // Vectors of a thread, wavefronts and lanes of a team of a backward pass; vectors 0: long rows.  One vector a thread up to 8192 channels: the sums and the row
-// that is on its way leave no registers for more.  A workgroup of 16 wavefronts has 128 registers a thread, which spills: of more than 4096 channels a norm alone,
-// and what goes through no norm, fits; otherwise rows of no whole vectors, and all of more than 8192, are long ones (us, in registers | long: 2048 x 8001 bf16
-// with two norms, gate and dropout 385 | 317, 2048 x 16384 630 | 416; a norm alone 4096 x 8001 87 | 164, 4096 x 16384 113 | 225, 4096 x 12001 395 | 284)
+// that is on its way leave no registers for more.  Two, of 16 wavefronts with 128 registers a thread, hold a norm alone and what goes through no norm; the rest spills
+// and is left to the passes of long rows (us, in registers | long: 2048 x 16384 bf16 with two norms, gate and dropout 591 | 457; a norm alone 4096 x 16384
+// 109 | 225, 4096 x 12001 120 | 282; 2048 x 8001 with two norms, gate and dropout, one vector, 163 | 360)
 TeamShape back_shape(const JoinGradients& g) {
   const int vectors = ceil_div(g.C, 8);
   if (vectors <= 64) {
@@ -19,9 +19,9 @@ TeamShape back_shape(const JoinGradients& g) {
   }
   for (int waves = 2; waves <= 8; waves *= 2)
     if (vectors <= 64 * waves) return {1, waves, 64};
-  const bool even = g.C % 8 == 0, alone = !g.gate_rows && !g.ds && !g.dx, little = !g.post.kind && (!g.pre.kind || alone);
-  if (vectors <= 1024 && (even || little)) return {1, 16, 64};
-  if (vectors <= 2048 && little && (even || !g.pre.kind)) return {2, 16, 64};
+  if (vectors <= 1024) return {1, 16, 64};
+  const bool alone = !g.gate_rows && !g.ds && !g.dx, little = !g.post.kind && (!g.pre.kind || alone);
+  if (vectors <= 2048 && little) return {2, 16, 64};
   return {0, 16, 64};
 }
 
