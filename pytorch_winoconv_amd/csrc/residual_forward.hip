@@ -1,6 +1,8 @@
 // s = a x + b g drop(post(f)) and y = pre(s) of residual.h, a row a team at a time: one read of f and x, one write of s and y, whatever of it there is.
 #include "residual.h"
 
+#include <algorithm>
+
 namespace wc {
 
 namespace {
@@ -52,7 +54,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
   const Keys keys = !ALONE && a.drop.level ? keys_of(a.drop) : Keys{0, 0};
   int c[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) c[i] = (i * width + slot) * 8;
+  for (int i = 0; i < NV; ++i) c[i] = (((int)blockIdx.y * NV + i) * width + slot) * 8;      // (a part of the row, where no norm wants all of it)
   Raw8<T> f[NV], x[NV];
   auto load = [&](long long row) {
 #pragma unroll
@@ -235,10 +237,10 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     // as many workgroups as the compute units hold at once, or as there are rows
-    auto go = [&](auto nv, auto waves, auto ahead, int lanes) -> int {
+    auto go = [&](auto nv, auto waves, auto ahead, int lanes, int pieces = 1) -> int {
       constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value, THREADS = WAVES > 1 ? 64 * WAVES : 256;
       constexpr bool AHEAD = decltype(ahead)::value;
-      const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? kCus * (2048 / THREADS) : kMostBlocks / 2;
+      const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? std::max(1, kCus * (2048 / THREADS) / pieces) : kMostBlocks / 2;
       // (what is there of a form: two vectors a thread of even rows alone, and of joins in 16 wavefronts alone)
       auto fn = alone ? &join_kernel<T, NV, WAVES, kEven, AHEAD, true> : &join_kernel<T, NV, WAVES, kEven, AHEAD, NV == 2 && WAVES < 16>;
       if constexpr (NV == 1) {
@@ -247,7 +249,7 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       if constexpr (NV == 1 && WAVES == 1) {
         if (a.C < 8) fn = alone ? &join_kernel<T, NV, WAVES, kTiny, AHEAD, true> : &join_kernel<T, NV, WAVES, kTiny, AHEAD, false>;
       }
-      hipLaunchKernelGGL(fn, dim3((unsigned)(wanted < most ? wanted : most)), dim3(THREADS), 0, as_stream(stream), a, lanes);
+      hipLaunchKernelGGL(fn, dim3((unsigned)(wanted < most ? wanted : most), (unsigned)pieces), dim3(THREADS), 0, as_stream(stream), a, lanes);
       WC_CHECK_LAUNCH("join_kernel");
       return WC_OK;
     };
@@ -258,6 +260,8 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       while (lanes < vectors) lanes *= 2;
       return go(ic<1>{}, ic<1>{}, ahead, lanes);
     }
+    // Without a norm nothing is wanted of a whole row: pieces of 1024 channels (us, dropout of 8192 x 8192 bf16 52, in whole rows 62)
+    if (!a.post.kind && !a.pre.kind) return go(ic<1>{}, ic<2>{}, ahead, 64, ceil_div(vectors, 128));
     // A norm alone of even rows takes two vectors a thread and every row a workgroup of its own: there is little to keep in registers, and fewer wait at a barrier
     // (us, bf16 rms, two | one ahead: 65536 x 1024 46.9 | 47.3, 16384 x 4096 46.0 | 49.3, 8192 x 8192 45.2 | 57.8).  Joins the other way about (8192 x 4096 76 | 63)
     if (alone && even) {
