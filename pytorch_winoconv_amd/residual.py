@@ -429,7 +429,8 @@ class ResidualStack(nn.Module):
     shape, as matrix_block makes; with channel_axis=1 convolutions may be among them.  Each join, with the next block's norm, is one pass over memory.
 
     kind: of the norms; post: norms behind the blocks too; gate: the value that a learned gate a channel starts with, or None; drop: probability, a whole sample
-    at a time (per="sample") or element by element."""
+    at a time (per="sample") or element by element.  A pass may be captured into a graph (counter=True draws another mask in every replay); as with every torch module, no eager
+    autograd graph of the same parameters may be alive while a backward pass is captured."""
 
     def __init__(self, blocks, channels, kind="layer", eps=1e-5, post=False, gate=None, drop=0.0, per="sample", stream_scale=1.0, block_scale=1.0, counter=False,
                  channel_axis=-1, device=None, dtype=None):
