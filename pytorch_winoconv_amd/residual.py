@@ -217,6 +217,8 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
     x = stats[2] if again else None
     if (post is not None or need_gate) and block is None:
         raise ValueError("join_backward: the gradients of post and the gate need block")
+    if through is not None and block is not None and given.dtype != torch.float32 and not again:
+        raise ValueError("join_backward: of 16-bit types stats holds the stream too, as join_forward kept it")
     if through is not None and s is None and not again:
         raise ValueError("join_backward: the gradient of pre needs s, or block and what join_forward kept")
     rows = _rows(given.shape)

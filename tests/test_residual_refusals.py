@@ -111,8 +111,10 @@ def test_operands_that_do_not_fit(host_layer):
             (lambda: residual.join_backward(f, f, f, f, None), ValueError, "dy without pre"),
             (lambda: residual.join_backward(f, None, None, f, None, post=Norm("rms")), ValueError, "need block"),
             (lambda: residual.join_backward(f, None, None, f, None, gate=half(C)), ValueError, "need block"),
-            (lambda: residual.join_backward(None, f, f, None, None, pre=Norm("rms")), ValueError, "needs s"),
-            (lambda: residual.join_backward(None, f, f, f, None, pre=Norm("rms")), ValueError, "statistics of pre"),
+            (lambda: residual.join_backward(None, f, None, None, None, pre=Norm("rms")), ValueError, "needs s"),
+            (lambda: residual.join_backward(None, f, None, f, None, pre=Norm("rms")), ValueError, "statistics of pre"),
+            (lambda: residual.join_backward(None, f, f, f, (None, torch.zeros(6, 2)), pre=Norm("rms")), ValueError, "holds the stream"),
+            (lambda: residual.join_backward(None, f, f, f, (None, torch.zeros(6, 2), f[:2]), pre=Norm("rms")), ValueError, "the stream has shape"),
             (lambda: residual.join_backward(f, None, f, f, (torch.zeros(5, 2), None), post=Norm("rms")), ValueError, "statistics of post"),
             (lambda: residual.join_backward(f, None, f[:2], f, None), ValueError, "block has shape")]:
         with pytest.raises(error, match=match):
