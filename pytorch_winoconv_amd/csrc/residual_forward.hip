@@ -46,17 +46,20 @@ __device__ __forceinline__ void scale_shift(const Norm& n, int c, int have, floa
   for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], w[e], b[e]);
 }
 
-// Rows blockIdx.x, blockIdx.x + gridDim.x, ... a team; one vector a thread: the next row is on its way while one is worked on, and the parameters stay in registers
+// Rows block, block + blocks, ... a team; one vector a thread: the next row is on its way while one is worked on, and the parameters stay in registers.  Without a
+// norm two wavefronts take one of the `pieces` of a row, neighbouring workgroups those of one row
 template <typename T, int NV, int WAVES, int ROW, bool AHEAD, bool ALONE>
-__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(JoinArgs a, int lanes) {
+__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(JoinArgs a, int lanes, int pieces) {
   __shared__ float meet[WAVES > 1 ? 4 * WAVES : 1];
   const int width = WAVES > 1 ? 64 * WAVES : lanes, slot = threadIdx.x & (width - 1), teams = WAVES > 1 ? 1 : 256 / lanes;
-  const long long step = (long long)gridDim.x * teams;
+  constexpr bool SPLIT = AHEAD && !ALONE && WAVES == 2;
+  const unsigned block = SPLIT ? blockIdx.x / (unsigned)pieces : blockIdx.x, piece = SPLIT ? blockIdx.x % (unsigned)pieces : 0u;
+  const long long step = (long long)(SPLIT ? gridDim.x / (unsigned)pieces : gridDim.x) * teams;
   Team<WAVES> team = {lanes, meet, 0};
   const Keys keys = !ALONE && a.drop.level ? keys_of(a.drop) : Keys{0, 0};
   int c[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) c[i] = (((int)blockIdx.y * NV + i) * width + slot) * 8;      // (a part of the row, where no norm wants all of it)
+  for (int i = 0; i < NV; ++i) c[i] = (((int)piece * NV + i) * width + slot) * 8;
   Raw8<T> f[NV], x[NV];
   auto load = [&](long long row) {
 #pragma unroll
@@ -79,9 +82,9 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) void join_kernel(Join
       if (a.pre.kind) parameters(a.pre, c[i], pre_w[i], pre_b[i]);
       if (!ALONE && a.gate_rows == kGateChannel) parameter8<T, ROW>(a.gate, a.gate_wide, 0, c[i], a.C, gate[i], 0.f);
     }
-    load((long long)blockIdx.x * teams + threadIdx.x / width);
+    load((long long)block * teams + threadIdx.x / width);
   }
-  for (long long base = (long long)blockIdx.x * teams; base < a.rows; base += step) {
+  for (long long base = (long long)block * teams; base < a.rows; base += step) {
     const long long row = base + (WAVES > 1 ? 0 : threadIdx.x / lanes);
     const bool there = row < a.rows;           // (lanes of other teams of the wavefront go on, and it takes them for its exchanges)
     if constexpr (!AHEAD) load(row);
@@ -238,11 +241,13 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
   const bool alone = a.pre.kind && !a.post.kind && !a.x && !a.gate_rows && !a.drop.level && !a.s && a.b == 1.f;
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    // as many workgroups as the compute units hold at once, or as there are rows
+    // as many workgroups as the compute units hold at once, or as there are rows; of two wavefronts, which end soon, four times as many (us, inputs from memory,
+    // one | four times: dropout of 8192 x 8192 bf16 64 | 59, with a stream 86 | 78; 60000 x 1000 fp16 with two norms, gate and dropout 137 | 129.  Of more wavefronts
+    // 8192 x 4096 takes 65 | 72, of less 200704 x 256 101 | 103)
     auto go = [&](auto nv, auto waves, auto ahead, int lanes, int pieces = 1) -> int {
       constexpr int NV = decltype(nv)::value, WAVES = decltype(waves)::value, THREADS = WAVES > 1 ? 64 * WAVES : 256;
       constexpr bool AHEAD = decltype(ahead)::value;
-      const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? std::max(1, kCus * (2048 / THREADS) / pieces) : kMostBlocks / 2;
+      const long long wanted = WAVES > 1 ? a.rows : ceil_div_ll(a.rows, 256 / lanes), most = AHEAD ? std::max(1, kCus * (2048 / THREADS) * (WAVES == 2 ? 4 : 1) / pieces) : kMostBlocks / 2;
       // (what is there of a form: two vectors a thread of even rows alone, and of joins in 16 wavefronts alone)
       auto fn = alone ? &join_kernel<T, NV, WAVES, kEven, AHEAD, true> : &join_kernel<T, NV, WAVES, kEven, AHEAD, NV == 2 && WAVES < 16>;
       if constexpr (NV == 1) {
@@ -251,7 +256,7 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       if constexpr (NV == 1 && WAVES == 1) {
         if (a.C < 8) fn = alone ? &join_kernel<T, NV, WAVES, kTiny, AHEAD, true> : &join_kernel<T, NV, WAVES, kTiny, AHEAD, false>;
       }
-      hipLaunchKernelGGL(fn, dim3((unsigned)(wanted < most ? wanted : most), (unsigned)pieces), dim3(THREADS), 0, as_stream(stream), a, lanes);
+      hipLaunchKernelGGL(fn, dim3((unsigned)((wanted < most ? wanted : most) * pieces)), dim3(THREADS), 0, as_stream(stream), a, lanes, pieces);
       WC_CHECK_LAUNCH("join_kernel");
       return WC_OK;
     };
@@ -262,7 +267,7 @@ int join_forward(const JoinArgs& a, int dtype, void* stream) {
       while (lanes < vectors) lanes *= 2;
       return go(ic<1>{}, ic<1>{}, ahead, lanes);
     }
-    // Without a norm nothing is wanted of a whole row: pieces of 1024 channels (us, dropout of 8192 x 8192 bf16 52, in whole rows 62)
+    // Without a norm nothing is wanted of a whole row: pieces of 1024 channels (us, dropout of 8192 x 8192 bf16 59, in whole rows 66)
     if (!a.post.kind && !a.pre.kind) return go(ic<1>{}, ic<2>{}, ahead, 64, ceil_div(vectors, 128));
     // A norm alone of even rows takes two vectors a thread and every row a workgroup of its own: there is little to keep in registers, and fewer wait at a barrier
     // (us, bf16 rms, two | one ahead: 65536 x 1024 46.9 | 47.3, 16384 x 4096 46.0 | 49.3, 8192 x 8192 45.2 | 57.8).  Joins the other way about (8192 x 4096 76 | 63)

@@ -441,3 +441,22 @@ def test_same_bits_every_time(dev):
     first = step()
     for _ in range(4):
         assert all(torch.equal(a, b) for a, b in zip(first, step()))
+
+
+@pytest.mark.parametrize("rows,C", [(5000, 4104), (17000, 523), (600, 70001)])
+def test_rows_in_pieces(dev, rows, C):
+    """Joins without a norm whose rows are taken in pieces, more rows than workgroups: the mask of narrower rows, and the sum value by value."""
+    g = torch.Generator().manual_seed(C)
+    f, x = torch.randn(rows, C, generator=g).cuda(), torch.randn(rows, C, generator=g).cuda()
+    gate, drop = torch.randn(C, generator=g).cuda(), Drop(0.25, 11, 12)
+    out = residual.dropout_forward(f, drop)
+    assert torch.equal(out[:, :512], residual.dropout_forward(f[:, :512].contiguous(), drop))
+    kept = out != 0
+    assert torch.equal(out, torch.where(kept, f * torch.tensor(1 / 0.75, device=dev), torch.zeros_like(f)))
+    # (the share of n channels: a standard deviation of sqrt(3 / 16 / n); six of them)
+    assert abs(kept.double().mean().item() - 0.75) < 6 * (3 / 16 / (rows * C)) ** 0.5
+    s, _, _ = residual.join_forward(f, x, gate=gate, drop=drop, stream_scale=0.5, block_scale=2.0)
+    block = torch.where(kept, f.double() * gate.double() * (2.0 / 0.75), torch.zeros((), dtype=torch.float64, device=dev))
+    # four roundings of the block's factors and products, one of the share, one of the sum
+    bound = (5 * block.abs() + (block + 0.5 * x.double()).abs()) * 2.0 ** -23
+    assert ((s.double() - (block + 0.5 * x.double())).abs() <= bound).all()
