@@ -846,6 +846,9 @@ wc_norm norm_of(int kind, double eps, const MaybeTensor& w, const MaybeTensor& b
 bool norm_fits(const MaybeTensor& w, const MaybeTensor& b, const at::Tensor& f, int64_t C) {
   return own_or_wide(w, f) && own_or_wide(b, f) && channels_of(w, C) && channels_of(b, C) && !(w && b && w->scalar_type() != b->scalar_type());
 }
+bool gate_fits(const MaybeTensor& t, const at::Tensor& f, int64_t C) {
+  return !t || (t->dim() == 1 && t->size(0) == C) || (t->dim() == 2 && t->size(0) == (f.dim() > 1 ? f.size(0) : 1) && t->size(1) == C);
+}
 wc_join_desc join_desc(const at::Tensor& f, const MaybeTensor& gate, double a, double b, const wc_norm& post, const wc_norm& pre, int level, bool per_sample, uint64_t seed,
                        uint64_t offset, const MaybeTensor& state) {
   const int64_t C = f.size(f.dim() - 1);
@@ -858,11 +861,10 @@ py::object join_forward(const at::Tensor& f_, const MaybeTensor& x_, const Maybe
                         uint64_t offset, const MaybeTensor& state, bool need_s, bool keep) {
   const int64_t nd = f_.dim();
   if (!linear_type(f_) || nd < 1 || f_.numel() == 0 || f_.size(nd - 1) > 1 << 24) return py::none();
-  const int64_t C = f_.size(nd - 1), samples = nd > 1 ? f_.size(0) : 1;
-  if (!same_kind(x_, f_) || (x_ && x_->sizes() != f_.sizes()) || !own_or_wide(gate_, f_) || !norm_fits(post_w_, post_b_, f_, C) || !norm_fits(pre_w_, pre_b_, f_, C) ||
+  const int64_t C = f_.size(nd - 1);
+  if (!same_kind(x_, f_) || (x_ && x_->sizes() != f_.sizes()) || !own_or_wide(gate_, f_) || !gate_fits(gate_, f_, C) || !norm_fits(post_w_, post_b_, f_, C) || !norm_fits(pre_w_, pre_b_, f_, C) ||
       (state && state->device() != f_.device()))
     return py::none();
-  if (gate_ && !(gate_->dim() == 1 && gate_->size(0) == C) && !(gate_->dim() == 2 && gate_->size(0) == samples && gate_->size(1) == C)) return py::none();
   const c10::DeviceGuard guard(f_.device());
   const at::Tensor f = f_.contiguous();
   const MaybeTensor x = dense(x_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_), pre_b = dense(pre_b_);
@@ -901,22 +903,36 @@ py::object norm_forward(const at::Tensor& x_, int kind, double eps, const MaybeT
   return keep ? py::object(py::make_tuple(y, stats)) : py::cast(y);
 }
 
-// operands that the Python layer has checked; rows > 0
-py::tuple join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& x_, const MaybeTensor& gate_, const MaybeTensor& post_stats,
-                        const MaybeTensor& pre_stats, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_, const MaybeTensor& post_b_, int pre_kind,
-                        double pre_eps, const MaybeTensor& pre_w_, const MaybeTensor& pre_b_, int level, bool per_sample, uint64_t seed, uint64_t offset,
-                        const MaybeTensor& state, bool need_f, bool need_x, bool need_gate, bool need_post, bool need_pre) {
+// The gradients of pre are those of what dy came through; f, s and x are checked where they are not read too.  None also where nothing is asked for
+py::object join_backward(const MaybeTensor& ds_, const MaybeTensor& dy_, const MaybeTensor& f_, const MaybeTensor& s_, const MaybeTensor& x_, bool again, const MaybeTensor& gate_,
+                         const MaybeTensor& post_stats, const MaybeTensor& pre_stats, double a, double b, int post_kind, double post_eps, const MaybeTensor& post_w_,
+                         const MaybeTensor& post_b_, int pre_kind, double pre_eps, const MaybeTensor& pre_w_, const MaybeTensor& pre_b_, int level, bool per_sample, uint64_t seed,
+                         uint64_t offset, const MaybeTensor& state, bool need_f, bool need_x, bool need_gate, bool need_post, bool need_pre) {
   const at::Tensor& like = ds_ ? *ds_ : *dy_;
+  const int64_t nd = like.dim();
+  if (!linear_type(like) || nd < 1 || like.numel() == 0 || like.size(nd - 1) > 1 << 24) return py::none();
+  const int64_t C = like.size(nd - 1), rows = like.numel() / C;
+  for (const MaybeTensor* t : {&ds_, &dy_, &f_, &s_, &x_})
+    if (!same_kind(*t, like) || (*t && (*t)->sizes() != like.sizes())) return py::none();
+  if (!own_or_wide(gate_, like) || !gate_fits(gate_, like, C) || !norm_fits(post_w_, post_b_, like, C) || !norm_fits(pre_w_, pre_b_, like, C) ||
+      (state && state->device() != like.device()))
+    return py::none();
+  auto kept = [&](const MaybeTensor& t) {
+    return t && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == rows && t->size(1) == 2 && t->device() == like.device() && t->is_contiguous();
+  };
+  if ((post_kind && !kept(post_stats)) || (pre_kind && !kept(pre_stats))) return py::none();
+  need_gate = need_gate && gate_;
+  if (!(need_f || need_x || need_gate || (need_post && (post_w_ || post_b_)) || (need_pre && (pre_w_ || pre_b_)))) return py::none();
   const c10::DeviceGuard guard(like.device());
-  const MaybeTensor ds = dense(ds_), dy = dense(dy_), f = dense(f_), s = dense(s_), x = dense(x_), gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_),
-                    pre_b = dense(pre_b_);
+  const MaybeTensor none, ds = dense(ds_), dy = dense(dy_), f = post_kind || need_gate || again ? dense(f_) : none, s = pre_kind && !again ? dense(s_) : none, x = dense(x_),
+                    gate = dense(gate_), post_w = dense(post_w_), post_b = dense(post_b_), pre_w = dense(pre_w_), pre_b = dense(pre_b_);
   const wc_join_desc d = join_desc(like, gate, a, b, norm_of(post_kind, post_eps, post_w, post_b, like), norm_of(pre_kind, pre_eps, pre_w, pre_b, like), level, per_sample, seed, offset,
                                    state);
   at::Tensor df, dx, dpost_w, dpost_b, dgate, dpre_w, dpre_b;
   auto fresh = [](const at::Tensor& t) { return at::empty(t.sizes(), t.options()); };
   if (need_f) df = fresh(like);
   if (need_x) dx = fresh(like);
-  if (need_gate && gate) dgate = fresh(*gate);
+  if (need_gate) dgate = fresh(*gate);
   if (need_post && post_w) dpost_w = fresh(*post_w);
   if (need_post && post_b) dpost_b = fresh(*post_b);
   if (need_pre && pre_w) dpre_w = fresh(*pre_w);

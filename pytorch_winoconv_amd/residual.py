@@ -221,6 +221,12 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
         raise ValueError("join_backward: of 16-bit types stats holds the stream too, as join_forward kept it")
     if through is not None and s is None and not again:
         raise ValueError("join_backward: the gradient of pre needs s, or block and what join_forward kept")
+    if engine.USE_EXT and through is pre:
+        out = engine._ext.join_backward(ds, dy, block, s, x, again, gate, post_stats, pre_stats, float(stream_scale), float(block_scale), *_ext_norm(post), *_ext_norm(pre),
+                                        *_ext_drop(drop), need_block, need_stream, need_gate, need_post, need_pre)
+        if out is not None:
+            df, dx, pw, pb, qw, qb, dg = out
+            return Gradients(df, dx, qw, qb, dg, pw, pb)
     rows = _rows(given.shape)
     for n, t, what in ((post, post_stats, "post"), (through, pre_stats, "pre")):
         if n is not None and (t is None or t.dtype != torch.float32 or tuple(t.shape) != (rows, 2) or t.device != given.device or not t.is_contiguous()):
@@ -239,23 +245,18 @@ def join_backward(ds, dy, block, s, stats, post=None, gate=None, pre=None, drop=
                          pb if silent[1] is None else zeros(silent[1]))
     if not (need_block or need_stream or any(t is not None for t in want)):
         return Gradients(None, None, None, None, None, zeros(silent[0]), zeros(silent[1]))
-    if engine.USE_EXT:
-        df, dx, pw, pb, qw, qb, dg = engine._ext.join_backward(ds, dy, block if post is not None or need_gate or again else None,
-                                                               s if through is not None and not again else None, x, gate, post_stats, pre_stats, float(stream_scale), float(block_scale), *_ext_norm(post), *_ext_norm(through),
-                                                               *_ext_drop(drop), need_block, need_stream, need_gate, need_post, need_pre)
-    else:
-        ds, dy, block, s, x, g = (_plain(t) for t in (ds, dy, block, s, x, gate))
-        d, kept = _desc(given, post, g, through, drop, stream_scale, block_scale)
-        df, dx = (dense(given) if wanted else None for wanted in (need_block, need_stream))
-        pw, pb, qw, qb, dg = (None if t is None else dense(t) for t in want)
-        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        q = _lib.JoinGradients(*(at(t) for t in (ds, dy, block if post is not None or need_gate or again else None,
-                                                 s if through is not None and not again else None, x, g, post_stats, pre_stats, df, dx, pw, pb, qw, qb, dg)))
-        lib, nbytes = _lib.load(), ctypes.c_size_t()
-        check(lib.wc_join_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(q), ctypes.byref(nbytes)))
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=given.device)
-        with engine._on_device(given):
-            check(lib.wc_join_backward(ctypes.byref(d), ctypes.byref(q), engine._ptr(ws), nbytes.value, engine._stream(given)))
+    ds, dy, block, s, x, g = (_plain(t) for t in (ds, dy, block, s, x, gate))
+    d, kept = _desc(given, post, g, through, drop, stream_scale, block_scale)
+    df, dx = (dense(given) if wanted else None for wanted in (need_block, need_stream))
+    pw, pb, qw, qb, dg = (None if t is None else dense(t) for t in want)
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    q = _lib.JoinGradients(*(at(t) for t in (ds, dy, block if post is not None or need_gate or again else None,
+                                             s if through is not None and not again else None, x, g, post_stats, pre_stats, df, dx, pw, pb, qw, qb, dg)))
+    lib, nbytes = _lib.load(), ctypes.c_size_t()
+    check(lib.wc_join_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(q), ctypes.byref(nbytes)))
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=given.device)
+    with engine._on_device(given):
+        check(lib.wc_join_backward(ctypes.byref(d), ctypes.byref(q), engine._ptr(ws), nbytes.value, engine._stream(given)))
     return Gradients(df, dx, qw, qb, dg, zeros(silent[0]) if pw is None else pw, zeros(silent[1]) if pb is None else pb)
 
 
