@@ -789,17 +789,20 @@ py::object pack4(const at::Tensor& x_) {
 }
 
 // codes and scales of a Packed4 with elements
-at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
+at::Tensor widened4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, at::ScalarType type) {
   const c10::DeviceGuard guard(codes.device());
   at::DimVector shape(codes.sizes());
   shape[shape.size() - 1] = C;
-  at::Tensor x = at::empty(shape, codes.options().dtype(torch::python::detail::py_object_to_dtype(type)));
+  at::Tensor x = at::empty(shape, codes.options().dtype(type));
   void* stream = stream_of(codes);
   {
     py::gil_scoped_release nogil;
     check(wc_unpack4(bytes_of(codes), bytes_of(scales), x.data_ptr(), x.numel() / C, (int)C, dtype_of(x), stream));
   }
   return x;
+}
+at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
+  return widened4(codes, scales, C, torch::python::detail::py_object_to_dtype(type));
 }
 
 // x as it is, or the codes and scales of a Packed4 that reads as `type`; codes and scales of w (K, C)
@@ -832,6 +835,34 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
                              bytes, stream));
   }
   return py::cast(y);
+}
+
+// dx alone of a layer over a Packed4 w (K, C)
+py::object linear4_backward(const at::Tensor& dy_, const at::Tensor& w_codes, const at::Tensor& w_scales, int64_t C, const MaybeTensor& z_, int activation) {
+  const int64_t nd = dy_.dim();
+  if (!linear_type(dy_) || nd < 1 || dy_.numel() == 0 || w_codes.numel() == 0 || w_codes.dim() != 2 || w_codes.size(0) != dy_.size(nd - 1) || w_codes.device() != dy_.device() || !fits(C) ||
+      !fits(w_codes.size(0)) || (activation && (!z_ || !same_kind(z_, dy_) || z_->sizes() != dy_.sizes())))
+    return py::none();
+  const c10::DeviceGuard guard(dy_.device());
+  const at::Tensor dy = packed_rows(dy_), w = widened4(w_codes, w_scales, C, dy.scalar_type());
+  const MaybeTensor z = activation ? packed_rows(z_) : MaybeTensor();
+  at::DimVector shape(dy.sizes());
+  const int64_t K = shape[nd - 1];
+  shape[nd - 1] = C;
+  at::Tensor dx = at::empty(shape, dy.options());
+  const int dtype = dtype_of(dy);
+  const wc_linear_desc d = {dy.numel() / K, (int)C, (int)K, dtype, activation, 0};
+  const wc_linear_gradients g = {dy.data_ptr(), nullptr, nullptr, w.data_ptr(), data_or_null(z), nullptr, dx.data_ptr(), nullptr, dtype, nullptr, dtype, nullptr};
+  size_t bytes = 0;
+  check(wc_linear_backward_workspace_bytes(&d, &g, &bytes));
+  void* stream = stream_of(dy);
+  at::Tensor ws;
+  if (bytes) ws = workspace_for(dy, bytes, stream);
+  {
+    py::gil_scoped_release nogil;
+    check(wc_linear_backward(&d, &g, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  }
+  return py::cast(dx);
 }
 
 // ---- joins of blocks to their stream (residual.py): None, as above, for operands that do not fit together
@@ -1492,6 +1523,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"));
   m.def("norm_forward", &norm_forward);
   m.def("join_forward", &join_forward);
+  m.def("linear4_backward", &linear4_backward);
   m.def("join_backward", &join_backward);
   m.def("version", []() { return std::string(wc_version()); });
 }

@@ -128,6 +128,10 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     the activation; without an activation that is dy itself.  x may be None without need_dw, w without need_dx.  w may be a Packed4, whose values
     are read in dy's type."""
     act = _activation(activation)
+    if isinstance(w, Packed4) and engine.USE_EXT and need_dx and not (need_dw or need_db or need_dz or isinstance(z, Packed8)):
+        dx = engine._ext.linear4_backward(dy, w.codes, w.scales, w.channels, z, act)
+        if dx is not None:
+            return dx, None, None, None
     dtype, device = dy.dtype, dy.device
     if dy.dim() < 1 or not dy.shape[-1]:
         raise ValueError("dy of shape %r: expected (..., K)" % (tuple(dy.shape),))

@@ -175,6 +175,24 @@ def test_gradients(dev, host_layer, act, shape):
             lo.within(v, *want[name], "%s %s" % (name, act))
 
 
+@pytest.mark.parametrize("act", lo.ACTS)
+def test_gradient_of_x_alone(dev, host_layer, act):
+    for lead, C, K, t in [((1,), 96, 8, torch.float16), ((3, 2), 33, 65, torch.bfloat16), ((2, 70), 300, 129, torch.float32), ((513,), 1000, 40, torch.bfloat16)]:
+        g = torch.Generator().manual_seed(C)
+        w, dy, z = torch.randn(K, C, generator=g), torch.randn(*lead, K, generator=g).to(t), torch.randn(*lead, K, generator=g).to(t)
+        w4 = packed4.pack4(w.cuda())
+        W = po.values(*po.pack(w), C).to(t).double()
+        want = lo.backward(dy.reshape(-1, K), torch.zeros(dy.numel() // K, C, dtype=t), W, z.reshape(-1, K), act)["dx"]
+        odd = torch.empty(dy.numel() + 1, dtype=t, device=dev)[1:].view(dy.shape).copy_(dy.cuda())
+        wide = torch.empty(*lead, 2 * K, dtype=t, device=dev)[..., ::2].copy_(dy.cuda())
+        for given in (dy.cuda(), odd, wide):
+            dx, dw, db, dz = matrix_linear.linear_backward(given, None, w4, z.cuda(), act, need_dw=False, need_db=False)
+            assert dx.shape == lead + (C,) and dx.dtype == t and dx.is_contiguous() and dw is None and db is None and dz is None
+            lo.within(dx.reshape(-1, C), *want, "dx")
+        with pytest.raises(ValueError, match="weight"):
+            matrix_linear.linear_backward(dy.cuda()[..., :-1].contiguous(), None, w4, z.cuda()[..., :-1].contiguous(), act, need_dw=False, need_db=False)
+
+
 def test_strides_and_starts(dev, host_layer):
     g = torch.Generator().manual_seed(1)
     base = torch.randn(50, 203, generator=g).bfloat16().cuda()
