@@ -35,7 +35,9 @@ void join_plan(JoinGradients* g) {
   const int held = g->post.kind || g->gate_rows == kGateRow ? 8 : g->pre.kind && (g->gate_rows || !g->s) ? 12 : 16;
   // (long rows: parts of at most 256 MB a sum)
   const long long most = t.vectors == 0 ? std::max(1ll, std::min<long long>(kCus, (64ll << 20) / g->C)) : kCus * std::max(1, held / (t.waves == 1 ? 4 : t.waves));
-  const long long wanted = std::max(1ll, std::min(most, ceil_div_ll(g->rows, 2 * teams)));
+  // (more than four a compute unit only with eight rows each: a second row of parts costs more than it spreads; us, layer norm of 4096 x 1024 bf16, 2048 | 1024
+  // workgroups 23.4 | 18.1, 8192 x 1024 24.5 | 21.8, 32768 x 1024 57 with 2048)
+  const long long wanted = std::max(1ll, std::min(most, std::max(std::min(4ll * kCus, ceil_div_ll(g->rows, 2 * teams)), ceil_div_ll(g->rows, 8 * teams))));
   g->parts = (int)std::max(1ll, std::min(wanted / g->segments, ceil_div_ll(length, teams)));
   g->blocks = (int)std::min<long long>(g->segments * g->parts, most);
 }
@@ -60,13 +62,19 @@ __global__ __launch_bounds__(1024) void join_sums_kernel(SumsArgs a, long long f
   const float* const from = s.part + b * s.parts * a.C + c;
   float u = 0.f;
   int r = lane;
-  for (; r + 96 < s.parts; r += 128) {
-    float v[4];
+  // (sixteen on their way at a time: there may be a few workgroups alone, and a thousand parts)
+  auto some = [&](auto n) {
+    constexpr int N = decltype(n)::value;
+    for (; r + 32 * (N - 1) < s.parts; r += 32 * N) {
+      float v[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = from[(long long)(r + 32 * i) * a.C];
+      for (int i = 0; i < N; ++i) v[i] = from[(long long)(r + 32 * i) * a.C];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u += v[i];
-  }
+      for (int i = 0; i < N; ++i) u += v[i];
+    }
+  };
+  some(ic<16>{});
+  some(ic<4>{});
   for (; r < s.parts; r += 32) u += from[(long long)r * a.C];
   t[lane][col] = u;
   __syncthreads();
