@@ -419,6 +419,9 @@ int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x,
 int wc_linear4_workspace_bytes(const wc_linear_desc* desc, int x_packed, size_t* bytes);
 int wc_linear4_forward(const wc_linear_desc* desc, const void* x, const wc_packed4* x4, const wc_packed4* w, const void* bias, const void* residual, void* y,
                        void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients of that layer for an x as it is, those of wc_linear_backward: w of the gradients is null, and the packed one read in the operands' type.  rows > 0. */
+int wc_linear4_backward_workspace_bytes(const wc_linear_desc* desc, const wc_linear_gradients* gradients, size_t* bytes);   /* goes by which pointers are null */
+int wc_linear4_backward(const wc_linear_desc* desc, const wc_linear_gradients* gradients, const wc_packed4* w, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Joins of a block to its stream, over rows of channels (no counterpart in the reference):
  *   n = post(f),  d = drop(n),  s = stream_scale x + block_scale gate d,  y = pre(s)

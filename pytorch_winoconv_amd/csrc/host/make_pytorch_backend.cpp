@@ -703,14 +703,14 @@ py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const Mayb
   return keep_z ? py::object(py::make_tuple(y, z)) : py::cast(y);
 }
 
-// operands that the Python layer has checked; rows > 0
-py::tuple linear_backward(const at::Tensor& dy_, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w_, const MaybeTensor& z, const MaybeTensor& z_exp,
-                          int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, const py::object& w_type, const py::object& b_type) {
+// operands that the Python layer has checked; rows > 0.  w as it is, or codes and scales of a Packed4
+py::tuple gradients_of(const at::Tensor& dy_, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w_, const MaybeTensor& codes, const MaybeTensor& scales,
+                       const MaybeTensor& z, const MaybeTensor& z_exp, int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, at::ScalarType wt,
+                       at::ScalarType bt) {
   const c10::DeviceGuard guard(dy_.device());
   const at::Tensor dy = packed_rows(dy_);
   const MaybeTensor w = packed_rows(w_);
   const int64_t nd = dy.dim(), K = dy.size(nd - 1);
-  const at::ScalarType wt = torch::python::detail::py_object_to_dtype(w_type), bt = torch::python::detail::py_object_to_dtype(b_type);
   at::DimVector shape(dy.sizes());
   shape[nd - 1] = C;
   at::Tensor dx, dw, db, dz;
@@ -724,16 +724,25 @@ py::tuple linear_backward(const at::Tensor& dy_, const MaybeTensor& x, const May
   const wc_linear_desc d = {dy.numel() / K, C, (int)K, dtype, activation, 0};
   const wc_linear_gradients g = {dy.data_ptr(), data_or_null(x), exps(x_exp), data_or_null(w), data_or_null(z), exps(z_exp), at_or_null(dx), at_or_null(dw),
                                  wt == at::kFloat ? WC_F32 : dtype, at_or_null(db), bt == at::kFloat ? WC_F32 : dtype, at_or_null(dz)};
+  const wc_packed4 w4 = codes ? wc_packed4{codes->data_ptr<uint8_t>(), scales->data_ptr<uint8_t>()} : wc_packed4{nullptr, nullptr};
   size_t bytes = 0;
-  check(wc_linear_backward_workspace_bytes(&d, &g, &bytes));
+  check(codes ? wc_linear4_backward_workspace_bytes(&d, &g, &bytes) : wc_linear_backward_workspace_bytes(&d, &g, &bytes));
   void* stream = stream_of(dy);
   at::Tensor ws;
   if (bytes) ws = workspace_for(dy, bytes, stream);
   {
     py::gil_scoped_release nogil;
-    check(wc_linear_backward(&d, &g, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+    void* const at = bytes ? ws.data_ptr() : nullptr;
+    check(codes ? wc_linear4_backward(&d, &g, &w4, at, bytes, stream) : wc_linear_backward(&d, &g, at, bytes, stream));
   }
   return py::make_tuple(or_none(dx), or_none(dw), or_none(db), or_none(dz));
+}
+
+py::tuple linear_backward(const at::Tensor& dy, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w, const MaybeTensor& z, const MaybeTensor& z_exp,
+                          int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, const py::object& w_type, const py::object& b_type,
+                          const MaybeTensor& codes, const MaybeTensor& scales) {
+  return gradients_of(dy, x, x_exp, w, codes, scales, z, z_exp, C, activation, need_dx, need_dw, need_db, need_dz, torch::python::detail::py_object_to_dtype(w_type),
+                      torch::python::detail::py_object_to_dtype(b_type));
 }
 
 py::object pack8(const at::Tensor& x_, int keep_sign) {
@@ -789,20 +798,17 @@ py::object pack4(const at::Tensor& x_) {
 }
 
 // codes and scales of a Packed4 with elements
-at::Tensor widened4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, at::ScalarType type) {
+at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
   const c10::DeviceGuard guard(codes.device());
   at::DimVector shape(codes.sizes());
   shape[shape.size() - 1] = C;
-  at::Tensor x = at::empty(shape, codes.options().dtype(type));
+  at::Tensor x = at::empty(shape, codes.options().dtype(torch::python::detail::py_object_to_dtype(type)));
   void* stream = stream_of(codes);
   {
     py::gil_scoped_release nogil;
     check(wc_unpack4(bytes_of(codes), bytes_of(scales), x.data_ptr(), x.numel() / C, (int)C, dtype_of(x), stream));
   }
   return x;
-}
-at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
-  return widened4(codes, scales, C, torch::python::detail::py_object_to_dtype(type));
 }
 
 // x as it is, or the codes and scales of a Packed4 that reads as `type`; codes and scales of w (K, C)
@@ -838,31 +844,14 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
 }
 
 // dx alone of a layer over a Packed4 w (K, C)
-py::object linear4_backward(const at::Tensor& dy_, const at::Tensor& w_codes, const at::Tensor& w_scales, int64_t C, const MaybeTensor& z_, int activation) {
-  const int64_t nd = dy_.dim();
-  if (!linear_type(dy_) || nd < 1 || dy_.numel() == 0 || w_codes.numel() == 0 || w_codes.dim() != 2 || w_codes.size(0) != dy_.size(nd - 1) || w_codes.device() != dy_.device() || !fits(C) ||
-      !fits(w_codes.size(0)) || (activation && (!z_ || !same_kind(z_, dy_) || z_->sizes() != dy_.sizes())))
+py::object linear4_backward(const at::Tensor& dy, const at::Tensor& w_codes, const at::Tensor& w_scales, int64_t C, const MaybeTensor& z_, int activation) {
+  const int64_t nd = dy.dim();
+  if (!linear_type(dy) || nd < 1 || dy.numel() == 0 || w_codes.numel() == 0 || w_codes.dim() != 2 || w_codes.size(0) != dy.size(nd - 1) || w_codes.device() != dy.device() || !fits(C) ||
+      !fits(w_codes.size(0)) || (activation && (!z_ || !same_kind(z_, dy) || z_->sizes() != dy.sizes())))
     return py::none();
-  const c10::DeviceGuard guard(dy_.device());
-  const at::Tensor dy = packed_rows(dy_), w = widened4(w_codes, w_scales, C, dy.scalar_type());
-  const MaybeTensor z = activation ? packed_rows(z_) : MaybeTensor();
-  at::DimVector shape(dy.sizes());
-  const int64_t K = shape[nd - 1];
-  shape[nd - 1] = C;
-  at::Tensor dx = at::empty(shape, dy.options());
-  const int dtype = dtype_of(dy);
-  const wc_linear_desc d = {dy.numel() / K, (int)C, (int)K, dtype, activation, 0};
-  const wc_linear_gradients g = {dy.data_ptr(), nullptr, nullptr, w.data_ptr(), data_or_null(z), nullptr, dx.data_ptr(), nullptr, dtype, nullptr, dtype, nullptr};
-  size_t bytes = 0;
-  check(wc_linear_backward_workspace_bytes(&d, &g, &bytes));
-  void* stream = stream_of(dy);
-  at::Tensor ws;
-  if (bytes) ws = workspace_for(dy, bytes, stream);
-  {
-    py::gil_scoped_release nogil;
-    check(wc_linear_backward(&d, &g, bytes ? ws.data_ptr() : nullptr, bytes, stream));
-  }
-  return py::cast(dx);
+  const c10::DeviceGuard guard(dy.device());
+  const MaybeTensor none, z = activation ? packed_rows(z_) : none;
+  return gradients_of(dy, none, none, none, w_codes, w_scales, z, none, (int)C, activation, true, false, false, false, dy.scalar_type(), dy.scalar_type())[0];
 }
 
 // ---- joins of blocks to their stream (residual.py): None, as above, for operands that do not fit together
@@ -1514,7 +1503,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_forward", &linear_forward, py::arg("x"), py::arg("w"), py::arg("bias"), py::arg("residual"), py::arg("activation"),
         py::arg("residual_after"), py::arg("keep_z"));
   m.def("linear_backward", &linear_backward, py::arg("dy"), py::arg("x"), py::arg("x_exponents"), py::arg("w"), py::arg("z"), py::arg("z_exponents"), py::arg("C"),
-        py::arg("activation"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"), py::arg("need_dz"), py::arg("w_type"), py::arg("b_type"));
+        py::arg("activation"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"), py::arg("need_dz"), py::arg("w_type"), py::arg("b_type"),
+        py::arg("codes") = py::none(), py::arg("scales") = py::none());
   m.def("pack8", &pack8, py::arg("x"), py::arg("keep_sign"));
   m.def("unpack8", &unpack8, py::arg("codes"), py::arg("exponents"), py::arg("type"));
   m.def("pack4", &pack4, py::arg("x"));

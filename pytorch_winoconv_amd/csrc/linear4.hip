@@ -54,6 +54,38 @@ LinearProduct tiled(LinearProduct p) {
   return p;
 }
 
+// What a backward pass leaves to wc_linear_backward, and what goes where in the workspace.  Up to kMostGradient4 rows dx is a pass over the packed weight, and dz and all
+// else are the other's; above, the weight is widened first
+struct Backward4 { bool few, inner; wc_linear_gradients g; const void* dz; void* wide; float* parts; size_t inner_at, bytes; };
+int backward4_plan(const wc_linear_desc* d, const wc_linear_gradients* g, void* workspace, Backward4* b) {
+  // (sizes go by which pointers are null)
+  char* const ws = workspace ? static_cast<char*>(workspace) : reinterpret_cast<char*>(256);
+  const size_t size = d->dtype == WC_F32 ? 4 : 2;
+  size_t at = 0;
+  auto take = [&](size_t n) { char* p = ws + at; at += rounded(n); return p; };
+  *b = {};
+  b->g = *g;
+  b->few = g->dx && d->rows <= kMostGradient4;
+  if (b->few) {
+    b->g.dx = nullptr;
+    b->g.w = nullptr;
+    if (d->activation != WC_ACT_NONE && !g->dz) b->g.dz = take((size_t)d->rows * d->K * size);
+    b->dz = d->activation != WC_ACT_NONE ? b->g.dz : g->dy;
+    const int s = linear4_gradient_parts(d->K, d->C);
+    if (s > 1) b->parts = reinterpret_cast<float*>(take((size_t)s * d->rows * d->C * 4));
+  } else if (g->dx) {
+    b->wide = take((size_t)d->K * d->C * size);
+    b->g.w = b->wide;
+  }
+  b->inner = b->g.dx || b->g.dw || b->g.db || b->g.dz;
+  b->inner_at = b->bytes = at;
+  if (!b->inner) return WC_OK;
+  size_t inner = 0;
+  if (int rc = wc_linear_backward_workspace_bytes(d, &b->g, &inner)) return rc;
+  b->bytes += inner;
+  return WC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -150,6 +182,39 @@ int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4*
   const size_t wide_bytes = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2));
   if (int rc = unpack4(w.codes, w.scales, ws, d->K, d->C, d->dtype, stream)) return rc;
   return wc_linear_forward(d, x, ws, bias, residual, y, nullptr, ws + wide_bytes, need - wide_bytes, stream);
+}
+
+int wc_linear4_backward_workspace_bytes(const wc_linear_desc* d, const wc_linear_gradients* g, size_t* bytes) {
+  WC_CHECK_ARG(bytes != nullptr && g != nullptr, "wc_linear4_backward_workspace_bytes: null pointer");
+  if (int rc = check_desc4(d, "wc_linear4_backward_workspace_bytes")) return rc;
+  *bytes = 0;
+  if (d->rows == 0) return WC_OK;
+  Backward4 b;
+  if (int rc = backward4_plan(d, g, nullptr, &b)) return rc;
+  *bytes = b.bytes;
+  return WC_OK;
+}
+
+int wc_linear4_backward(const wc_linear_desc* d, const wc_linear_gradients* g, const wc_packed4* w4, void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  if (int rc = wc_linear4_backward_workspace_bytes(d, g, &need)) return rc;
+  WC_CHECK_ARG(d->rows > 0, "wc_linear4_backward: no rows (the gradients of the parameters are zero)");
+  WC_CHECK_ARG(g->dy, "wc_linear4_backward: dy is null");
+  WC_CHECK_ARG(!g->w, "wc_linear4_backward: w is given packed");
+  WC_CHECK_ARG(d->activation == WC_ACT_NONE || g->z, "wc_linear4_backward: an activation's gradient needs z");
+  if (g->dx)
+    if (int rc = check_packed(w4, "w", "wc_linear4_backward")) return rc;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(WC_ERR_WORKSPACE, "wc_linear4_backward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(WC_ERR_WORKSPACE, "wc_linear4_backward: workspace must be 256-byte aligned");
+  Backward4 b;
+  if (int rc = backward4_plan(d, g, workspace, &b)) return rc;
+  if (b.wide)
+    if (int rc = unpack4(w4->codes, w4->scales, b.wide, d->K, d->C, d->dtype, stream)) return rc;
+  if (b.inner)
+    if (int rc = wc_linear_backward(d, &b.g, need ? static_cast<char*>(workspace) + b.inner_at : nullptr, need - b.inner_at, stream)) return rc;
+  if (!b.few) return WC_OK;
+  return linear4_gradient(b.dz, {w4->codes, w4->scales}, g->dx, b.parts, d->rows, d->K, d->C, d->dtype, stream);
 }
 
 }  // extern "C"

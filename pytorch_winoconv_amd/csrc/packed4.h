@@ -57,6 +57,10 @@ int unpack4(const unsigned char* codes, const unsigned char* scales, void* x, lo
 struct Operand4 { const unsigned char* codes; const unsigned char* scales; };
 // linear4_few.hip: at most 16 rows of x, a pass over w
 int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, int dtype, void* stream);
+// linear4_gradient.hip: dx = dz w of at most 32 rows of dz, a pass over w (K, C); parts: (linear4_gradient_parts, M, C), where those are more than one
+constexpr int kMostGradient4 = 32;
+int linear4_gradient_parts(long long K, long long C);
+int linear4_gradient(const void* dz, const Operand4& w, void* dx, float* parts, long long M, int K, int C, int dtype, void* stream);
 // linear4_wide.hip: more rows of 16-bit x (rows of whole 16 bytes), w's codes widened in the registers.  R_part of its plan is in stages
 constexpr int kMostWide4 = 2048;
 bool linear4_wide_fits(const void* x, long long C, int dtype);

@@ -157,8 +157,7 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     if not dy.is_cuda:
         raise ValueError("winoconv runs on the GPU only: got a %s tensor" % device)
     engine._require_gpu(dy)
-    if isinstance(w, Packed4):
-        w = unpack4(w, dtype) if need_dx and dy.numel() else None
+    packed, w = (w if need_dx else None, None) if isinstance(w, Packed4) else (None, w)
     w_type, b_type = w_type or dtype, b_type or dtype
     w_own, b_own = (t if t == torch.float32 else dtype for t in (w_type, b_type))
     if need_dz and not act:
@@ -177,7 +176,7 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     (x_data, x_exp), (z_data, z_exp) = split(x), split(z)
     if engine.USE_EXT:
         dx, dw, db, own_dz = engine._ext.linear_backward(dy, x_data, x_exp, w, z_data, z_exp, C, act, bool(need_dx), bool(need_dw), bool(need_db),
-                                                         bool(need_dz), w_own, b_own)
+                                                         bool(need_dz), w_own, b_own, *((None, None) if packed is None else (packed.codes, packed.scales)))
     else:
         dy, w = _contiguous(dy), _contiguous(w)
         dx = new(lead + (C,), dtype) if need_dx else None
@@ -188,10 +187,11 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
         lib, d, nbytes = _lib.load(), _desc(rows, C, K, dtype, act), ctypes.c_size_t()
         g = LinearGradients(at(dy), at(x_data), at(x_exp), at(w), at(z_data), at(z_exp), at(dx), at(dw), engine._DTYPES[w_own], at(db),
                             engine._DTYPES[b_own], at(own_dz))
-        check(lib.wc_linear_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(g), ctypes.byref(nbytes)))
+        name, w4 = ("wc_linear_backward", ()) if packed is None else ("wc_linear4_backward", (ctypes.byref(packed._pointers()),))
+        check(getattr(lib, name + "_workspace_bytes")(ctypes.byref(d), ctypes.byref(g), ctypes.byref(nbytes)))
         ws = new((nbytes.value,), torch.uint8)
         with engine._on_device(dy):
-            check(lib.wc_linear_backward(ctypes.byref(d), ctypes.byref(g), engine._ptr(ws), nbytes.value, engine._stream(dy)))
+            check(getattr(lib, name)(ctypes.byref(d), ctypes.byref(g), *w4, engine._ptr(ws), nbytes.value, engine._stream(dy)))
     return (dx, dw if dw is None or w_type == w_own else dw.to(w_type), db if db is None or b_type == b_own else db.to(b_type),
             dz if own_dz is None else own_dz)
 

@@ -177,7 +177,10 @@ def test_gradients(dev, host_layer, act, shape):
 
 @pytest.mark.parametrize("act", lo.ACTS)
 def test_gradient_of_x_alone(dev, host_layer, act):
-    for lead, C, K, t in [((1,), 96, 8, torch.float16), ((3, 2), 33, 65, torch.bfloat16), ((2, 70), 300, 129, torch.float32), ((513,), 1000, 40, torch.bfloat16)]:
+    # a pass over the packed weight (up to 32 rows), in one part and several, and the weight widened
+    for lead, C, K, t in [((1,), 96, 8, torch.float16), ((3, 2), 33, 65, torch.bfloat16), ((2, 70), 300, 129, torch.float32), ((513,), 1000, 40, torch.bfloat16),
+                          ((8,), 17001, 100, torch.bfloat16), ((16,), 516, 4100, torch.float16), ((17,), 131, 517, torch.float32), ((32,), 1, 1, torch.float16),
+                          ((2, 9), 129, 31, torch.bfloat16), ((4,), 520, 1024, torch.float32), ((33,), 64, 64, torch.bfloat16), ((31,), 16500, 256, torch.float32)]:
         g = torch.Generator().manual_seed(C)
         w, dy, z = torch.randn(K, C, generator=g), torch.randn(*lead, K, generator=g).to(t), torch.randn(*lead, K, generator=g).to(t)
         w4 = packed4.pack4(w.cuda())
@@ -189,8 +192,28 @@ def test_gradient_of_x_alone(dev, host_layer, act):
             dx, dw, db, dz = matrix_linear.linear_backward(given, None, w4, z.cuda(), act, need_dw=False, need_db=False)
             assert dx.shape == lead + (C,) and dx.dtype == t and dx.is_contiguous() and dw is None and db is None and dz is None
             lo.within(dx.reshape(-1, C), *want, "dx")
-        with pytest.raises(ValueError, match="weight"):
+        with pytest.raises(ValueError, match="weight|dy of shape"):
             matrix_linear.linear_backward(dy.cuda()[..., :-1].contiguous(), None, w4, z.cuda()[..., :-1].contiguous(), act, need_dw=False, need_db=False)
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_gradients_of_few_rows(dev, host_layer, act):
+    """dx from the packed weight, and beside it the gradients of the bias and of the residual."""
+    for rows, C, K, t in [(8, 260, 72, torch.float16), (20, 1000, 600, torch.bfloat16), (3, 40, 33, torch.float32)]:
+        g = torch.Generator().manual_seed(K)
+        w, dy, z = torch.randn(K, C, generator=g), torch.randn(rows, K, generator=g).to(t), torch.randn(rows, K, generator=g).to(t)
+        w4, x = packed4.pack4(w.cuda()), torch.randn(rows, C, generator=g).to(t)
+        want = lo.backward(dy, x, po.values(*po.pack(w), C).to(t).double(), z, act)
+        got = matrix_linear.linear_backward(dy.cuda(), x.cuda(), w4, z.cuda(), act, need_dz=True)
+        for name, v in zip(("dx", "dw", "db", "dz"), got):
+            lo.within(v, *want[name], name)
+        # a NaN, of dz or as a group of the weight, is a NaN of its row or group alone
+        dy[1, 5] = float("nan")
+        w4.scales[0, 0, 7, 0] = 255
+        dx = matrix_linear.linear_backward(dy.cuda(), None, w4, z.cuda(), act, need_dw=False, need_db=False)[0].cpu()
+        bad = torch.zeros(rows, C, dtype=torch.bool)
+        bad[1], bad[:, :32] = True, True
+        assert torch.equal(dx.isnan(), bad)
 
 
 def test_strides_and_starts(dev, host_layer):
