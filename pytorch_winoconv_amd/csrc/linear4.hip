@@ -54,7 +54,7 @@ LinearProduct tiled(LinearProduct p) {
   return p;
 }
 
-// What a backward pass leaves to wc_linear_backward, and what goes where in the workspace.  Up to kMostGradient4 rows dx is a pass over the packed weight, and dz and all
+// What a backward pass leaves to wc_linear_backward, and what goes where in the workspace.  Up to most_gradient4 rows dx is passes over the packed weight, and dz and all
 // else are the other's; above, the weight is widened first
 struct Backward4 { bool few, inner; wc_linear_gradients g; const void* dz; void* wide; float* parts; size_t inner_at, bytes; };
 int backward4_plan(const wc_linear_desc* d, const wc_linear_gradients* g, void* workspace, Backward4* b) {
@@ -65,13 +65,13 @@ int backward4_plan(const wc_linear_desc* d, const wc_linear_gradients* g, void* 
   auto take = [&](size_t n) { char* p = ws + at; at += rounded(n); return p; };
   *b = {};
   b->g = *g;
-  b->few = g->dx && d->rows <= kMostGradient4;
+  b->few = g->dx && d->rows <= most_gradient4(d->dtype);
   if (b->few) {
     b->g.dx = nullptr;
     b->g.w = nullptr;
     if (d->activation != WC_ACT_NONE && !g->dz) b->g.dz = take((size_t)d->rows * d->K * size);
     b->dz = d->activation != WC_ACT_NONE ? b->g.dz : g->dy;
-    const int s = linear4_gradient_parts(d->K, d->C);
+    const int s = linear4_gradient_parts(d->rows, d->K, d->C, d->dtype);
     if (s > 1) b->parts = reinterpret_cast<float*>(take((size_t)s * d->rows * d->C * 4));
   } else if (g->dx) {
     b->wide = take((size_t)d->K * d->C * size);

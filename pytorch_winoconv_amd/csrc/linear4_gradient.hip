@@ -1,10 +1,11 @@
-// dx = dz w of few rows over a weight in 4 bits (packed4.h): a pass over the weight, which bounds it, where widening it first writes and reads four times its bytes.
+// dx = dz w over a weight in 4 bits (packed4.h): a pass over the codes, which bounds it for few rows, where widening them first writes and reads four times their bytes.
 //
 // A wavefront takes 32 rows of w by a stage of 128 channels: a lane eight rows by the eight channels of a word.  Its 64 values, widened to the type of dz, turn
 // about in the registers into eight operands of 16 x 16 x 32 instructions, each a channel's eight rows, for eight neighbouring elements of a row of dz; fp32 dz is
 // taken as the three bf16 numbers that it is the sum of.  The wavefronts of a workgroup share the rows of w, and their sums meet in LDS; where the channels
-// give too few workgroups the rows are shared among several, whose parts are joined in a fixed order.
-// us, the weight widened first | this: fp16 1 x 4096 <- 4096 33 | 8.4, 8 x 25088 <- 4096 108 | 16 (3.2 TB/s of codes), 7 x 15435 <- 5920 266 | 19, 32 x 8192 <- 8192 67 | 18.5.
+// give too few workgroups the rows are shared among several, whose parts are joined in a fixed order.  A pass takes 16 MB rows of dz; more are passes of the same launch, side by side.
+// us, the weight widened first | this: fp16 1 x 4096 <- 4096 33 | 8.2, 8 x 25088 <- 4096 108 | 16 (3.3 TB/s of codes), 7 x 15435 <- 5920 266 | 19, 32 x 8192 <- 8192
+// 67 | 18.5, 512 133 | 97; fp32 16 x 8192 <- 8192 173 | 18, 4096 4219 | 1674.
 #include "linear4_rows.h"
 
 #include <algorithm>
@@ -39,9 +40,10 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_gradient_kernel(GradientA
   const int begin = (int)s * g.steps_part, end = min(g.steps, begin + g.steps_part), whole = min(end, g.K / kStep);
   const unsigned char* const codes = g.w.codes + stage * (kStage4 / 2) + r * 4;
   const unsigned char* const scales = g.w.scales + stage * (kRows4 * 4) + kg * 32;
+  const long long m0 = (long long)blockIdx.y * (16 * MB);
   long long from[MB];                      // (rows behind the last give results that go nowhere)
 #pragma unroll
-  for (int i = 0; i < MB; ++i) from[i] = min((long long)(i * 16 + r), g.M - 1) * g.K;
+  for (int i = 0; i < MB; ++i) from[i] = min(m0 + i * 16 + r, g.M - 1) * g.K;
   f32x4 acc[MB][8];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_gradient_kernel(GradientA
   // register e of a lane, operand j: channel 8 (4 kg + e) + j, row r of dz.  Chunks of four channels are exchanged by the row, so that rows are in different banks
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
-    if (i * 16 >= g.M) break;
+    if (m0 + i * 16 >= g.M) break;
     if (i) __syncthreads();
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -104,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_gradient_kernel(GradientA
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) t += *reinterpret_cast<const f32x4*>(&sums[w][row][(chunk ^ row * 2) * 4]);
-    const long long m = i * 16 + row;
+    const long long m = m0 + i * 16 + row;
     const int c = (int)stage * kStage4 + chunk * 4, have = m < g.M ? max(min(g.C - c, 4), 0) : 0;
     if (g.parts) {
       const float o[4] = {t[0], t[1], t[2], t[3]};
@@ -118,16 +120,20 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_gradient_kernel(GradientA
 
 }  // namespace
 
-// Parts: four workgroups to a compute unit where the rows of w have a step for every wavefront; one where the channels alone give half of one a unit
-int linear4_gradient_parts(long long K, long long C) {
-  const long long tiles = stages4(C), steps = ceil_div_ll(K, kStep);
+// Rows of dz that a workgroup takes: fp32 ones, of three parts, leave no registers for more than 32
+static int rows_of_pass(long long M, int dtype) { return M <= 16 ? 16 : M <= 32 || dtype == WC_F32 ? 32 : 64; }
+
+// Parts: two workgroups to a compute unit where the rows of w have a step for every wavefront; one where there is one for half of the units anyway; of more than 2 MB
+// no more bytes than the codes (us, fp16 64 x 4096 <- 4096 in 8 and 4 parts 24 | 17, 384 x 2048 <- 1000 in 3 and one 21 | 11)
+int linear4_gradient_parts(long long M, long long K, long long C, int dtype) {
+  const long long tiles = stages4(C) * ceil_div_ll(M, rows_of_pass(M, dtype)), steps = ceil_div_ll(K, kStep);
   if (tiles >= kCus / 2) return 1;
-  return (int)std::max(1ll, std::min(ceil_div_ll(2 * kCus, tiles), steps / kWaves));
+  return (int)std::max(1ll, std::min({ceil_div_ll(2 * kCus, tiles), steps / kWaves, std::max(K / (16 * M), (1ll << 19) / (M * C))}));
 }
 
 int linear4_gradient(const void* dz, const Operand4& w, void* dx, float* parts, long long M, int K, int C, int dtype, void* stream) {
   GradientArgs g = {dz, M, K, C, w, stages4(C), dx, nullptr, ceil_div(K, kStep), 0, 0, 0};
-  const int S = linear4_gradient_parts(K, C);
+  const int S = linear4_gradient_parts(M, K, C, dtype), rows = rows_of_pass(M, dtype);
   g.steps_part = ceil_div(g.steps, S);
   g.parts = S > 1 ? parts : nullptr;
   const long long blocks = g.stages * S;
@@ -135,8 +141,11 @@ int linear4_gradient(const void* dz, const Operand4& w, void* dx, float* parts, 
   g.per_xcd = ceil_div(g.n_blocks, kXcds);
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    auto fn = M <= 16 ? &linear4_gradient_kernel<T, 1> : &linear4_gradient_kernel<T, 2>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)(g.per_xcd * kXcds)), dim3(64 * kWaves), 0, as_stream(stream), g);
+    auto fn = rows == 16 ? &linear4_gradient_kernel<T, 1> : &linear4_gradient_kernel<T, 2>;
+    if constexpr (sizeof(T) == 2) {
+      if (rows == 64) fn = &linear4_gradient_kernel<T, 4>;
+    }
+    hipLaunchKernelGGL(fn, dim3((unsigned)(g.per_xcd * kXcds), (unsigned)ceil_div_ll(M, rows)), dim3(64 * kWaves), 0, as_stream(stream), g);
     WC_CHECK_LAUNCH("linear4_gradient_kernel");
     if (S == 1) return WC_OK;
     LinearJoin join = {{}, parts, S, M, C};

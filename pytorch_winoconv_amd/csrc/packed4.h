@@ -57,9 +57,11 @@ int unpack4(const unsigned char* codes, const unsigned char* scales, void* x, lo
 struct Operand4 { const unsigned char* codes; const unsigned char* scales; };
 // linear4_few.hip: at most 16 rows of x, a pass over w
 int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, int dtype, void* stream);
-// linear4_gradient.hip: dx = dz w of at most 32 rows of dz, a pass over w (K, C); parts: (linear4_gradient_parts, M, C), where those are more than one
-constexpr int kMostGradient4 = 32;
-int linear4_gradient_parts(long long K, long long C);
+// linear4_gradient.hip: dx = dz w, passes over the codes of w (K, C); parts: (linear4_gradient_parts, M, C), where those are more than one
+// us, passes of 64 rows | the weight widened first: fp16 512 rows of 8192 <- 8192 97 | 133, of 25088 <- 4096 176 | 176; fp32, whose three bf16 products are faster than
+// one of fp32 operands, passes of 32: 4096 rows 1674 | 4219 and 2747 | 6580 (2^20: a launch's passes)
+inline int most_gradient4(int dtype) { return dtype == WC_F32 ? 1 << 20 : 512; }
+int linear4_gradient_parts(long long M, long long K, long long C, int dtype);
 int linear4_gradient(const void* dz, const Operand4& w, void* dx, float* parts, long long M, int K, int C, int dtype, void* stream);
 // linear4_wide.hip: more rows of 16-bit x (rows of whole 16 bytes), w's codes widened in the registers.  R_part of its plan is in stages
 constexpr int kMostWide4 = 2048;

@@ -177,10 +177,10 @@ def test_gradients(dev, host_layer, act, shape):
 
 @pytest.mark.parametrize("act", lo.ACTS)
 def test_gradient_of_x_alone(dev, host_layer, act):
-    # a pass over the packed weight (up to 32 rows), in one part and several, and the weight widened
+    # passes over the packed weight (up to 512 rows, of fp32 all), in one part and several, and the weight widened
     for lead, C, K, t in [((1,), 96, 8, torch.float16), ((3, 2), 33, 65, torch.bfloat16), ((2, 70), 300, 129, torch.float32), ((513,), 1000, 40, torch.bfloat16),
                           ((8,), 17001, 100, torch.bfloat16), ((16,), 516, 4100, torch.float16), ((17,), 131, 517, torch.float32), ((32,), 1, 1, torch.float16),
-                          ((2, 9), 129, 31, torch.bfloat16), ((4,), 520, 1024, torch.float32), ((33,), 64, 64, torch.bfloat16), ((31,), 16500, 256, torch.float32)]:
+                          ((2, 9), 129, 31, torch.bfloat16), ((4,), 520, 1024, torch.float32), ((33,), 64, 64, torch.bfloat16), ((64,), 700, 333, torch.float16), ((100,), 300, 129, torch.float32), ((128,), 520, 300, torch.float32), ((512,), 129, 96, torch.float16), ((700,), 1000, 40, torch.float16), ((1000,), 257, 65, torch.float32), ((200,), 2048, 777, torch.bfloat16), ((31,), 16500, 256, torch.float32)]:
         g = torch.Generator().manual_seed(C)
         w, dy, z = torch.randn(K, C, generator=g), torch.randn(*lead, K, generator=g).to(t), torch.randn(*lead, K, generator=g).to(t)
         w4 = packed4.pack4(w.cuda())
