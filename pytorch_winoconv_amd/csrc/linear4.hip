@@ -43,7 +43,11 @@ LinearProduct product_of(const wc_linear_desc* d, const void* x, const void* bia
 
 // A pass over the packed weight, whose workgroups read x anew for every 16 of its rows, up to 8 rows, and up to 16 over a weight of up to 2^25 values.  us, fp16, the pass | tiles:
 // 16 x 4096 -> 4096 7.6 | 10, 16 x 8192 -> 8192 23.8 | 20.2, 16 x 25088 -> 4096 33 | 26
-bool few(const wc_linear_desc* d) { return d->rows <= 8 || (d->rows <= 16 && (long long)d->C * d->K <= 1ll << 25); }
+// fp32 rows, whose other way widens the weight and multiplies fp32 operands, are taken 16 at a time beside each other (us, passes | widened: 16 x 8192 -> 8192
+// 42 | 179, 128 298 | 382, 128 x 25088 -> 4096 413 | 590, 256 x 512 -> 2048 29 | 22)
+bool few(const wc_linear_desc* d, bool packed) {
+  return d->rows <= 8 || (d->rows <= 16 && (long long)d->C * d->K <= 1ll << 25) || (!packed && d->dtype == WC_F32 && d->rows <= kMostFew4);
+}
 // Tiles that widen the codes in the registers, up to 2048 rows; above, and for fp32 and rows of x that are no whole 16 bytes, the weight is widened first, a launch and
 // a pass over it, for the product of its own type.  us, fp16 8192 -> 8192, tiles | widened first: 64 rows 23 | 64, 1024 128 | 182, 2048 247 | 270, 4096 509 | 499
 bool wide(const wc_linear_desc* d) { return d->rows <= kMostWide4 && linear4_wide_fits(nullptr, d->C, d->dtype); }
@@ -118,7 +122,7 @@ int wc_linear4_workspace_bytes(const wc_linear_desc* d, int x_packed, size_t* by
   WC_CHECK_ARG(bytes != nullptr, "wc_linear4_workspace_bytes: null output");
   if (int rc = check_desc4(d, "wc_linear4_workspace_bytes")) return rc;
   *bytes = 0;
-  if (d->rows == 0 || few(d)) return WC_OK;
+  if (d->rows == 0 || few(d, x_packed != 0)) return WC_OK;
   if (x_packed) {
     // (a plan goes by whether the epilogue is heavy: the larger of both)
     LinearProduct p = tiled(product_of(d, nullptr, nullptr, nullptr, nullptr));
@@ -156,7 +160,7 @@ int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4*
   if (need && reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: workspace must be 256-byte aligned");
   const LinearProduct p = product_of(d, x, bias, residual, y);
   const Operand4 w = {w4->codes, w4->scales};
-  if (few(d)) {
+  if (few(d, x4 != nullptr)) {
     const Operand4 xp = x4 ? Operand4{x4->codes, x4->scales} : Operand4{nullptr, nullptr};
     return product4_few(p, x4 ? &xp : nullptr, w, d->dtype, stream);
   }

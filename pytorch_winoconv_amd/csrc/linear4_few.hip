@@ -1,6 +1,6 @@
 // Linear layers of few rows over a weight in 4 bits (packed4.h): a pass over the weight, half a byte and a scale's 32nd a value, which bounds it.
 //
-// A workgroup of 16 wavefronts takes NR rows of w (4, 8 or 16: as many workgroups as there are compute units, where it can be), whose reduction
+// A workgroup of 16 wavefronts takes NR rows of w and as many of x (4, 8 or 16: as many workgroups as there are compute units, where it can be), whose reduction
 // the wavefronts share, a stage of 128 channels at a time.  A lane holds a group of 32 channels of its row: 16 bytes of codes and one scale.
 // x as it is: the codes become eight values of the type of x at a time, exact, straight into the operands of 16 x 16 x 32 instructions, each
 // lane multiplying its own group (the order of the channels within a sum is free); fp32 x is taken as the three bf16 numbers that it is
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_few_kernel(FewArgs g) {
   __shared__ float sums[kWaves * PLACES][NR][NR + 1];
   const LinearProduct& p = g.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane % NR, place = (lane & 15) / NR, c = lane >> 4;
-  const long long n0 = (long long)blockIdx.x * NR, n = min(n0 + r, p.N - 1), m = min((long long)r, p.M - 1);      // (results of rows behind the last go nowhere)
+  const long long n0 = (long long)blockIdx.x * NR, n = min(n0 + r, p.N - 1), m0 = (long long)blockIdx.y * NR, m = min(m0 + r, p.M - 1);      // (results of rows behind the last go nowhere)
   const unsigned char* const codes = g.w.codes + n * g.stages * (kStage4 / 2) + c * 16;
   const unsigned char* const scales = g.w.scales + scale_at4(n, c, g.stages);
   const unsigned char* const x_codes = X4 ? g.x.codes + m * g.stages * (kStage4 / 2) + c * 16 : nullptr;
@@ -137,11 +137,11 @@ __global__ __launch_bounds__(64 * kWaves) void linear4_few_kernel(FewArgs g) {
     if ((4 * c + e) / NR == place) sums[wave * PLACES + place][r][(4 * c + e) % NR] = acc[e];
   __syncthreads();
   const int mr = threadIdx.x / NR, nr = threadIdx.x % NR;
-  if (mr >= NR || mr >= p.M || n0 + nr >= p.N) return;
+  if (mr >= NR || m0 + mr >= p.M || n0 + nr >= p.N) return;
   float v = 0.f;
 #pragma unroll 16
   for (int s = 0; s < kWaves * PLACES; ++s) v += sums[s][mr][nr];
-  finish_one<T>(p.e, mr, n0 + nr, p.N, v);
+  finish_one<T>(p.e, m0 + mr, n0 + nr, p.N, v);
 }
 
 }  // namespace
@@ -157,7 +157,7 @@ int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, i
       return nr == 4 ? &linear4_few_kernel<T, X4, 4> : nr == 8 ? &linear4_few_kernel<T, X4, 8> : &linear4_few_kernel<T, X4, 16>;
     };
     auto fn = x ? pick(std::true_type{}) : pick(std::false_type{});
-    hipLaunchKernelGGL(fn, dim3((unsigned)ceil_div_ll(p.N, nr)), dim3(64 * kWaves), 0, as_stream(stream), g);
+    hipLaunchKernelGGL(fn, dim3((unsigned)ceil_div_ll(p.N, nr), (unsigned)ceil_div_ll(p.M, nr)), dim3(64 * kWaves), 0, as_stream(stream), g);
     WC_CHECK_LAUNCH("linear4_few_kernel");
     return WC_OK;
   });

@@ -55,7 +55,8 @@ int unpack4(const unsigned char* codes, const unsigned char* scales, void* x, lo
 
 // y = act(x wT + b + r), one operand or both in 4 bits; p's a (x as it is) and b are null where they are packed
 struct Operand4 { const unsigned char* codes; const unsigned char* scales; };
-// linear4_few.hip: at most 16 rows of x, a pass over w
+// linear4_few.hip: few rows of x, a pass over w for each 16 (a call takes at most kMostFew4)
+constexpr int kMostFew4 = 128;
 int product4_few(const LinearProduct& p, const Operand4* x, const Operand4& w, int dtype, void* stream);
 // linear4_gradient.hip: dx = dz w, passes over the codes of w (K, C); parts: (linear4_gradient_parts, M, C), where those are more than one
 // us, passes of 64 rows | the weight widened first: fp16 512 rows of 8192 <- 8192 97 | 133, of 25088 <- 4096 176 | 176; fp32, whose three bf16 products are faster than
