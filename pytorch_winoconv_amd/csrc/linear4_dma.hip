@@ -6,7 +6,7 @@
 // once a stage.  The stages' 64-byte halves of L2 lines come in pairs, two pairs of buffers: while one is multiplied the other lands.
 //
 // us and PFLOP/s without an epilogue: 4096^3 41 (3.4), 8192^3 287 (3.8), 8192 x 25088 -> 4096 399 (4.2), matrix cores busy 39 % of the cycles: the wavefronts' reads of LDS, 96 of
-// its 128 bytes a cycle, and the stages' way there take as long as the instructions.  Four wavefronts of 128 x 128, which read a third less, have nobody to wait beside
+// its 128 bytes a cycle, and the stages' way there take as long as the instructions (8192^3 with that way left out 222, without the reads 253, the instructions alone 194).  Four wavefronts of 128 x 128, which read a third less, have nobody to wait beside
 // them (8192^3 300); single stages in a ring of four come at half lines of the L2 (306).
 //
 // The wavefronts each bring a share of a stage's scales, some of their lanes 16 bytes each, so that all count the same loads.

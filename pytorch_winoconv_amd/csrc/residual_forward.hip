@@ -1,5 +1,5 @@
 // s = a x + b g drop(post(f)) and y = pre(s) of residual.h, a row a team at a time: one read of f and x, one write of s and y, whatever of it there is.
-// Bound by memory: us and TB/s, fp16 layer norm of 200704 x 256 37 (5.6), bf16 RMS norm of 16384 x 4096 48 (5.6), dropout of 8192 x 8192 52 (5.2); two norms,
+// Bound by memory: us and TB/s, fp16 layer norm of 200704 x 256 37 (5.6), bf16 RMS norm of 16384 x 4096 48 (5.6), dropout of 8192 x 8192 51 (5.2; inputs from memory 59); two norms,
 // gate and dropout of 16384 x 2048 57 (4.7), whose arithmetic takes about as long.
 #include "residual.h"
 
