@@ -355,3 +355,32 @@ def test_beyond_32_bits(dev):
             want, _, bound, _ = lo.forward(X, W, None, None, "none", False)
             lo.within(y[part], want, bound)
         del y
+
+
+def test_gradients_captured_and_side_by_side(dev):
+    g = torch.Generator().manual_seed(5)
+    w4 = packed4.pack4(torch.randn(520, 300, generator=g).cuda())
+    for rows, t in [(3, torch.float16), (40, torch.bfloat16), (70, torch.float32)]:
+        z, dys = torch.randn(rows, 520, generator=g).to(t).cuda(), [torch.randn(rows, 520, generator=g).to(t).cuda() for _ in range(3)]
+        grad = lambda dy: matrix_linear.linear_backward(dy, None, w4, z, "silu", need_dw=False)  # noqa: E731
+        want = [grad(dy) for dy in dys]
+        given = dys[0].clone()
+        grad(given)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dx, _, db, _ = grad(given)
+        for dy, (dx64, _, db64, _) in zip(dys + dys[:1], want + want[:1]):
+            given.copy_(dy)
+            graph.replay()
+            other = grad(dys[1])                       # (eager work of the same shape beside the replay's results)
+            assert torch.equal(dx, dx64) and torch.equal(db, db64) and torch.equal(other[0], want[1][0])
+            torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in dys]
+        torch.cuda.synchronize()
+        got = []
+        for s, dy in zip(streams, dys):
+            with torch.cuda.stream(s):
+                got.append([grad(dy) for _ in range(3)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a[0], b[0]) and torch.equal(a[2], b[2]) for runs, b in zip(got, want) for a in runs)

@@ -120,3 +120,33 @@ def test_c_entry_points_refuse():
     assert run(at, None, ctypes.byref(w), at, ctypes.c_void_p(8), n.value) == _lib.WC_ERR_WORKSPACE
     d.K = (1 << 22) + 1
     assert lib.wc_linear4_workspace_bytes(ctypes.byref(d), 0, ctypes.byref(n)) == _lib.WC_ERR_UNSUPPORTED
+
+
+def test_c_gradients_refuse():
+    lib = _lib.load()
+    n, w = ctypes.c_size_t(), _lib.Packed4Parts(256, 256)
+    for rows, act in [(3, 0), (3, 2), (600, 0), (600, 2)]:
+        d = _lib.LinearDesc(rows, 256, 64, _lib.WC_F16, act, 0)
+        grads = lambda dy=256, w=None, z=256, dx=256, x=None, dw=None, db=None: _lib.LinearGradients(dy, x, None, w, z, None, dx, dw, _lib.WC_F16, db, _lib.WC_F32, None)  # noqa: E731,B023
+        size = lambda g: (lib.wc_linear4_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(g), ctypes.byref(n)), n.value)  # noqa: E731,B023
+        run = lambda g, w4, ws=None, size=0: lib.wc_linear4_backward(ctypes.byref(d), ctypes.byref(g), w4, ws, size, None)  # noqa: E731,B023
+        rc, need = size(grads())
+        # dz of few rows, or the weight widened
+        assert rc == 0 and need >= (0 if rows == 3 and not act else rows * 64 * 2 if rows == 3 else 64 * 256 * 2)
+        at = ctypes.c_void_p(256)
+        assert run(grads(dy=None), ctypes.byref(w), at, need) == _lib.WC_ERR_BAD_ARG
+        assert run(grads(w=256), ctypes.byref(w), at, need) == _lib.WC_ERR_BAD_ARG
+        assert run(grads(), None, at, need) == _lib.WC_ERR_BAD_ARG
+        assert run(grads(), ctypes.byref(_lib.Packed4Parts(256, 8)), at, need) == _lib.WC_ERR_BAD_ARG
+        if act:
+            assert run(grads(z=None), ctypes.byref(w), at, need) == _lib.WC_ERR_BAD_ARG
+        if need:
+            assert run(grads(), ctypes.byref(w), at, need - 1) == _lib.WC_ERR_WORKSPACE
+            assert run(grads(), ctypes.byref(w), ctypes.c_void_p(8), need) == _lib.WC_ERR_WORKSPACE
+        d.rows = 0
+        assert size(grads()) == (0, 0) and run(grads(), ctypes.byref(w)) == _lib.WC_ERR_BAD_ARG
+        d.rows, d.C = rows, 0
+        assert size(grads())[0] == _lib.WC_ERR_BAD_ARG
+        d.C = (1 << 22) + 1
+        assert size(grads())[0] == _lib.WC_ERR_UNSUPPORTED
+    assert lib.wc_linear4_backward_workspace_bytes(ctypes.byref(d), None, ctypes.byref(n)) == _lib.WC_ERR_BAD_ARG
