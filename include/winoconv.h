@@ -414,10 +414,10 @@ int wc_packed4_bytes(long long rows, int C, size_t* codes, size_t* scales);
 int wc_pack4(const void* x, unsigned char* codes, unsigned char* scales, long long rows, int C, int dtype, void* stream);
 int wc_unpack4(const unsigned char* codes, const unsigned char* scales, void* x, long long rows, int C, int dtype, void* stream);
 
-/* A linear layer (wc_linear_forward, without z) whose weight w (K, C) is in 4 bits; x (rows, C) is of the descriptor's type, or packed as well (the
+/* A linear layer (wc_linear_forward; z or null for x as it is) whose weight w (K, C) is in 4 bits; x (rows, C) is of the descriptor's type, or packed as well (the
  * other of the two null).  x of its type meets w's values in that type; of two packed operands the products are exact.  Sums fp32, one rounding. */
 int wc_linear4_workspace_bytes(const wc_linear_desc* desc, int x_packed, size_t* bytes);
-int wc_linear4_forward(const wc_linear_desc* desc, const void* x, const wc_packed4* x4, const wc_packed4* w, const void* bias, const void* residual, void* y,
+int wc_linear4_forward(const wc_linear_desc* desc, const void* x, const wc_packed4* x4, const wc_packed4* w, const void* bias, const void* residual, void* y, void* z,
                        void* workspace, size_t workspace_bytes, void* stream);
 /* The gradients of that layer for an x as it is, those of wc_linear_backward: w of the gradients is null, and the packed one read in the operands' type.  rows > 0. */
 int wc_linear4_backward_workspace_bytes(const wc_linear_desc* desc, const wc_linear_gradients* gradients, size_t* bytes);   /* goes by which pointers are null */

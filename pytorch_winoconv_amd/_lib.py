@@ -123,7 +123,7 @@ SIGNATURES = {
     "wc_linear4_workspace_bytes": (_i, [_linear_p, _i, ctypes.POINTER(_sz)]),
     "wc_linear4_backward_workspace_bytes": (_i, [_linear_p, _linear_grads_p, ctypes.POINTER(_sz)]),
     "wc_linear4_backward": (_i, [_linear_p, _linear_grads_p, _packed4_p, _vp, _sz, _vp]),
-    "wc_linear4_forward": (_i, [_linear_p, _vp, _packed4_p, _packed4_p, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "wc_linear4_forward": (_i, [_linear_p, _vp, _packed4_p, _packed4_p, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "wc_join_forward": (_i, [_join_p] + [_vp] * 8),
     "wc_join_backward_workspace_bytes": (_i, [_join_p, _join_grads_p, ctypes.POINTER(_sz)]),
     "wc_join_backward": (_i, [_join_p, _join_grads_p, _vp, _sz, _vp]),

@@ -813,7 +813,7 @@ at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C,
 
 // x as it is, or the codes and scales of a Packed4 that reads as `type`; codes and scales of w (K, C)
 py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, const MaybeTensor& x_scales, const py::object& type, const at::Tensor& w_codes,
-                           const at::Tensor& w_scales, int64_t C, const MaybeTensor& bias_, const MaybeTensor& residual_, int activation, bool residual_after) {
+                           const at::Tensor& w_scales, int64_t C, const MaybeTensor& bias_, const MaybeTensor& residual_, int activation, bool residual_after, bool keep_z) {
   const at::Tensor& first = x_ ? *x_ : *x_codes;
   const int64_t nd = first.dim(), K = w_codes.size(0);
   const at::ScalarType st = x_ ? first.scalar_type() : torch::python::detail::py_object_to_dtype(type);
@@ -827,7 +827,8 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
   if (residual_ && residual_->sizes() != at::IntArrayRef(shape)) return py::none();
   const c10::DeviceGuard guard(first.device());
   const MaybeTensor x = packed_rows(x_), bias = packed_rows(bias_), residual = packed_rows(residual_);
-  at::Tensor y = at::empty(shape, first.options().dtype(st));
+  at::Tensor y = at::empty(shape, first.options().dtype(st)), z;
+  if (keep_z) z = at::empty(shape, y.options());
   const wc_linear_desc d = {rows, (int)C, (int)K, dtype_of(y), activation, residual_after};
   const wc_packed4 w4 = {bytes_of(w_codes), bytes_of(w_scales)}, x4 = x ? wc_packed4{nullptr, nullptr} : wc_packed4{bytes_of(*x_codes), bytes_of(*x_scales)};
   size_t bytes = 0;
@@ -837,10 +838,10 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
   if (bytes) ws = workspace_for(y, bytes, stream);
   {
     py::gil_scoped_release nogil;
-    check(wc_linear4_forward(&d, data_or_null(x), x ? nullptr : &x4, &w4, data_or_null(bias), data_or_null(residual), y.data_ptr(), bytes ? ws.data_ptr() : nullptr,
-                             bytes, stream));
+    check(wc_linear4_forward(&d, data_or_null(x), x ? nullptr : &x4, &w4, data_or_null(bias), data_or_null(residual), y.data_ptr(), keep_z ? z.data_ptr() : nullptr,
+                             bytes ? ws.data_ptr() : nullptr, bytes, stream));
   }
-  return py::cast(y);
+  return keep_z ? py::object(py::make_tuple(y, z)) : py::cast(y);
 }
 
 // dx alone of a layer over a Packed4 w (K, C)
@@ -1510,7 +1511,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack4", &pack4, py::arg("x"));
   m.def("unpack4", &unpack4, py::arg("codes"), py::arg("scales"), py::arg("C"), py::arg("type"));
   m.def("linear4_forward", &linear4_forward, py::arg("x"), py::arg("x_codes"), py::arg("x_scales"), py::arg("type"), py::arg("w_codes"), py::arg("w_scales"),
-        py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"));
+        py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"), py::arg("keep_z"));
   m.def("norm_forward", &norm_forward);
   m.def("join_forward", &join_forward);
   m.def("linear4_backward", &linear4_backward);

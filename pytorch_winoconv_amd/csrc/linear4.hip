@@ -147,7 +147,7 @@ int wc_linear4_workspace_bytes(const wc_linear_desc* d, int x_packed, size_t* by
 }
 
 int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4* x4, const wc_packed4* w4, const void* bias, const void* residual, void* y,
-                       void* workspace, size_t workspace_bytes, void* stream) {
+                       void* z, void* workspace, size_t workspace_bytes, void* stream) {
   size_t need = 0;
   if (int rc = wc_linear4_workspace_bytes(d, x4 != nullptr, &need)) return rc;
   if (d->rows == 0) return WC_OK;
@@ -158,7 +158,9 @@ int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4*
   if (need && (!workspace || workspace_bytes < need))
     return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   if (need && reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(WC_ERR_WORKSPACE, "wc_linear4_forward: workspace must be 256-byte aligned");
-  const LinearProduct p = product_of(d, x, bias, residual, y);
+  WC_CHECK_ARG(!z || !x4, "wc_linear4_forward: no z of an x in 4 bits, which has no gradient");
+  LinearProduct p = product_of(d, x, bias, residual, y);
+  p.e.z = z;
   const Operand4 w = {w4->codes, w4->scales};
   if (few(d, x4 != nullptr)) {
     const Operand4 xp = x4 ? Operand4{x4->codes, x4->scales} : Operand4{nullptr, nullptr};
@@ -185,7 +187,7 @@ int wc_linear4_forward(const wc_linear_desc* d, const void* x, const wc_packed4*
   char* const ws = static_cast<char*>(workspace);
   const size_t wide_bytes = rounded((size_t)d->K * d->C * (d->dtype == WC_F32 ? 4 : 2));
   if (int rc = unpack4(w.codes, w.scales, ws, d->K, d->C, d->dtype, stream)) return rc;
-  return wc_linear_forward(d, x, ws, bias, residual, y, nullptr, ws + wide_bytes, need - wide_bytes, stream);
+  return wc_linear_forward(d, x, ws, bias, residual, y, z, ws + wide_bytes, need - wide_bytes, stream);
 }
 
 int wc_linear4_backward_workspace_bytes(const wc_linear_desc* d, const wc_linear_gradients* g, size_t* bytes) {

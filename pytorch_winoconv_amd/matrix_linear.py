@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
 from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
-from .packed4 import Packed4, _made as _made4, linear4_ext, linear4_forward, pack4, unpack4
+from .packed4 import Packed4, _made as _made4, linear4_ext, linear4_forward, pack4
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -103,21 +103,17 @@ def _linear4(x, w, bias, residual, activation, residual_after, keep_z):
     """linear_forward over a Packed4 w."""
     if not isinstance(w, Packed4):
         raise TypeError("linear_forward: x in 4 bits takes a weight in 4 bits, got a tensor")
-    if not keep_z:
-        y = linear4_ext(x, w, bias, residual, ACTIVATIONS[activation], residual_after)
-        if y is not None:
-            return y
+    y = linear4_ext(x, w, bias, residual, ACTIVATIONS[activation], residual_after, keep_z)
+    if y is not None:
+        return y
     _check_weight(x.shape, w, "x")
     K = w.shape[0]
     shape = tuple(x.shape[:-1]) + (K,)
-    if keep_z:
-        # z is for a backward pass, which wants many rows: the weight is widened for them all the same
-        if isinstance(x, Packed4):
-            raise NotImplementedError("linear_forward: no z of an x in 4 bits, which has no gradient")
-        return linear_forward(x, unpack4(w, x.dtype), bias, residual, activation, residual_after, True)
+    if keep_z and isinstance(x, Packed4):
+        raise NotImplementedError("linear_forward: no z of an x in 4 bits, which has no gradient")
     _check_like(bias, (K,), x.dtype, x.device, "the bias")
     _check_like(residual, shape, x.dtype, x.device, "the residual")
-    return linear4_forward(x, w, bias, residual, ACTIVATIONS[activation], residual_after)
+    return linear4_forward(x, w, bias, residual, ACTIVATIONS[activation], residual_after, keep_z)
 
 
 def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=True, need_db=True, need_dz=False, w_type=None, b_type=None):

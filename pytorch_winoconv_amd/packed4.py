@@ -139,20 +139,20 @@ def unpack4(packed, dtype=None):
     return x
 
 
-def linear4_ext(x, w, bias, residual, activation, residual_after):
+def linear4_ext(x, w, bias, residual, activation, residual_after, keep_z=False):
     """linear4_forward by the compiled host layer, which takes operands that fit together; None for others."""
     if not engine.USE_EXT or not w.codes.is_cuda or w.codes.dim() != 2:
         return None
     if not isinstance(x, Packed4):
-        return engine._ext.linear4_forward(x, None, None, None, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after))
-    if x.channels != w.channels:
+        return engine._ext.linear4_forward(x, None, None, None, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after), bool(keep_z))
+    if keep_z or x.channels != w.channels:
         return None
-    return engine._ext.linear4_forward(None, x.codes, x.scales, x.dtype, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after))
+    return engine._ext.linear4_forward(None, x.codes, x.scales, x.dtype, w.codes, w.scales, w.channels, bias, residual, activation, bool(residual_after), False)
 
 
-def linear4_forward(x, w, bias, residual, activation, residual_after):
-    """matrix_linear.linear_forward without z for w a Packed4 (K, C) and x a tensor (..., C) or a Packed4; activation is its number."""
-    y = linear4_ext(x, w, bias, residual, activation, residual_after)
+def linear4_forward(x, w, bias, residual, activation, residual_after, keep_z=False):
+    """matrix_linear.linear_forward for w a Packed4 (K, C) and x a tensor (..., C) or, without z, a Packed4; activation is its number."""
+    y = linear4_ext(x, w, bias, residual, activation, residual_after, keep_z)
     if y is not None:
         return y
     packed, C = isinstance(x, Packed4), w.channels
@@ -166,6 +166,7 @@ def linear4_forward(x, w, bias, residual, activation, residual_after):
     if w.device != x.device:
         raise ValueError("the weight is on %s, expected %s" % (w.device, x.device))
     y = torch.empty(shape, dtype=dtype, device=x.device)
+    z = torch.empty_like(y) if keep_z else None
     rows = _rows(shape)
     own = lambda t: t.clone() if engine.misaligned(t) else t  # noqa: E731
     x_, bias, residual = (None if t is None else own(t.detach().contiguous()) for t in (None if packed else x, bias, residual))
@@ -176,6 +177,6 @@ def linear4_forward(x, w, bias, residual, activation, residual_after):
     w4, x4 = w._pointers(), x._pointers() if packed else None
     with engine._on_device(y):
         p = engine._ptr
-        check(lib.wc_linear4_forward(ctypes.byref(d), p(x_), ctypes.byref(x4) if packed else None, ctypes.byref(w4), p(bias), p(residual), p(y), p(ws),
+        check(lib.wc_linear4_forward(ctypes.byref(d), p(x_), ctypes.byref(x4) if packed else None, ctypes.byref(w4), p(bias), p(residual), p(y), p(z), p(ws),
                                      nbytes.value, engine._stream(y)))
-    return y
+    return (y, z) if keep_z else y

@@ -384,3 +384,21 @@ def test_gradients_captured_and_side_by_side(dev):
                 got.append([grad(dy) for _ in range(3)])
         torch.cuda.synchronize()
         assert all(torch.equal(a[0], b[0]) and torch.equal(a[2], b[2]) for runs, b in zip(got, want) for a in runs)
+
+
+@pytest.mark.parametrize("t", lo.TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(3, 300, 72), (16, 520, 41), (64, 4096, 136), (200, 72, 264), (300, 1000, 77), (2050, 136, 72), (33, 257, 72)], ids=str)
+def test_z_is_kept(dev, host_layer, shape, t):
+    rows, C, K = shape
+    for act, after in (("gelu", False), ("silu", True), ("none", False)):
+        g = torch.Generator().manual_seed(rows + C)
+        x, w = torch.randn(rows, C, generator=g).to(t), torch.randn(K, C, generator=g) * C ** -0.5
+        b, r = torch.randn(K, generator=g).to(t), torch.randn(rows, K, generator=g).to(t)
+        W = po.values(*po.pack(w), C).to(t).double()
+        w4 = packed4.pack4(w.cuda())
+        y, z = matrix_linear.linear_forward(x.cuda(), w4, b.cuda(), r.cuda(), act, after, keep_z=True)
+        want = lo.forward(x, W, b, r, act, after)
+        lo.within(y, want[0], want[2], "y " + act)
+        lo.within(z, want[1], want[3], "z " + act)
+        # y is that of a pass without z
+        assert torch.equal(y, matrix_linear.linear_forward(x.cuda(), w4, b.cuda(), r.cuda(), act, after))

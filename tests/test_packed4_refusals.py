@@ -111,7 +111,7 @@ def test_c_entry_points_refuse():
     n = ctypes.c_size_t()
     assert lib.wc_linear4_workspace_bytes(ctypes.byref(d), 0, ctypes.byref(n)) == 0 and n.value >= 64 * 256 * 2
     w, at = _lib.Packed4Parts(256, 256), ctypes.c_void_p(256)
-    run = lambda x, x4, w, y, ws=None, size=0: lib.wc_linear4_forward(ctypes.byref(d), x, x4, w, None, None, y, ws, size, None)  # noqa: E731
+    run = lambda x, x4, w, y, ws=None, size=0: lib.wc_linear4_forward(ctypes.byref(d), x, x4, w, None, None, y, None, ws, size, None)  # noqa: E731
     assert run(None, None, ctypes.byref(w), at) == _lib.WC_ERR_BAD_ARG
     assert run(at, ctypes.byref(w), ctypes.byref(w), at) == _lib.WC_ERR_BAD_ARG
     assert run(at, None, None, at) == _lib.WC_ERR_BAD_ARG
