@@ -703,7 +703,7 @@ py::object linear_forward(const at::Tensor& x_, const at::Tensor& w_, const Mayb
   return keep_z ? py::object(py::make_tuple(y, z)) : py::cast(y);
 }
 
-// operands that the Python layer has checked; rows > 0.  w as it is, or codes and scales of a Packed4
+// operands that the Python layer, or linear4_backward, has checked; rows > 0.  w as it is, or codes and scales of a Packed4
 py::tuple gradients_of(const at::Tensor& dy_, const MaybeTensor& x, const MaybeTensor& x_exp, const MaybeTensor& w_, const MaybeTensor& codes, const MaybeTensor& scales,
                        const MaybeTensor& z, const MaybeTensor& z_exp, int C, int activation, bool need_dx, bool need_dw, bool need_db, bool need_dz, at::ScalarType wt,
                        at::ScalarType bt) {
@@ -778,6 +778,13 @@ py::object unpack8(const at::Tensor& codes, const at::Tensor& exps, const py::ob
 
 // ---- tensors in 4 bits (packed4.py) and linear layers over them
 unsigned char* bytes_of(const at::Tensor& t) { return t.data_ptr<uint8_t>(); }
+// whether codes and scales are those of a tensor of C channels and lie as the kernels read them
+bool packed4_fits(const at::Tensor& codes, const at::Tensor& scales, int64_t C) {
+  auto lies = [](const at::Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kByte && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
+  if (!lies(codes) || !lies(scales) || codes.device() != scales.device() || codes.dim() < 1 || C < 1) return false;
+  const int64_t stages = (C + 127) / 128, rows = codes.size(codes.dim() - 1) == stages * 64 ? codes.numel() / (stages * 64) : -1;
+  return rows >= 0 && scales.numel() == (rows + 31) / 32 * stages * 128;
+}
 
 py::object pack4(const at::Tensor& x_) {
   const int64_t nd = x_.dim();
@@ -797,7 +804,7 @@ py::object pack4(const at::Tensor& x_) {
   return py::make_tuple(codes, scales);
 }
 
-// codes and scales of a Packed4 with elements
+// codes and scales of a Packed4 with elements, which the Python layer has checked
 at::Tensor unpack4(const at::Tensor& codes, const at::Tensor& scales, int64_t C, const py::object& type) {
   const c10::DeviceGuard guard(codes.device());
   at::DimVector shape(codes.sizes());
@@ -818,7 +825,8 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
   const int64_t nd = first.dim(), K = w_codes.size(0);
   const at::ScalarType st = x_ ? first.scalar_type() : torch::python::detail::py_object_to_dtype(type);
   const auto own = [&](const MaybeTensor& t) { return !t || (t->scalar_type() == st && t->device() == first.device() && t->layout() == at::kStrided); };
-  if ((x_ && (!linear_type(first) || nd < 1 || first.size(nd - 1) != C)) || first.numel() == 0 || w_codes.device() != first.device() || !own(bias_) || !own(residual_) ||
+  if ((x_ && (!linear_type(first) || nd < 1 || first.size(nd - 1) != C)) || first.numel() == 0 || !packed4_fits(w_codes, w_scales, C) || w_codes.dim() != 2 ||
+      (x_codes && !packed4_fits(*x_codes, *x_scales, C)) || w_codes.device() != first.device() || !own(bias_) || !own(residual_) ||
       (bias_ && (bias_->dim() != 1 || bias_->size(0) != K)))
     return py::none();
   at::DimVector shape(first.sizes());
@@ -847,7 +855,8 @@ py::object linear4_forward(const MaybeTensor& x_, const MaybeTensor& x_codes, co
 // dx alone of a layer over a Packed4 w (K, C)
 py::object linear4_backward(const at::Tensor& dy, const at::Tensor& w_codes, const at::Tensor& w_scales, int64_t C, const MaybeTensor& z_, int activation) {
   const int64_t nd = dy.dim();
-  if (!linear_type(dy) || nd < 1 || dy.numel() == 0 || w_codes.numel() == 0 || w_codes.dim() != 2 || w_codes.size(0) != dy.size(nd - 1) || w_codes.device() != dy.device() || !fits(C) ||
+  if (!linear_type(dy) || nd < 1 || dy.numel() == 0 || w_codes.numel() == 0 || w_codes.dim() != 2 || w_codes.size(0) != dy.size(nd - 1) || w_codes.device() != dy.device() ||
+      !packed4_fits(w_codes, w_scales, C) || !fits(C) ||
       !fits(w_codes.size(0)) || (activation && (!z_ || !same_kind(z_, dy) || z_->sizes() != dy.sizes())))
     return py::none();
   const c10::DeviceGuard guard(dy.device());

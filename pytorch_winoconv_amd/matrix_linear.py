@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
 from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
-from .packed4 import Packed4, _made as _made4, linear4_ext, linear4_forward, pack4
+from .packed4 import ROWS as ROWS4, Packed4, _made as _made4, linear4_ext, linear4_forward, pack4, settled as settled4
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -153,7 +153,7 @@ def linear_backward(dy, x, w, z=None, activation="none", need_dx=True, need_dw=T
     if not dy.is_cuda:
         raise ValueError("winoconv runs on the GPU only: got a %s tensor" % device)
     engine._require_gpu(dy)
-    packed, w = (w if need_dx else None, None) if isinstance(w, Packed4) else (None, w)
+    packed, w = (settled4(w) if need_dx else None, None) if isinstance(w, Packed4) else (None, w)
     w_type, b_type = w_type or dtype, b_type or dtype
     w_own, b_own = (t if t == torch.float32 else dtype for t in (w_type, b_type))
     if need_dz and not act:
@@ -309,8 +309,8 @@ class MatrixLinear(nn.Module):
 
 class MatrixLinear4(nn.Module):
     """A linear layer whose weight is frozen, in 4 bits (MatrixLinear.pack4, or of a Packed4 w (out_features, in_features)): 1/2 + 1/32 bytes a
-    weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales`; the bias is a parameter, which with x4 does not
-    learn either."""
+    weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales` (with one axis for a stage's 32 rows and 4 groups: of a
+    buffer of four axes Module.to(memory_format=...) would change the strides); the bias is a parameter, which with x4 does not learn either."""
 
     def __init__(self, weight, bias=None, activation="none", residual_after=False, channel_axis=-1, x4=False):
         super().__init__()
@@ -324,16 +324,28 @@ class MatrixLinear4(nn.Module):
         self.activation, self.residual_after, self.channel_axis, self.x4 = activation, residual_after, channel_axis, bool(x4)
         self.dtype = w4.dtype
         self.register_buffer("codes", w4.codes)
-        self.register_buffer("scales", w4.scales)
+        self.register_buffer("scales", w4.scales.flatten(2))
         self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=bias.requires_grad and not x4)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        # (a Packed4's own scales, of four axes)
+        scales = state_dict.get(prefix + "scales")
+        if isinstance(scales, torch.Tensor) and scales.dim() == 4:
+            state_dict[prefix + "scales"] = scales.flatten(2)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
+    def _parts(self):
+        """The buffers as a Packed4's; where they do not lie as the kernels read them, the layer's calls copy them."""
+        blocks, stages = self.scales.shape[:2]
+        return self.codes, self.scales.reshape(blocks, stages, ROWS4, 4), self.in_features, self.dtype
 
     @property
     def weight(self):
         """The Packed4 of the buffers as they are now."""
-        return Packed4(self.codes, self.scales, self.in_features, self.dtype)
+        return Packed4(*self._parts())
 
     def forward(self, x, residual=None):
-        w = _made4(self.codes, self.scales, self.in_features, self.dtype)
+        w = _made4(*self._parts())
         if not self.x4:
             return linear(x, w, self.bias, residual, self.activation, self.residual_after, None, self.channel_axis)
         if torch.is_grad_enabled() and x.requires_grad:

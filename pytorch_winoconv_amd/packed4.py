@@ -101,6 +101,20 @@ def _made(codes, scales, channels, dtype):
     return p
 
 
+def _belong(p):
+    """Whether codes and scales lie as the kernels read them: whole, one after the other, from multiples of 16 bytes."""
+    codes, scales = p.codes, p.scales
+    stages = -(-p.channels // STAGE)
+    return (codes.is_contiguous() and scales.is_contiguous() and not engine.misaligned(codes, scales) and codes.dtype == scales.dtype == torch.uint8
+            and codes.device == scales.device and codes.shape[-1] == 64 * stages and tuple(scales.shape) == (-(-_rows(codes.shape) // ROWS), stages, ROWS, 4))
+
+
+def settled(p):
+    """A Packed4 whose parts the kernels may read: p as it is, or its parts copied where they lie otherwise (a module's buffers take other strides and starts
+    when it is moved or loaded); parts that are not each other's are refused."""
+    return p if _belong(p) else Packed4(p.codes, p.scales, p.channels, p.dtype)
+
+
 def pack4(x):
     """x (..., C) in 4 bits."""
     if engine.USE_EXT:
@@ -129,6 +143,7 @@ def unpack4(packed, dtype=None):
         raise TypeError("winoconv supports float32, float16 and bfloat16, got %s" % dtype)
     if not packed.codes.is_cuda:
         raise ValueError("winoconv runs on the GPU only: got a %s tensor" % packed.device)
+    packed = settled(packed)
     if engine.USE_EXT and packed.codes.numel():
         return engine._ext.unpack4(packed.codes, packed.scales, packed.channels, dtype)
     x = torch.empty(packed.shape, dtype=dtype, device=packed.device)
@@ -140,7 +155,7 @@ def unpack4(packed, dtype=None):
 
 
 def linear4_ext(x, w, bias, residual, activation, residual_after, keep_z=False):
-    """linear4_forward by the compiled host layer, which takes operands that fit together; None for others."""
+    """linear4_forward by the compiled host layer, which takes operands that fit together and lie as the kernels read them; None for others."""
     if not engine.USE_EXT or not w.codes.is_cuda or w.codes.dim() != 2:
         return None
     if not isinstance(x, Packed4):
@@ -155,7 +170,8 @@ def linear4_forward(x, w, bias, residual, activation, residual_after, keep_z=Fal
     y = linear4_ext(x, w, bias, residual, activation, residual_after, keep_z)
     if y is not None:
         return y
-    packed, C = isinstance(x, Packed4), w.channels
+    packed, w = isinstance(x, Packed4), settled(w)
+    x, C = settled(x) if packed else x, w.channels
     K, shape, dtype = w.codes.shape[0], tuple(x.shape[:-1]) + (w.codes.shape[0],), x.dtype
     if packed:
         if not x.codes.is_cuda:
