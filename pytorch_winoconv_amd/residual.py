@@ -384,15 +384,34 @@ class BlockNorm(nn.Module):
         return "%d, %r, eps=%g" % (self.channels, self.kind, self.eps)
 
 
+# Passes that may be run again, of which a module keeps what they drew: 100 bytes each, with counter=True 512 of the GPU's
+PASSES_KEPT = 4096
+
+
+def _in_backward():
+    """Whether this is run within a backward pass, as a checkpointed pass is the second time."""
+    return torch._C._current_graph_task_id() != -1
+
+
+def _may_run_again():
+    """Whether the pass may be the first run of a checkpointed one, which has no gradients of its own or hooks on the tensors that it saves."""
+    return not torch.is_grad_enabled() or torch._C._autograd._top_saved_tensors_default_hooks(True) is not None
+
+
 class Dropout(nn.Module):
     """Dropout whose mask is never stored.  Each pass in training counts the offset up; the seed is drawn from torch's generator where none is given, and both are in
-    the state dict.  counter=True keeps them on the GPU, in the buffer `state`, so that a captured pass draws another mask in every replay (a launch more a pass)."""
+    the state dict.  counter=True keeps them on the GPU, in the buffer `state`, so that a captured pass draws another mask in every replay (two small launches more a pass).
+
+    A pass that torch.utils.checkpoint runs again in the backward pass takes the mask of its first run.  It is known by the state of torch's CPU generator, which checkpoint
+    restores (preserve_rng_state) and from which passes without gradients or under saved-tensor hooks draw one number; in a backward pass a mask that is no earlier pass's, or
+    that may be several's, is refused, as are those of captured passes with counter=True.  `dropout` and `join` with a Drop of one's own have no such passes."""
 
     def __init__(self, p=0.5, per="element", seed=None, counter=False, channel_axis=-1, device=None):
         super().__init__()
         seed = int(torch.randint(0, 1 << 62, (1,)).item()) if seed is None else seed
         Drop(p, seed, 0, per)
         self.p, self.per, self.channel_axis = p, per, channel_axis
+        self._passes = {}                      # token of a pass: what it drew (None: one of several), whether it was run again
         if counter:
             if seed >= 1 << 63:
                 raise ValueError("Dropout: seed %r in a buffer, from 0 to 2^63 - 1" % (seed,))
@@ -404,12 +423,40 @@ class Dropout(nn.Module):
         """The Drop of the next pass; None where nothing is dropped."""
         if not self.training or Drop(self.p, 0).level == 0:
             return None
+        again = _in_backward()
+        # (a second run starts where torch's generator was, so it draws what the first run did)
+        token = int(torch.randint(1 << 62, (), device="cpu")) if again or _may_run_again() else None
+        if again:
+            return self._drawn_by(token)
         if self.state is not None:
             used = self.state.clone()
             self.state[1].add_(1)
-            return Drop(self.p, used, 0, self.per)
-        self.calls += 1
-        return Drop(self.p, self.seed, self.calls - 1, self.per)
+            drop = Drop(self.p, used, 0, self.per)
+        else:
+            self.calls += 1
+            drop = Drop(self.p, self.seed, self.calls - 1, self.per)
+        # (what a captured pass drew is the graph's)
+        if token is not None and not (self.state is not None and self.state.is_cuda and torch.cuda.is_current_stream_capturing()):
+            had = self._passes.pop(token, None)
+            self._passes[token] = [drop if had is None or had[1] else None, False]
+            if len(self._passes) > PASSES_KEPT:
+                del self._passes[next(iter(self._passes))]
+        return drop
+
+    def _drawn_by(self, token):
+        """The Drop of the first run of a pass."""
+        found = self._passes.get(token)
+        if found is None or found[0] is None:
+            raise RuntimeError("Dropout: a pass run again in a backward pass starts at the state that torch's generator had the first time, no other pass's "
+                               "(torch.utils.checkpoint with preserve_rng_state, which is its default); else give dropout or join a Drop")
+        found[1] = True
+        return found[0]
+
+    def __getstate__(self):
+        return {**self.__dict__, "_passes": {}}
+
+    def __setstate__(self, state):
+        super().__setstate__({"_passes": {}, **state})
 
     def get_extra_state(self):
         return None if self.state is not None else torch.tensor([self.seed - (1 << 64) if self.seed >> 63 else self.seed, self.calls])

@@ -1,0 +1,56 @@
+"""Modules of joins and dropout in training: checkpointed, copied, in the forms that stacks of layers take."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import pytorch_winoconv_amd as pkg
+from pytorch_winoconv_amd import residual
+
+pytestmark = pytest.mark.gpu
+
+
+def _grads(y, x, params):
+    for v in [x] + params:
+        v.grad = None
+    y.square().sum().backward()
+    return [v.grad for v in [x] + params]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("counter", [False, True])
+@pytest.mark.parametrize("per", ["element", "sample"])
+def test_checkpointed_dropout(dev, host_layer, per, counter, reentrant):
+    """The mask of a pass that is run again is that of its result, also with another pass between."""
+    m = pkg.Dropout(0.4, per, seed=3, counter=counter).cuda()
+    leaves = [(torch.rand(40, 3, 72, device=dev) + 1).requires_grad_() for _ in range(2)]
+    ys = [checkpoint(lambda v: m(v * 2).exp(), x, use_reentrant=reentrant) for x in leaves]
+    for i in (1, 0):
+        ys[i].sum().backward()
+        assert torch.equal(leaves[i].grad != 0, ys[i] != 1)
+    assert not torch.equal(ys[0] != 1, ys[1] != 1) and (int(m.state[1]) if counter else m.calls) == 2
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("counter", [False, True])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=str)
+def test_checkpointed_stacks(dev, t, counter, reentrant):
+    """Whole and block by block: results and gradients of the stack that is not checkpointed, bit for bit."""
+    def make():
+        torch.manual_seed(4)
+        return pkg.ResidualStack([residual.matrix_block(72, 200, "silu") for _ in range(2)], 72, "rms", post=True, gate=0.5, drop=0.3, per="element", counter=counter).cuda().to(t)
+    stack, plain = make(), make()
+    for _ in range(3):
+        x = torch.randn(4, 33, 72, device=dev).to(t).requires_grad_()
+        y, want = checkpoint(stack, x, use_reentrant=reentrant), plain(x)
+        assert torch.equal(y, want)
+        got = _grads(y, x, list(stack.parameters()))
+        for a, b in zip(got, _grads(want, x, list(plain.parameters()))):
+            assert torch.equal(a, b)
+
+
+def test_runs_again_that_cannot_be_told(dev):
+    m = pkg.Dropout(0.4).cuda()
+    x = torch.randn(6, 24, device=dev).requires_grad_()
+    y = checkpoint(lambda v: m(v.sin()).exp(), x, use_reentrant=False, preserve_rng_state=False)
+    with pytest.raises(RuntimeError, match="run again in a backward pass"):
+        y.sum().backward()

@@ -1,0 +1,160 @@
+"""Dropout's passes and stacks of blocks on the CPU, by the definition in the kernels' place."""
+import copy
+import io
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import pytorch_winoconv_amd as pkg
+from pytorch_winoconv_amd import residual
+
+import residual_oracle as ro
+
+
+def _kept(shape, drop):
+    seed, offset = (int(v) for v in drop.seed) if isinstance(drop.seed, torch.Tensor) else (drop.seed, drop.offset)
+    return ro.mask(tuple(shape), drop.p, seed, offset, drop.per)
+
+
+@pytest.fixture
+def definition(monkeypatch):
+    """dropout, norm and join by their formulas, with torch's own gradients."""
+    def dropout(x, drop, axis=-1):
+        kept, scale = _kept(x.shape, drop)
+        return torch.where(kept, x * scale, torch.zeros_like(x))
+
+    def norm(x, n, axis=-1):
+        return ro.norm(x, n.kind, n.weight, n.bias, n.eps)
+
+    def join(f, x, post, gate, pre, drop, a, b, axis=-1):
+        v = f if post is None else norm(f, post)
+        v = v if drop is None else dropout(v, drop)
+        s = a * x + b * (v if gate is None else v * gate)
+        return s, norm(s, pre)
+    for name, f in (("dropout", dropout), ("norm", norm), ("join", join)):
+        monkeypatch.setattr(residual, name, f)
+
+
+def _modules(counter):
+    return [pkg.Dropout(0.4, seed=5 + i, counter=counter) for i in range(2)]
+
+
+@pytest.mark.parametrize("counter", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_passes_that_are_run_again(definition, counter, reentrant):
+    """The mask of the gradient is that of the result, with several passes on their way, whichever goes back first; masks are those of passes that are not run again."""
+    for order in ((0, 1, 2), (2, 1, 0), (1, 2, 0)):
+        ms, plain = _modules(counter), _modules(counter)
+        leaves = [(torch.randn(6, 24) + 3).requires_grad_() for _ in order]
+        run = lambda x: ms[1](torch.sin(ms[0](x * 1.5)))  # noqa: E731,B023
+        ys = [checkpoint(run, x, use_reentrant=reentrant) for x in leaves]
+        want = [plain[1](torch.sin(plain[0](x * 1.5))) for x in leaves]
+        assert all(torch.equal(a, b) for a, b in zip(ys, want))
+        for i in order:
+            (a,), (b,) = (torch.autograd.grad(y[i].sum(), leaves[i]) if not reentrant else (_through(y[i], leaves[i]),) for y in (ys, want))
+            assert torch.equal(a, b)
+        # a run again is no pass of its own
+        assert [int(m.state[1]) if counter else m.calls for m in ms] == [3, 3]
+        assert torch.equal(ms[0](leaves[0]), plain[0](leaves[0]))
+
+
+def _through(y, leaf):
+    leaf.grad = None
+    y.sum().backward()
+    return leaf.grad
+
+
+@pytest.mark.parametrize("counter", [False, True])
+def test_nested_and_twice(definition, counter):
+    ms, plain = _modules(counter), _modules(counter)
+    x = (torch.randn(5, 16) + 3).requires_grad_()
+    inner = lambda v: ms[0](v).exp()  # noqa: E731
+    y = checkpoint(lambda v: ms[1](checkpoint(inner, v.sin(), use_reentrant=False)).cos(), x, use_reentrant=False)
+    want = plain[1](plain[0](x.sin()).exp()).cos()
+    (b,) = torch.autograd.grad(want.sum(), x)
+    for _ in range(2):
+        (a,) = torch.autograd.grad(y.sum(), x, retain_graph=True)
+        assert torch.equal(a, b)
+    # one module twice in a pass
+    y = checkpoint(lambda v: ms[0](ms[0](v).exp()).sin(), x, use_reentrant=False)
+    want = plain[0](plain[0](x).exp()).sin()
+    assert torch.equal(y, want) and torch.equal(torch.autograd.grad(y.sum(), x)[0], torch.autograd.grad(want.sum(), x)[0])
+
+
+@pytest.mark.parametrize("counter", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_stacks(definition, counter, reentrant):
+    def make():
+        torch.manual_seed(7)
+        return pkg.ResidualStack([torch.nn.Sequential(torch.nn.Linear(24, 40), torch.nn.SiLU(), torch.nn.Linear(40, 24)) for _ in range(3)], 24, post=True, gate=0.5, drop=0.4,
+                                 per="element", counter=counter)
+    stack, plain = make(), make()
+    for _ in range(2):
+        x = torch.randn(4, 9, 24).requires_grad_()
+        y, want = checkpoint(stack, x, use_reentrant=reentrant), plain(x)
+        assert torch.equal(y, want)
+        y.square().sum().backward()
+        got = [x.grad] + [p.grad for p in stack.parameters()]
+        x.grad = None
+        want.square().sum().backward()
+        for a, b in zip(got, [x.grad] + [p.grad for p in plain.parameters()]):
+            # (gradients of several uses are added up in another order)
+            assert float((a - b).abs().max()) <= 1e-5 * float(b.abs().max())
+
+
+@pytest.mark.parametrize("counter", [False, True])
+def test_runs_again_that_cannot_be_told(definition, counter):
+    """Refused, not given another mask."""
+    m = pkg.Dropout(0.4, counter=counter)
+    x = torch.randn(6, 24).requires_grad_()
+    run = lambda v: m(v.sin()).exp()  # noqa: E731
+    for reentrant in (False, True):
+        y = checkpoint(run, x, use_reentrant=reentrant, preserve_rng_state=False)
+        with pytest.raises(RuntimeError, match="run again in a backward pass"):
+            y.sum().backward()
+    # two passes from the same state of torch's generator: one after the other, and both on their way
+    for _ in range(3):
+        torch.manual_seed(1)
+        y = checkpoint(run, x, use_reentrant=False)
+        (g,) = torch.autograd.grad(y.sum(), x)
+        assert torch.equal(g != 0, y != 1)
+    torch.manual_seed(2)
+    first = checkpoint(run, x, use_reentrant=False)
+    torch.manual_seed(2)
+    second = checkpoint(run, x, use_reentrant=False)
+    for y in (first, second):
+        with pytest.raises(RuntimeError, match="run again in a backward pass"):
+            y.sum().backward()
+    # a pass whose number is kept no longer
+    y = checkpoint(run, x, use_reentrant=False)
+    with torch.no_grad():
+        for _ in range(residual.PASSES_KEPT):
+            m.draw()
+    with pytest.raises(RuntimeError, match="run again in a backward pass"):
+        y.sum().backward()
+
+
+def test_other_passes_leave_the_generator_alone(definition):
+    m = pkg.Dropout(0.4, seed=1)
+    before = torch.get_rng_state()
+    y = m(torch.randn(3, 8, generator=torch.Generator()).requires_grad_())
+    y.sum().backward()
+    m.eval()
+    with torch.no_grad():
+        m(torch.ones(3, 8))
+    assert torch.equal(torch.get_rng_state(), before)
+    assert not m._passes
+
+
+def test_what_is_kept_of_passes_stays_here(definition):
+    m = pkg.Dropout(0.4, seed=1, counter=True)
+    with torch.no_grad():
+        m(torch.ones(3, 8))
+    assert len(m._passes) == 1
+    buffer = io.BytesIO()
+    torch.save(m, buffer)
+    buffer.seek(0)
+    for other in (copy.deepcopy(m), torch.load(buffer, weights_only=False)):
+        assert not other._passes and torch.equal(other.state, m.state)
+    assert set(m.state_dict()) == set(pkg.Dropout(0.1, counter=True).state_dict())
