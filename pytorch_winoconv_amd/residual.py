@@ -502,12 +502,15 @@ class ResidualStack(nn.Module):
         return y
 
     def pack4(self, x4=False):
-        """This stack for serving: every MatrixLinear in its blocks becomes a MatrixLinear4 (in place; MatrixLinear.pack4)."""
-        for block in self.blocks:
-            for parent in list(block.modules()):
-                for name, child in list(parent.named_children()):
-                    if isinstance(child, MatrixLinear):
-                        setattr(parent, name, child.pack4(x4))
+        """This stack for serving: every MatrixLinear among its blocks and in them becomes a MatrixLinear4, one in several places one (in place; MatrixLinear.pack4)."""
+        made = {}
+        for parent in list(self.blocks.modules()):
+            # (named_children would give a module that stands twice under one parent once)
+            for name, child in list(parent._modules.items()):
+                if isinstance(child, MatrixLinear):
+                    if child not in made:
+                        made[child] = child.pack4(x4)
+                    setattr(parent, name, made[child])
         return self
 
 

@@ -54,3 +54,20 @@ def test_runs_again_that_cannot_be_told(dev):
     y = checkpoint(lambda v: m(v.sin()).exp(), x, use_reentrant=False, preserve_rng_state=False)
     with pytest.raises(RuntimeError, match="run again in a backward pass"):
         y.sum().backward()
+
+
+def test_stacks_of_layers_packed(dev):
+    """A block that is a layer itself is served in 4 bits as the layers in other blocks are."""
+    torch.manual_seed(5)
+    layer = pkg.MatrixLinear(72, 72, activation="silu")
+    stack = pkg.ResidualStack([layer, residual.matrix_block(72, 136), torch.nn.Sequential(layer, layer)], 72, "rms").cuda().eval()
+    x = torch.randn(5, 72, device=dev)
+    with torch.no_grad():
+        for m in stack.blocks.modules():
+            if isinstance(m, pkg.MatrixLinear):
+                m.weight.copy_(pkg.packed4.unpack4(pkg.packed4.pack4(m.weight)))
+        want = stack(x)
+        got = stack.pack4()(x)
+    # (the same values in 4 bits, fp32 sums of 72 and 136 products in another order)
+    assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
+    assert isinstance(stack.blocks[0], pkg.MatrixLinear4) and stack.blocks[2][0] is stack.blocks[2][1] is stack.blocks[0]

@@ -7,8 +7,9 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import pytorch_winoconv_amd as pkg
-from pytorch_winoconv_amd import residual
+from pytorch_winoconv_amd import matrix_linear, packed4, residual
 
+import packed4_oracle as po
 import residual_oracle as ro
 
 
@@ -158,3 +159,25 @@ def test_what_is_kept_of_passes_stays_here(definition):
     for other in (copy.deepcopy(m), torch.load(buffer, weights_only=False)):
         assert not other._passes and torch.equal(other.state, m.state)
     assert set(m.state_dict()) == set(pkg.Dropout(0.1, counter=True).state_dict())
+
+
+@pytest.fixture
+def pack_on_cpu(monkeypatch):
+    monkeypatch.setattr(matrix_linear, "pack4", lambda w: packed4.Packed4.from_parts(*po.pack(w.detach()), w.shape[1], w.dtype))
+
+
+def test_every_layer_of_a_stack_is_packed(pack_on_cpu):
+    """A block that is a layer itself, layers at any depth, and one layer in several places, which stays one."""
+    shared, deep = pkg.MatrixLinear(40, 40), pkg.MatrixLinear(40, 40)
+    once, pair = pkg.MatrixLinear(40, 40), torch.nn.Sequential(shared, torch.nn.SiLU(), shared)
+    blocks = [once, residual.matrix_block(40, 64), pair, shared, once, torch.nn.Sequential(torch.nn.Sequential(deep), torch.nn.Linear(40, 40)), pair]
+    for x4 in (False, True):
+        stack = pkg.ResidualStack(copy.deepcopy(blocks), 40)
+        made = stack.pack4(x4)
+        assert made is stack and not any(isinstance(m, pkg.MatrixLinear) for m in stack.modules())
+        packed = [m for m in stack.modules() if isinstance(m, pkg.MatrixLinear4)]
+        assert len(packed) == 5 and all(m.x4 == x4 for m in packed)
+        b = stack.blocks
+        assert b[0] is b[4] and b[2] is b[6] and b[2][0] is b[2][2] is b[3] and b[3] is not b[0] and isinstance(b[5][1], torch.nn.Linear)
+        for i, layer in ((0, once), (3, shared)):
+            assert torch.equal(b[i].weight.parts()[0], po.pack(layer.weight.detach())[0])
