@@ -303,25 +303,29 @@ class MatrixLinear(nn.Module):
         layer = MatrixLinear4.__new__(MatrixLinear4)
         nn.Module.__init__(layer)
         w4 = pack4(self.weight)
-        layer._hold(w4, self.bias, self.activation, self.residual_after, self.channel_axis, x4)
+        layer._hold(w4, self.bias, self.activation, self.residual_after, self.channel_axis, x4, self.checkpoint)
         return layer
 
 
 class MatrixLinear4(nn.Module):
     """A linear layer whose weight is frozen, in 4 bits (MatrixLinear.pack4, or of a Packed4 w (out_features, in_features)): 1/2 + 1/32 bytes a
     weight, which is what a layer of few rows reads.  The weight is in the buffers `codes` and `scales` (with one axis for a stage's 32 rows and 4 groups: of a
-    buffer of four axes Module.to(memory_format=...) would change the strides); the bias is a parameter, which with x4 does not learn either."""
+    buffer of four axes Module.to(memory_format=...) would change the strides); the bias is a parameter, which with x4 does not learn either.  checkpoint: as
+    MatrixLinear's, of z."""
 
-    def __init__(self, weight, bias=None, activation="none", residual_after=False, channel_axis=-1, x4=False):
+    checkpoint = None                        # (of layers that were saved whole before they had one)
+
+    def __init__(self, weight, bias=None, activation="none", residual_after=False, channel_axis=-1, x4=False, checkpoint=None):
         super().__init__()
         _activation(activation)
+        _check_checkpoint(checkpoint)
         if not isinstance(weight, Packed4) or len(weight.shape) != 2:
             raise TypeError("MatrixLinear4: the weight is a Packed4 of two axes")
-        self._hold(weight, bias, activation, residual_after, channel_axis, x4)
+        self._hold(weight, bias, activation, residual_after, channel_axis, x4, checkpoint)
 
-    def _hold(self, w4, bias, activation, residual_after, channel_axis, x4):
+    def _hold(self, w4, bias, activation, residual_after, channel_axis, x4, checkpoint):
         self.out_features, self.in_features = w4.shape
-        self.activation, self.residual_after, self.channel_axis, self.x4 = activation, residual_after, channel_axis, bool(x4)
+        self.activation, self.residual_after, self.channel_axis, self.x4, self.checkpoint = activation, residual_after, channel_axis, bool(x4), checkpoint
         self.dtype = w4.dtype
         self.register_buffer("codes", w4.codes)
         self.register_buffer("scales", w4.scales.flatten(2))
@@ -347,7 +351,7 @@ class MatrixLinear4(nn.Module):
     def forward(self, x, residual=None):
         w = _made4(*self._parts())
         if not self.x4:
-            return linear(x, w, self.bias, residual, self.activation, self.residual_after, None, self.channel_axis)
+            return linear(x, w, self.bias, residual, self.activation, self.residual_after, self.checkpoint, self.channel_axis)
         if torch.is_grad_enabled() and x.requires_grad:
             raise NotImplementedError("MatrixLinear4: no gradient passes a layer that puts its inputs into 4 bits")
         axis = self.channel_axis

@@ -54,3 +54,21 @@ def test_parts_that_lie_otherwise(dev, host_layer):
                 other.codes, other.scales = move(p.codes), move(p.scales)
                 others.append(other)
             assert all(torch.equal(a, b) for a, b in zip(results(*others), want))
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_checkpoints_are_kept(dev, checkpoint):
+    """What a layer keeps for its backward pass, and its gradient, are those of `linear` with the same checkpoint."""
+    torch.manual_seed(2)
+    layer = pkg.MatrixLinear(96, 64, activation="gelu", checkpoint=checkpoint).cuda()
+    four, x = layer.pack4(), torch.randn(70, 96, device=dev)
+
+    def kept(call):
+        held = []
+        leaf = x.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: (held.append((v.dtype, tuple(v.shape))), v)[1], lambda v: v):
+            y = call(leaf)
+        return held, torch.autograd.grad(y.sum(), leaf)[0]
+    got, want = kept(four), kept(lambda v: matrix_linear.linear(v, four.weight, four.bias, None, "gelu", checkpoint=checkpoint))
+    assert got[0] == want[0] and torch.equal(got[1], want[1])
+    assert ((torch.int8, (70, 64)) in got[0]) == (checkpoint == "int8") and ((torch.float32, (70, 64)) in got[0]) == (checkpoint is None)

@@ -82,3 +82,21 @@ def test_parts_that_lie_otherwise():
         other.codes, other.scales = codes, scales
         with pytest.raises(ValueError, match="Packed4: codes of shape"):
             packed4.settled(other)
+
+
+def test_checkpoints_are_kept(monkeypatch):
+    """A layer that keeps z in 8 bits does so with its weight in 4."""
+    monkeypatch.setattr(matrix_linear, "pack4", lambda w: Packed4.from_parts(*po.pack(w.detach()), w.shape[1], w.dtype))
+    seen = []
+    for checkpoint in (None, "int8"):
+        layer = pkg.MatrixLinear(40, 72, activation="gelu", checkpoint=checkpoint)
+        for four in (layer.pack4(), copy.deepcopy(layer.pack4()), pkg.MatrixLinear4(layer.pack4().weight, layer.bias, "gelu", checkpoint=checkpoint)):
+            assert four.checkpoint == checkpoint
+            with monkeypatch.context() as m:
+                m.setattr(matrix_linear, "linear", lambda x, w, b, r, act, after, kept, axis: seen.append(kept))
+                four(torch.zeros(3, 40))
+            assert seen.pop() == checkpoint
+    with pytest.raises(ValueError, match="checkpoint"):
+        pkg.MatrixLinear4(_packed(), checkpoint="fp8")
+    stack = pkg.ResidualStack([pkg.residual.matrix_block(40, 64, checkpoint="int8")], 40).pack4()
+    assert [m.checkpoint for m in stack.blocks[0]] == ["int8", "int8"]
