@@ -14,6 +14,7 @@ of it is stored, and the same numbers give the same mask whatever the strides, t
 probability is the nearest multiple of 2^-16, and what is kept is divided by exactly the share that is.
 """
 import collections
+import copy
 import ctypes
 import math
 
@@ -399,8 +400,9 @@ def _may_run_again():
 
 
 class Dropout(nn.Module):
-    """Dropout whose mask is never stored.  Each pass in training counts the offset up; the seed is drawn from torch's generator where none is given, and both are in
-    the state dict.  counter=True keeps them on the GPU, in the buffer `state`, so that a captured pass draws another mask in every replay (two small launches more a pass).
+    """Dropout whose mask is never stored.  Each pass in training counts the offset up; the seed is drawn from torch's generator where none is given (and again for a
+    copy.deepcopy, whose masks are its own), and both are in the state dict.  counter=True keeps them on the GPU, in the buffer `state`, so that a captured pass draws another
+    mask in every replay (two small launches more a pass).
 
     A pass that torch.utils.checkpoint runs again in the backward pass takes the mask of its first run.  It is known by the state of torch's CPU generator, which checkpoint
     restores (preserve_rng_state) and from which passes without gradients or under saved-tensor hooks draw one number; in a backward pass a mask that is no earlier pass's, or
@@ -408,7 +410,8 @@ class Dropout(nn.Module):
 
     def __init__(self, p=0.5, per="element", seed=None, counter=False, channel_axis=-1, device=None):
         super().__init__()
-        seed = int(torch.randint(0, 1 << 62, (1,)).item()) if seed is None else seed
+        self.drawn = seed is None
+        seed = self._new_seed() if seed is None else seed
         Drop(p, seed, 0, per)
         self.p, self.per, self.channel_axis = p, per, channel_axis
         self._passes = {}                      # token of a pass: what it drew (None: one of several), whether it was run again
@@ -418,6 +421,10 @@ class Dropout(nn.Module):
             self.register_buffer("state", torch.tensor([seed, 0], dtype=torch.int64, device=device))
         else:
             self.state, self.seed, self.calls = None, seed, 0
+
+    @staticmethod
+    def _new_seed():
+        return int(torch.randint(0, 1 << 62, (1,)).item())
 
     def draw(self):
         """The Drop of the next pass; None where nothing is dropped."""
@@ -456,7 +463,17 @@ class Dropout(nn.Module):
         return {**self.__dict__, "_passes": {}}
 
     def __setstate__(self, state):
-        super().__setstate__({"_passes": {}, **state})
+        super().__setstate__({"_passes": {}, "drawn": False, **state})
+
+    def __deepcopy__(self, memo):
+        made = type(self).__new__(type(self))
+        memo[id(self)] = made
+        made.__setstate__(copy.deepcopy(self.__getstate__(), memo))
+        if made.drawn and made.state is not None:
+            made.state[0] = self._new_seed()
+        elif made.drawn:
+            made.seed = self._new_seed()
+        return made
 
     def get_extra_state(self):
         return None if self.state is not None else torch.tensor([self.seed - (1 << 64) if self.seed >> 63 else self.seed, self.calls])

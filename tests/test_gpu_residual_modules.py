@@ -1,4 +1,6 @@
 """Modules of joins and dropout in training: checkpointed, copied, in the forms that stacks of layers take."""
+import copy
+
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
@@ -71,3 +73,20 @@ def test_stacks_of_layers_packed(dev):
     # (the same values in 4 bits, fp32 sums of 72 and 136 products in another order)
     assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
     assert isinstance(stack.blocks[0], pkg.MatrixLinear4) and stack.blocks[2][0] is stack.blocks[2][1] is stack.blocks[0]
+
+
+@pytest.mark.parametrize("counter", [False, True])
+def test_copies_draw_their_own_masks(dev, counter):
+    """Blocks that are copies of one another, as stacks are often made."""
+    torch.manual_seed(6)
+    m = pkg.Dropout(0.5, counter=counter).cuda()
+    x = torch.ones(50, 64, device=dev)
+    layers = [m] + [copy.deepcopy(m) for _ in range(3)]
+    masks = [layer(x) != 0 for layer in layers]
+    for i in range(4):
+        for j in range(i):
+            # (800 of 3200, six deviations of 24.5)
+            assert abs(int((masks[i] & masks[j]).sum()) - 800) < 147
+    other = pkg.Dropout(0.5, counter=counter).cuda()
+    other.load_state_dict(layers[2].state_dict())
+    assert torch.equal(other(x), layers[2](x))

@@ -181,3 +181,33 @@ def test_every_layer_of_a_stack_is_packed(pack_on_cpu):
         assert b[0] is b[4] and b[2] is b[6] and b[2][0] is b[2][2] is b[3] and b[3] is not b[0] and isinstance(b[5][1], torch.nn.Linear)
         for i, layer in ((0, once), (3, shared)):
             assert torch.equal(b[i].weight.parts()[0], po.pack(layer.weight.detach())[0])
+
+
+@pytest.mark.parametrize("counter", [False, True])
+def test_copies_draw_their_own_masks(definition, counter):
+    """Unless a seed was given; a state dict, and a module saved whole, go on with the masks of the module that they are from."""
+    torch.manual_seed(0)
+    x = torch.ones(50, 64)
+    m = pkg.Dropout(0.5, counter=counter)
+    m(x)
+    copies = [copy.deepcopy(m) for _ in range(2)]
+    buffer = io.BytesIO()
+    torch.save(m, buffer)
+    buffer.seek(0)
+    whole, loaded = torch.load(buffer, weights_only=False), pkg.Dropout(0.5, counter=counter)
+    loaded.load_state_dict(m.state_dict())
+    state = [copy.deepcopy(c.state_dict()) for c in copies]
+    masks = [v(x) != 0 for v in [m] + copies]
+    # (of 3200 values in halves, kept in both: 800, six deviations of 24.5)
+    for a, b in ((0, 1), (0, 2), (1, 2)):
+        assert abs(int((masks[a] & masks[b]).sum()) - 800) < 147
+    assert torch.equal(whole(x) != 0, masks[0]) and torch.equal(loaded(x) != 0, masks[0])
+    for c, mask in zip(state, masks[1:]):
+        again = pkg.Dropout(0.5, counter=counter)
+        again.load_state_dict(c)
+        assert torch.equal(again(x) != 0, mask)
+    # copies of copies, and one of the copies by itself in a larger module
+    layers = copy.deepcopy(torch.nn.ModuleList([copies[0]] * 2 + [copies[1]]))
+    assert layers[0] is layers[1] and not torch.equal(layers[0](x), layers[2](x))
+    given = pkg.Dropout(0.5, seed=9, counter=counter)
+    assert torch.equal(copy.deepcopy(given)(x), given(x))
