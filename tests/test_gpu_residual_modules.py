@@ -8,6 +8,8 @@ from torch.utils.checkpoint import checkpoint
 import pytorch_winoconv_amd as pkg
 from pytorch_winoconv_amd import residual
 
+import residual_oracle as ro
+
 pytestmark = pytest.mark.gpu
 
 
@@ -90,3 +92,20 @@ def test_copies_draw_their_own_masks(dev, counter):
     other = pkg.Dropout(0.5, counter=counter).cuda()
     other.load_state_dict(layers[2].state_dict())
     assert torch.equal(other(x), layers[2](x))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,C", [(5000, 4104), (17000, 523), (600, 70001)])
+def test_masks_of_rows_in_pieces(dev, rows, C, t):
+    """Joins without a norm, whose rows are taken in pieces by fewer workgroups than there are rows: the first, the middle and the last rows' masks bit for bit, all channels of them."""
+    level, seed, offset = 16384, 11, 1 << 40 | 12
+    f = torch.randn(rows, C, device=dev).to(t).abs() + 0.25
+    x, drop = torch.randn(rows, C, device=dev).to(t), residual.Drop(0.25, seed, offset)
+    out = residual.dropout_forward(f, drop)
+    s = residual.join_forward(f, x, drop=drop, stream_scale=0.0)[0]
+    df = residual.join_backward(f, None, None, None, None, drop=drop, need_stream=False).block
+    for first in (0, 2047, rows // 2 + 1, rows - 6):
+        first = min(first, rows - 6)
+        kept = (ro.words(6, C, seed, offset, first)[:, :C] >= level).to(dev)
+        for v in (out, s, df):
+            assert torch.equal(v[first:first + 6] != 0, kept)
