@@ -244,6 +244,12 @@ class LinearFunction(torch.autograd.Function):
         return dx, dw, db, dy if need_r and residual_after else dz, None, None, None
 
 
+def _refuse_tangents(given):
+    # (asked of torch for each tensor only within a level of forward mode: 3 us)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise NotImplementedError("linear has no forward-mode derivative: a tangent of its operands would be lost")
+
+
 def linear(x, w, bias=None, residual=None, activation="none", residual_after=False, checkpoint=None, channel_axis=-1):
     """linear_forward with gradients.  checkpoint="int8" keeps x and z in 8 bits for the backward pass (checkpoint8); relu's gate
     stays z's own, so that of its gradients the weight's alone differs.  channel_axis: the axis of the channels in x and the residual, so that 1 takes the (N, C, H, W) tensors of the convolutions; a
@@ -256,6 +262,7 @@ def linear(x, w, bias=None, residual=None, activation="none", residual_after=Fal
             raise ValueError("linear: channel_axis %r of an x in 4 bits, whose channels are last" % (channel_axis,))
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual)):
             raise NotImplementedError("linear: no gradient passes a layer whose x is in 4 bits")
+        _refuse_tangents((bias, residual))
         return linear_forward(x, w, bias, residual, activation, residual_after)
     if channel_axis not in (-1, x.dim() - 1):
         if residual is not None and residual.dim() != x.dim():
@@ -264,9 +271,7 @@ def linear(x, w, bias=None, residual=None, activation="none", residual_after=Fal
         residual = None if residual is None else residual.movedim(channel_axis, -1)
         return linear(x, w, bias, residual, activation, residual_after, checkpoint).movedim(-1, channel_axis)
     given = [t for t in (x, w, bias, residual) if t is not None and not isinstance(t, Packed4)]
-    # (asked of torch for each tensor only within a level of forward mode: 3 us)
-    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
-        raise NotImplementedError("linear has no forward-mode derivative: a tangent of its operands would be lost")
+    _refuse_tangents(given)
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return LinearFunction.apply(x, w, bias, residual, activation, bool(residual_after), checkpoint)
     own = lambda t: t if t is None or isinstance(t, Packed4) or t.dtype == x.dtype else t.to(x.dtype)  # noqa: E731
@@ -354,6 +359,7 @@ class MatrixLinear4(nn.Module):
             return linear(x, w, self.bias, residual, self.activation, self.residual_after, self.checkpoint, self.channel_axis)
         if torch.is_grad_enabled() and x.requires_grad:
             raise NotImplementedError("MatrixLinear4: no gradient passes a layer that puts its inputs into 4 bits")
+        _refuse_tangents((x,))
         axis = self.channel_axis
         if axis not in (-1, x.dim() - 1):
             return self._last(x.movedim(axis, -1), w, None if residual is None else residual.movedim(axis, -1)).movedim(-1, axis)

@@ -4,6 +4,7 @@ import io
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import pytorch_winoconv_amd as pkg
 from pytorch_winoconv_amd import matrix_linear, packed4
@@ -100,3 +101,22 @@ def test_checkpoints_are_kept(monkeypatch):
         pkg.MatrixLinear4(_packed(), checkpoint="fp8")
     stack = pkg.ResidualStack([pkg.residual.matrix_block(40, 64, checkpoint="int8")], 40).pack4()
     assert [m.checkpoint for m in stack.blocks[0]] == ["int8", "int8"]
+
+
+@pytest.mark.parametrize("which", ["x", "bias", "residual"])
+def test_forward_mode_is_refused(monkeypatch, which):
+    """Also where x is in 4 bits, or put into them by the layer: a tangent would be lost."""
+    monkeypatch.setattr(matrix_linear, "pack4", lambda x: Packed4.from_parts(*po.pack(x.detach()), x.shape[1], x.dtype))
+    w = _packed(70, 300, torch.float32)
+    layer = pkg.MatrixLinear4(w, torch.zeros(70), x4=True)
+    with forward_ad.dual_level():
+        ts = {"x": torch.randn(3, 300), "bias": torch.zeros(70), "residual": torch.zeros(3, 70)}
+        ts[which] = forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                if which != "bias":
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        layer(ts["x"], ts["residual"])
+                if which != "x":
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        matrix_linear.linear(_packed(3, 300, torch.float32), w, ts["bias"], ts["residual"])
