@@ -47,7 +47,7 @@ template <int WM_, int WN_, int NWM_, int NWN_> struct Shape4 {
 constexpr int kBand4 = 8;
 
 template <typename T, typename SH>
-__global__ __launch_bounds__(64 * SH::NW, SH::WM * SH::WN == 16 ? 1 : 2) void product4_dma_kernel(Dma4Args g) {
+__global__ __launch_bounds__(64 * SH::NW, 2) void product4_dma_kernel(Dma4Args g) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   constexpr int WM = SH::WM, WN = SH::WN, NWM = SH::NWM, NWN = SH::NWN, BM = SH::BM, BN = SH::BN, NW = SH::NW;
   using E = half_t;           // what an element of 16 bits is called
@@ -174,17 +174,10 @@ __global__ __launch_bounds__(64 * SH::NW, SH::WM * SH::WN == 16 ? 1 : 2) void pr
   }
   __syncthreads();                                          // the buffers are done with
   float* const stage = reinterpret_cast<float*>(lds) + wave * 32 * (WN * 32 + 4);
-  auto finish = [&](auto act) {
+  with_activation(p.e.act, [&](auto act) {
     if (m0 + BM <= p.M && n0 + BN <= p.N) finish_blocks<T, act(), true, true, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
     else finish_blocks<T, act(), false, true, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
-  };
-  switch (p.e.act) {
-    case WC_ACT_RELU: finish(ic<WC_ACT_RELU>{}); break;
-    case WC_ACT_GELU: finish(ic<WC_ACT_GELU>{}); break;
-    case WC_ACT_GELU_TANH: finish(ic<WC_ACT_GELU_TANH>{}); break;
-    case WC_ACT_SILU: finish(ic<WC_ACT_SILU>{}); break;
-    default: finish(ic<WC_ACT_NONE>{});
-  }
+  });
 }
 
 using Tile256 = Shape4<4, 2, 2, 4>;

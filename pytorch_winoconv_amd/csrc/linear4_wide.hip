@@ -150,17 +150,10 @@ __global__ __launch_bounds__(64 * SH::NW, SH::NW / 4) void linear4_wide_kernel(W
   }
   __syncthreads();                                           // the ring is done with
   float* const stage = reinterpret_cast<float*>(lds) + wave * 32 * (WN * 32 + 4);
-  auto finish = [&](auto act) {
+  with_activation(p.e.act, [&](auto act) {
     if (m0 + BM <= p.M && n0 + BN <= p.N) finish_blocks<T, act(), true, true, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
     else finish_blocks<T, act(), false, true, WM, WN>(p.e, acc, stage, wm0, p.M, (int)wn0, p.N, lane);
-  };
-  switch (p.e.act) {
-    case WC_ACT_RELU: finish(ic<WC_ACT_RELU>{}); break;
-    case WC_ACT_GELU: finish(ic<WC_ACT_GELU>{}); break;
-    case WC_ACT_GELU_TANH: finish(ic<WC_ACT_GELU_TANH>{}); break;
-    case WC_ACT_SILU: finish(ic<WC_ACT_SILU>{}); break;
-    default: finish(ic<WC_ACT_NONE>{});
-  }
+  });
 }
 
 using Wide64 = ShapeWide<2, 1, 1, 4, 4>;          // 64 x 128, 97 KB

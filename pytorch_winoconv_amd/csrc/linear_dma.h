@@ -219,6 +219,18 @@ __device__ __forceinline__ void finish_blocks(const LinearEpilogue& e, const f32
   }
 }
 
+// run(ic<act>), the activation a constant of its instructions
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& run) {
+  switch (act) {
+    case WC_ACT_RELU: run(ic<WC_ACT_RELU>{}); break;
+    case WC_ACT_GELU: run(ic<WC_ACT_GELU>{}); break;
+    case WC_ACT_GELU_TANH: run(ic<WC_ACT_GELU_TANH>{}); break;
+    case WC_ACT_SILU: run(ic<WC_ACT_SILU>{}); break;
+    default: run(ic<WC_ACT_NONE>{});
+  }
+}
+
 // A wavefront's blocks to a part's sums (M, N).  Register 4 q + e of a lane: row l32, column 8 q + 4 lhi + e of the block.  vec: rows are multiples of 16 bytes; of others
 // sixteen bytes start at any float (us, the call of fp16 299 x 9352 -> 1745 over a weight in 4 bits, float by float 44, so 33; over one in 16 bits 46 | 36)
 template <int WM, int WN>

@@ -212,15 +212,7 @@ __device__ __forceinline__ void product_block(const DmaArgs& g, int hw_block, un
   };
   // (a gradient has no epilogue, and the largest tiles, whose epilogue nothing runs beside, are left to products without a heavy one)
   if constexpr (BO || AHEAD) finish(ic<WC_ACT_NONE>{}, std::false_type{});
-  else {
-    switch (p.e.act) {
-      case WC_ACT_RELU: finish(ic<WC_ACT_RELU>{}, std::true_type{}); break;
-      case WC_ACT_GELU: finish(ic<WC_ACT_GELU>{}, std::true_type{}); break;
-      case WC_ACT_GELU_TANH: finish(ic<WC_ACT_GELU_TANH>{}, std::true_type{}); break;
-      case WC_ACT_SILU: finish(ic<WC_ACT_SILU>{}, std::true_type{}); break;
-      default: finish(ic<WC_ACT_NONE>{}, std::true_type{});
-    }
-  }
+  else with_activation(p.e.act, [&](auto act) { finish(act, std::true_type{}); });
 }
 
 template <typename SH> constexpr int kMinWaves = SH::AHEAD ? 1 : 2;
