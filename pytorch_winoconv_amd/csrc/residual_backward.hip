@@ -9,7 +9,7 @@ namespace wc {
 // Vectors of a thread, wavefronts and lanes of a team of a backward pass; vectors 0: long rows.  One vector a thread up to 8192 channels: the sums and the row
 // that is on its way leave no registers for more.  Two, of 16 wavefronts with 128 registers a thread, hold a norm alone and what goes through no norm; the rest spills
 // and is left to the passes of long rows (us, in registers | long: 2048 x 16384 bf16 with two norms, gate and dropout 591 | 457; a norm alone 4096 x 16384
-// 109 | 225, 4096 x 12001 120 | 282; 2048 x 8001 with two norms, gate and dropout, one vector, 163 | 360)
+// 109 | 225, 4096 x 12001 120 | 282; 2048 x 8001 with two norms, gate and dropout, one vector, 147 | 360)
 TeamShape back_shape(const JoinGradients& g) {
   const int vectors = ceil_div(g.C, 8);
   if (vectors <= 64) {
