@@ -1518,6 +1518,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack8", &pack8, py::arg("x"), py::arg("keep_sign"));
   m.def("unpack8", &unpack8, py::arg("codes"), py::arg("exponents"), py::arg("type"));
   m.def("pack4", &pack4, py::arg("x"));
+  m.def("packed4_fits", &packed4_fits);
   m.def("unpack4", &unpack4, py::arg("codes"), py::arg("scales"), py::arg("C"), py::arg("type"));
   m.def("linear4_forward", &linear4_forward, py::arg("x"), py::arg("x_codes"), py::arg("x_scales"), py::arg("type"), py::arg("w_codes"), py::arg("w_scales"),
         py::arg("C"), py::arg("bias"), py::arg("residual"), py::arg("activation"), py::arg("residual_after"), py::arg("keep_z"));

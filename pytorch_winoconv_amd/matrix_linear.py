@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, engine
 from ._lib import LinearDesc, LinearGradients, check
 from .checkpoint8 import Packed8, check_channels, pack8, pack_gates
-from .packed4 import ROWS as ROWS4, Packed4, _made as _made4, linear4_ext, linear4_forward, pack4, settled as settled4
+from .packed4 import Packed4, _made as _made4, four_axes, linear4_ext, linear4_forward, pack4, settled as settled4
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -343,18 +343,14 @@ class MatrixLinear4(nn.Module):
             state_dict[prefix + "scales"] = scales.flatten(2)
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
-    def _parts(self):
-        """The buffers as a Packed4's; where they do not lie as the kernels read them, the layer's calls copy them."""
-        blocks, stages = self.scales.shape[:2]
-        return self.codes, self.scales.reshape(blocks, stages, ROWS4, 4), self.in_features, self.dtype
-
     @property
     def weight(self):
         """The Packed4 of the buffers as they are now."""
-        return Packed4(*self._parts())
+        return Packed4(self.codes, four_axes(self.scales), self.in_features, self.dtype)
 
     def forward(self, x, residual=None):
-        w = _made4(*self._parts())
+        # (the kernels read the scales whatever their axes; where the buffers do not lie as they read them, the calls copy)
+        w = _made4(self.codes, self.scales, self.in_features, self.dtype)
         if not self.x4:
             return linear(x, w, self.bias, residual, self.activation, self.residual_after, self.checkpoint, self.channel_axis)
         if torch.is_grad_enabled() and x.requires_grad:

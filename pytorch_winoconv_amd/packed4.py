@@ -101,18 +101,25 @@ def _made(codes, scales, channels, dtype):
     return p
 
 
+def four_axes(scales):
+    """The scales of a Packed4, of which a module's buffer has the last two axes in one."""
+    return scales.unflatten(2, (ROWS, 4)) if scales.dim() == 3 else scales
+
+
 def _belong(p):
     """Whether codes and scales lie as the kernels read them: whole, one after the other, from multiples of 16 bytes."""
     codes, scales = p.codes, p.scales
+    if engine.USE_EXT and codes.is_cuda:
+        return engine._ext.packed4_fits(codes, scales, p.channels)
     stages = -(-p.channels // STAGE)
     return (codes.is_contiguous() and scales.is_contiguous() and not engine.misaligned(codes, scales) and codes.dtype == scales.dtype == torch.uint8
-            and codes.device == scales.device and codes.shape[-1] == 64 * stages and tuple(scales.shape) == (-(-_rows(codes.shape) // ROWS), stages, ROWS, 4))
+            and codes.device == scales.device and codes.shape[-1] == 64 * stages and scales.numel() == -(-_rows(codes.shape) // ROWS) * stages * ROWS * 4)
 
 
 def settled(p):
     """A Packed4 whose parts the kernels may read: p as it is, or its parts copied where they lie otherwise (a module's buffers take other strides and starts
     when it is moved or loaded); parts that are not each other's are refused."""
-    return p if _belong(p) else Packed4(p.codes, p.scales, p.channels, p.dtype)
+    return p if _belong(p) else Packed4(p.codes, four_axes(p.scales), p.channels, p.dtype)
 
 
 def pack4(x):

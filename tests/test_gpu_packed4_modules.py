@@ -66,9 +66,9 @@ def test_checkpoints_are_kept(dev, checkpoint):
     def kept(call):
         held = []
         leaf = x.clone().requires_grad_()
-        with torch.autograd.graph.saved_tensors_hooks(lambda v: (held.append((v.dtype, tuple(v.shape))), v)[1], lambda v: v):
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: (held.append((v.dtype, v.numel())), v)[1], lambda v: v):
             y = call(leaf)
         return held, torch.autograd.grad(y.sum(), leaf)[0]
     got, want = kept(four), kept(lambda v: matrix_linear.linear(v, four.weight, four.bias, None, "gelu", checkpoint=checkpoint))
     assert got[0] == want[0] and torch.equal(got[1], want[1])
-    assert ((torch.int8, (70, 64)) in got[0]) == (checkpoint == "int8") and ((torch.float32, (70, 64)) in got[0]) == (checkpoint is None)
+    assert ((torch.int8, 70 * 64) in got[0]) == (checkpoint == "int8") and ((torch.float32, 70 * 64) in got[0]) == (checkpoint is None)
